@@ -1,0 +1,486 @@
+"""The sequence operators as they are used next to a vectorised task: one pass of each, in a plain form made of
+elementary torch operations in 32 bits and through the framework's own calls, on the same inputs.
+
+A policy with a recurrent core trains on rollouts [T, N, D] - time, environment, channel - whose episodes begin where
+the step kernels raised the reset flag.  The operators are the gated linear recurrence over such a rollout (training,
+one step of a running policy, the discounted sums behind advantages), the norms before and after the policy's blocks
+with the branch's gate and residual scale, and the 8-bit checkpoints that keep the blocks' activations for the
+backward pass.
+"""
+import math
+
+import torch
+
+own = False
+
+DEVICE = "cuda"
+GROUP = 64            # elements that share one scale of an 8-bit checkpoint
+SMALLEST = 2.0 ** -120  # a group whose largest magnitude is below this is stored as zeros
+EPS = 1e-5
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+SIZES = {"f32": 4, "bf16": 2, "f16": 2}
+
+
+def listed():
+    return [
+        # a policy answers one step of 4 096 environments (the tasks' default): the state is advanced, latency counts
+        dict(name="step_4096x64_f32", op="step", dtype="f32", N=4096, D=64, resets=0.002),
+        # the same at 2^18 environments in bf16
+        dict(name="step_262144x64_bf16", op="step", dtype="bf16", N=262144, D=64, resets=0.002),
+        # training on one horizon of the default number of environments, episodes ending inside it
+        dict(name="rec_train_32x4096x64_f32", op="recurrence", train=True, dtype="f32", T=32, N=4096, D=64, resets=0.03,
+             reverse=False, batch_first=False, discount=False),
+        # training on a large rollout in bf16
+        dict(name="rec_train_32x65536x64_bf16", op="recurrence", train=True, dtype="bf16", T=32, N=65536, D=64,
+             resets=0.03, reverse=False, batch_first=False, discount=False),
+        # one long recorded trajectory, wide state: the work has to be split over time
+        dict(name="rec_train_8192x1x512_bf16", op="recurrence", train=True, dtype="bf16", T=8192, N=1, D=512,
+             resets=0.001, reverse=False, batch_first=False, discount=False),
+        # whole episodes (1 000 steps) of an odd number of environments, odd width, stored environment by environment
+        dict(name="rec_train_1000x37x105_f16", op="recurrence", train=True, dtype="f16", T=1000, N=37, D=105,
+             resets=0.002, reverse=False, batch_first=True, discount=False),
+        # advantages: the discounted sum of temporal differences backwards in time, one channel per environment
+        dict(name="rec_returns_32x262144_f32", op="recurrence", train=False, dtype="f32", T=32, N=262144, D=1,
+             resets=0.01, reverse=True, batch_first=False, discount=True),
+        # the norm in front of a block for one step of the default number of environments
+        dict(name="norm_4096x64_f32", op="norm", train=False, dtype="f32", R=4096, D=64, checkpoint=False),
+        # training: odd rows of 211 features
+        dict(name="residual_train_16411x211_f32", op="residual", train=True, dtype="f32", R=16411, D=211, gate=True,
+             scale=True, next=True, activation="sigmoid", checkpoint=False),
+        # training: the largest, a rollout of 32 x 32 768 steps
+        dict(name="residual_train_1048576x256_bf16", op="residual", train=True, dtype="bf16", R=1 << 20, D=256, gate=True,
+             scale=True, next=True, activation="silu", checkpoint=False),
+        # training with the block's output and gate kept in 8 bits
+        dict(name="residual_train8_131072x512_bf16", op="residual", train=True, dtype="bf16", R=131072, D=512, gate=True,
+             scale=True, next=True, activation="silu", checkpoint=True),
+        # activations of 2^17 steps packed for the backward pass and unpacked there
+        dict(name="pack_131072x105_f32", op="pack", dtype="f32", R=131072, D=105),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["step", "recurrence", "recurrence", "recurrence", "norm", "residual", "residual", "pack"])
+    dtype = rng.choice(["f32", "bf16", "f16"])
+    if op == "step":
+        d = _log_int(rng, 1, 1024)
+        return dict(op=op, dtype=dtype, N=_log_int(rng, 1, min(1 << 20, (1 << 26) // d)), D=d,
+                    resets=rng.choice([0.0, 0.01, 0.3]))
+    if op == "recurrence":
+        discount = rng.random() < 0.2
+        d = 1 if discount else _log_int(rng, 1, 1024)
+        t = _log_int(rng, 1, 16384)
+        n = _log_int(rng, 1, max(1, min(1 << 18, (1 << 26) // (t * d))))
+        return dict(op=op, train=not discount and rng.random() < 0.7, dtype="f32" if discount else dtype, T=t, N=n, D=d,
+                    resets=rng.choice([0.0, 1.0 / t, 0.1]), reverse=discount or rng.random() < 0.3,
+                    batch_first=not discount and rng.random() < 0.3, discount=discount)
+    d = _log_int(rng, 1, 4096)
+    r = _log_int(rng, 1, min(1 << 20, (1 << 27) // d))
+    if op == "pack":
+        return dict(op=op, dtype=dtype, R=r, D=d)
+    train = rng.random() < 0.7
+    checkpoint = train and rng.random() < 0.4
+    if op == "norm":
+        return dict(op=op, train=train, dtype=dtype, R=r, D=d, checkpoint=checkpoint)
+    return dict(op=op, train=train, dtype=dtype, R=r, D=d, gate=rng.random() < 0.7, scale=rng.random() < 0.7,
+                next=rng.random() < 0.6, activation=rng.choice(["silu", "sigmoid", "none"]), checkpoint=checkpoint)
+
+
+def work(case):
+    e = SIZES[case["dtype"]]
+    op = case["op"]
+    if op == "step":
+        n = case["N"] * case["D"]
+        return {"bytes": n * (3 * e + 8) + 8 * case["N"], "flops": 2 * n}
+    if op == "recurrence":
+        c = case["N"] * case["D"]
+        n = case["T"] * c
+        flags = 8 * case["T"] * case["N"]
+        gate = 4 if case["discount"] else n * e
+        if case["train"]:  # in: gate, input, d out, state, d last; out: out, last, d gate, d input, d state
+            return {"bytes": 6 * n * e + flags + 16 * c, "flops": 5 * n}
+        return {"bytes": gate + 2 * n * e + flags + 8 * c, "flops": 2 * n}
+    n = case["R"] * case["D"]
+    w = 4 * case["D"]
+    if op == "pack":  # read, written as codes and scales, read again, written decoded
+        return {"bytes": n * (2 * e + 2) + 8 * case["R"] * -(-case["D"] // GROUP), "flops": 4 * n}
+    if op == "norm":
+        return {"bytes": (4 if case["train"] else 2) * n * e + (2 if case["train"] else 1) * w,
+                "flops": (12 if case["train"] else 4) * n}
+    arrays = 3 + case["gate"] + case["next"]
+    params = 1 + case["scale"] + case["next"]
+    if case["train"]:
+        arrays += 3 + case["gate"] + case["next"]
+        params *= 2
+    return {"bytes": arrays * n * e + params * w, "flops": (40 if case["train"] else 14) * n}
+
+
+# ---- inputs ---------------------------------------------------------------------------------------------------
+
+def prepare(case, seed):
+    gen = torch.Generator(device=DEVICE)
+    gen.manual_seed(seed)
+    dt = TYPES[case["dtype"]]
+    op = case["op"]
+
+    def normal(*shape, dtype=dt, scale=1.0, shift=0.0):
+        x = torch.randn(*shape, generator=gen, device=DEVICE)
+        return x.mul_(scale).add_(shift).to(dtype)
+
+    def gates(*shape):  # a forget gate after its sigmoid, most of it near one
+        x = torch.randn(*shape, generator=gen, device=DEVICE)
+        return x.mul_(1.5).add_(2.0).sigmoid_().to(dt)
+
+    def flags(*shape):
+        return (torch.rand(*shape, generator=gen, device=DEVICE) < case["resets"]).to(torch.int64)
+
+    s = {"case": case}
+    if op == "step":
+        n, d = case["N"], case["D"]
+        s.update(gate=gates(n, d), inp=normal(n, d, scale=0.5), state=normal(n, d, dtype=torch.float32), reset=flags(n),
+                 state_out=torch.empty(n, d, device=DEVICE))
+        return s
+    if op == "recurrence":
+        t, n, d = case["T"], case["N"], case["D"]
+
+        def rollout(make, **kw):
+            return make(n, t, d, **kw).transpose(0, 1) if case["batch_first"] else make(t, n, d, **kw)
+
+        if case["discount"]:  # gamma * lambda; the temporal differences
+            s["gate"] = torch.full((1, 1, 1), 0.99 * 0.95, dtype=dt, device=DEVICE).expand(t, n, d)
+        else:
+            s["gate"] = rollout(gates)
+        s.update(inp=rollout(normal, scale=0.5), state=normal(n, d, dtype=torch.float32), reset=flags(t, n))
+        if case["train"]:
+            s.update(d_out=rollout(normal), d_last=normal(n, d, dtype=torch.float32))
+            for k in ("gate", "inp", "state"):
+                s[k].requires_grad_(True)
+        return s
+    r, d = case["R"], case["D"]
+    s["x"] = normal(r, d)
+    if op == "pack":
+        return s
+    s["weight"] = normal(d, dtype=torch.float32, scale=0.1, shift=1.0)
+    if op == "residual":
+        s["y"] = normal(r, d, scale=2.0)
+        s["gate"] = normal(r, d) if case["gate"] else None
+        s["scale"] = normal(d, dtype=torch.float32, scale=0.05, shift=0.5) if case["scale"] else None
+        s["next_weight"] = normal(d, dtype=torch.float32, scale=0.1, shift=1.0) if case["next"] else None
+    if case["train"]:
+        s["d_out"] = normal(r, d)
+        if op == "residual" and case["next"]:
+            s["d_next"] = normal(r, d)
+        for k in _leaves(case):
+            s[k].requires_grad_(True)
+    return s
+
+
+def _leaves(case):
+    if case["op"] == "norm":
+        return ["x", "weight"]
+    return (["x", "y", "weight"] + (["gate"] if case["gate"] else []) + (["scale"] if case["scale"] else []) +
+            (["next_weight"] if case["next"] else []))
+
+
+# ---- one pass ---------------------------------------------------------------------------------------------------
+
+def run(state):
+    if own:
+        return _run_own(state)
+    with torch.no_grad():
+        return _run_plain(state)
+
+
+def _run_own(s):
+    from isaacgym_amd import sequence
+
+    case = s["case"]
+    op = case["op"]
+    if op == "step":
+        out = sequence.linear_recurrence_step(s["gate"], s["inp"], s["state"], reset=s["reset"], state_out=s["state_out"])
+        return [out, s["state_out"]]
+    if op == "recurrence":
+        out, last = sequence.linear_recurrence(s["gate"], s["inp"], state=s["state"], reset=s["reset"],
+                                               reverse=case["reverse"])
+        if not case["train"]:
+            return [out, last]
+        grads = torch.autograd.grad((out, last), (s["gate"], s["inp"], s["state"]), (s["d_out"], s["d_last"]))
+        return [out.detach(), last.detach(), *grads]
+    if op == "pack":
+        return [sequence.unpack8(*sequence.pack8(s["x"]), dtype=s["x"].dtype)]
+    if op == "norm":
+        out = sequence.rms_norm(s["x"], s["weight"], eps=EPS, checkpoint=case["checkpoint"])
+        outs, heads = (out,), (s.get("d_out"),)
+    else:
+        outs = sequence.residual_norm(s["x"], s["y"], s["weight"], gate=s["gate"], scale=s["scale"],
+                                      next_weight=s["next_weight"], activation=case["activation"], eps=EPS,
+                                      checkpoint=case["checkpoint"])
+        outs = outs if case["next"] else (outs,)
+        heads = (s.get("d_out"), s.get("d_next"))[:len(outs)]
+    if not case["train"]:
+        return list(outs)
+    grads = torch.autograd.grad(outs, [s[k] for k in _leaves(case)], heads)
+    return [o.detach() for o in outs] + list(grads)
+
+
+def _scan(gate, add, state):
+    """h[t] = gate[t] * h[t - 1] + add[t] over [T, N, D] in the inputs' type: step by step over few steps, by doubling
+    over many."""
+    t = add.shape[0]
+    h = add.clone()
+    h[0] += gate[0] * state
+    if t <= 64:
+        for i in range(1, t):
+            h[i] += gate[i] * h[i - 1]
+        return h
+    a = gate.expand_as(add).clone()
+    k = 1
+    while k < t:
+        h = torch.cat((h[:k], h[k:] + a[k:] * h[:-k]))
+        a = torch.cat((a[:k], a[k:] * a[:-k]))
+        k *= 2
+    return h
+
+
+def _act(z, kind):
+    """The gate's activation and its derivative."""
+    if kind == "none":
+        return z, torch.ones_like(z)
+    p = 1 / (1 + torch.exp(-z))
+    if kind == "sigmoid":
+        return p, p * (1 - p)
+    return z * p, p * (1 + z * (1 - p))
+
+
+def _codes(x):
+    """The 8-bit codes of x [R, D] in groups of 64 along a row, and their scales: the operator's definition, given in
+    32-bit steps (largest magnitude, 127 / largest, product, nearest integer with ties to even)."""
+    r, d = x.shape
+    g = torch.nn.functional.pad(x.float(), (0, -d % GROUP)).reshape(r, -1, GROUP)
+    top = g.abs().amax(-1, keepdim=True)
+    tiny = top < SMALLEST
+    full = torch.full_like(top, 127.0)  # tensors on both sides: torch turns a quotient with a number into a product
+    inverse = torch.where(tiny, torch.zeros_like(top), full / top)
+    scale = torch.where(tiny, torch.zeros_like(top), top / full)
+    return torch.round(g * inverse), scale
+
+
+def _through8(x):
+    """x as the backward pass sees it after its 8-bit checkpoint."""
+    q, scale = _codes(x)
+    return (q * scale).reshape(x.shape[0], -1)[:, :x.shape[1]]
+
+
+def _run_plain(s):
+    case = s["case"]
+    op = case["op"]
+    dt = TYPES[case["dtype"]]
+    if op == "step":
+        first = (s["reset"] != 0)[:, None]
+        carried = torch.where(first, torch.zeros_like(s["state"]), s["gate"].float() * s["state"])
+        h = carried + s["inp"].float()
+        return [h.to(dt), h]
+    if op == "recurrence":
+        return _plain_recurrence(s, case, dt)
+    if op == "pack":
+        return [_through8(s["x"]).to(dt)]
+    return _plain_norms(s, case, dt)
+
+
+def _plain_recurrence(s, case, dt):
+    keep = (s["reset"] == 0)[:, :, None]
+    gate, add = s["gate"].float(), s["inp"].float()
+    gate = torch.where(keep, gate, torch.zeros_like(gate[:1, :1, :1]))
+    if case["reverse"]:
+        gate, add = gate.flip(0), add.flip(0)
+    h = _scan(gate, add, s["state"])
+    out = h.flip(0) if case["reverse"] else h
+    if not case["train"]:
+        return [out.to(dt), h[-1].clone()]
+    d_out = s["d_out"].float()
+    if case["reverse"]:
+        d_out = d_out.flip(0)
+    # dh[t] = d_out[t] + gate[t + 1] dh[t + 1]: the same recurrence backwards, one step later's gate
+    later = torch.cat((gate[1:], torch.ones_like(gate[:1])))
+    d_inp = _scan(later.flip(0), d_out.flip(0), s["d_last"]).flip(0)
+    before = torch.cat((s["state"][None], h[:-1]))
+    kept = keep.flip(0) if case["reverse"] else keep
+    d_gate = torch.where(kept, d_inp * before, torch.zeros_like(before))
+    d_state = gate[0] * d_inp[0]
+    if case["reverse"]:
+        d_gate, d_inp = d_gate.flip(0), d_inp.flip(0)
+    return [out.to(dt), h[-1].clone(), d_gate.to(dt), d_inp.to(dt), d_state]
+
+
+def _rms(x):
+    return torch.rsqrt((x * x).mean(-1, keepdim=True) + EPS)
+
+
+def _rms_backward(d_normed, x, inverse, weight):
+    """d x and d weight of x * inverse * weight, inverse being the row's 1 / rms."""
+    unit = x * inverse
+    d_unit = d_normed * weight
+    return inverse * (d_unit - unit * (d_unit * unit).mean(-1, keepdim=True)), (d_normed * unit).sum(0)
+
+
+def _plain_norms(s, case, dt):
+    x = s["x"].float()
+    if case["op"] == "norm":
+        inverse = _rms(x)
+        out = x * inverse * s["weight"]
+        if not case["train"]:
+            return [out.to(dt)]
+        seen = _through8(s["x"]) if case["checkpoint"] else x
+        d_x, d_w = _rms_backward(s["d_out"].float(), seen, inverse, s["weight"])
+        return [out.to(dt), d_x.to(dt), d_w]
+    y = s["y"].float()
+    one = torch.ones((), device=x.device)
+    scale = s["scale"] if case["scale"] else one
+    gate, _ = _act(s["gate"].float(), case["activation"]) if case["gate"] else (one, None)
+    inverse = _rms(y)
+    out = x + scale * gate * (y * inverse * s["weight"])
+    outs = [out.to(dt)]
+    if case["next"]:
+        inverse_next = _rms(out)
+        outs.append((out * inverse_next * s["next_weight"]).to(dt))
+    if not case["train"]:
+        return outs
+    slope = None
+    if case["gate"]:
+        gate, slope = _act(_through8(s["gate"]) if case["checkpoint"] else s["gate"].float(), case["activation"])
+    if case["checkpoint"]:
+        y = _through8(s["y"])
+        out = x + scale * gate * (y * inverse * s["weight"])
+    d_out = s["d_out"].float()
+    grads = {}
+    if case["next"]:
+        through, grads["next_weight"] = _rms_backward(s["d_next"].float(), out, inverse_next, s["next_weight"])
+        d_out = d_out + through
+    normed = y * inverse * s["weight"]
+    grads["x"] = d_out.to(dt)
+    if case["gate"]:
+        grads["gate"] = (d_out * scale * normed * slope).to(dt)
+    if case["scale"]:
+        grads["scale"] = (d_out * gate * normed).sum(0)
+    d_y, grads["weight"] = _rms_backward(d_out * scale * gate, y, inverse, s["weight"])
+    grads["y"] = d_y.to(dt)
+    return outs + [grads[k] for k in _leaves(case)]
+
+
+# ---- the definitions in 64 bits -----------------------------------------------------------------------------------
+
+def exact(case, seed):
+    if case["op"] == "recurrence" and case["T"] * (5 if case["train"] else 2) > 1 << 18:
+        return None
+    with torch.no_grad():
+        s = prepare(case, seed)
+        if case["op"] == "step":
+            g, h = s["gate"].double(), s["state"].double()
+            h = torch.where(s["reset"].bool().unsqueeze(1), 0.0, g * h) + s["inp"].double()
+            return [h, h]
+        if case["op"] == "recurrence":
+            return _exact_recurrence(s, case)
+        if case["op"] == "pack":
+            return [_decoded(s["x"])]
+        return _exact_norms(s, case)
+
+
+def _decoded(x):
+    """The values that the 8-bit checkpoint of x stands for, from the codes that its 32-bit definition gives, group by
+    group of columns."""
+    parts = []
+    for lo in range(0, x.shape[1], GROUP):
+        part = x[:, lo:lo + GROUP].to(torch.float32)
+        top = torch.maximum(part.max(1).values, -part.min(1).values).unsqueeze(1)
+        ok = (top >= SMALLEST).to(torch.float32)
+        levels = ok * 127.0
+        code = (part * (levels / torch.where(ok > 0, top, torch.ones_like(top)))).round()
+        # the product of a 7-bit code and a 24-bit scale is rounded once more, to 32 bits
+        parts.append((code * (ok * top / torch.full_like(top, 127.0))).double())
+    return torch.cat(parts, 1)
+
+
+def _exact_recurrence(s, case):
+    t_all = case["T"]
+    order = range(t_all - 1, -1, -1) if case["reverse"] else range(t_all)
+    start = s["reset"].bool()
+    shape = s["inp"].shape
+    out = torch.empty(shape, dtype=torch.float64, device=DEVICE)
+    h = s["state"].double()
+    for t in order:
+        h = s["inp"][t].double() + (s["gate"][t].double() * h).masked_fill(start[t].unsqueeze(1), 0.0)
+        out[t] = h
+    if not case["train"]:
+        return [out, h]
+    d_gate, d_inp = torch.empty_like(out), torch.empty_like(out)
+    order = list(order)
+    d = s["d_last"].double()
+    for i in range(t_all - 1, -1, -1):
+        t = order[i]
+        d = d + s["d_out"][t].double()
+        d_inp[t] = d
+        before = out[order[i - 1]] if i else s["state"].double()
+        d_gate[t] = (d * before).masked_fill(start[t].unsqueeze(1), 0.0)
+        d = (d * s["gate"][t].double()).masked_fill(start[t].unsqueeze(1), 0.0)
+    return [out, h, d_gate, d_inp, d]
+
+
+def _exact_norms(s, case):
+    d = case["D"]
+
+    def weighted(v):
+        return s[v].double()
+
+    def norm_grad(top, unit, r, w):  # of r * v * w with unit = r * v: the Jacobian of v -> r * v is r (1 - unit unit' / D)
+        inner = top * w
+        return r * (inner - unit * ((inner * unit).sum(1, keepdim=True) / d))
+
+    x = s["x"].double()
+    if case["op"] == "norm":
+        r = 1.0 / torch.sqrt(x.square().sum(1, keepdim=True) / d + EPS)
+        out = [x * r * weighted("weight")]
+        if case["train"]:
+            unit = (_decoded(s["x"]) if case["checkpoint"] else x) * r
+            top = s["d_out"].double()
+            out += [norm_grad(top, unit, r, weighted("weight")), torch.sum(top * unit, 0)]
+        return out
+    y, z = s["y"].double(), (s["gate"].double() if case["gate"] else None)
+    r = 1.0 / torch.sqrt(y.square().sum(1, keepdim=True) / d + EPS)
+    per_channel = weighted("scale") if case["scale"] else torch.ones(d, dtype=torch.float64, device=DEVICE)
+
+    def factor(z):
+        if z is None:
+            return 1.0
+        return {"none": lambda: z, "sigmoid": lambda: torch.sigmoid(z), "silu": lambda: z * torch.sigmoid(z)}[case["activation"]]()
+
+    sum_ = x + per_channel * weighted("weight") * factor(z) * y * r
+    outs = [sum_]
+    if case["next"]:
+        r_next = 1.0 / torch.sqrt(sum_.square().sum(1, keepdim=True) / d + EPS)
+        outs.append(sum_ * r_next * weighted("next_weight"))
+    if not case["train"]:
+        return outs
+    if case["checkpoint"]:
+        y, z = _decoded(s["y"]), (_decoded(s["gate"]) if case["gate"] else None)
+        sum_ = x + per_channel * weighted("weight") * factor(z) * y * r
+    g = {}
+    top = s["d_out"].double()
+    if case["next"]:
+        head, unit = s["d_next"].double(), sum_ * r_next
+        g["next_weight"] = torch.sum(head * unit, 0)
+        top = top + norm_grad(head, unit, r_next, weighted("next_weight"))
+    g["x"] = top
+    unit = y * r
+    f = factor(z)
+    if case["gate"]:
+        p = torch.sigmoid(z)
+        slope = {"none": 1.0, "sigmoid": p * torch.sigmoid(-z), "silu": p + z * p * torch.sigmoid(-z)}[case["activation"]]
+        g["gate"] = top * per_channel * weighted("weight") * unit * slope
+    if case["scale"]:
+        g["scale"] = torch.sum(top * f * weighted("weight") * unit, 0)
+    g["weight"] = torch.sum(top * per_channel * f * unit, 0)
+    g["y"] = norm_grad(top * per_channel * f, unit, r, weighted("weight"))
+    return outs + [g[k] for k in _leaves(case)]
