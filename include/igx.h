@@ -46,8 +46,9 @@ extern "C" {
 typedef void *igx_stream_t; /* hipStream_t */
 
 /* Library identification and error text (no reference counterpart).
- * igx_version() = 100 * major + 10 * minor, 120 for this header: a binding that needs igx_motion_fetch_amp_obs,
- * igx_motion_amp_obs_history or igx_extract_positions_from_rigid_body_states checks for >= 120. */
+ * igx_version() = 100 * major + 10 * minor, 130 for this header: a binding that needs igx_motion_fetch_amp_obs,
+ * igx_motion_amp_obs_history or igx_extract_positions_from_rigid_body_states checks for >= 120, one that needs the
+ * sequence operators (igx_linear_recurrence*, igx_block_norm*, igx_pack8, igx_unpack8) for >= 130. */
 int igx_version(void);
 const char *igx_last_error_string(void);
 
@@ -1051,6 +1052,142 @@ int igx_calc_heading_quat(const float *q, float *out, int64_t n, igx_stream_t st
  * tasks/humanoid_imitate.py:708, :811).  row_stride = floats between consecutive rows of `states`. */
 int igx_extract_positions_from_rigid_body_states(const float *states, int64_t row_stride, int32_t num_bodies, float *out,
                                                  int64_t n, igx_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Sequence operators: what a policy with a recurrent core computes on rollouts
+ * [T, N, D] (step, environment, channel).  Element types of the arrays marked
+ * "elements"; every sum, state and statistic is kept in fp32.
+ * Strides are counted in elements.  Unlike the task buffers these arrays need
+ * only their element's own alignment.
+ * ---------------------------------------------------------------------- */
+#define IGX_F32 0
+#define IGX_F16 1
+#define IGX_BF16 2
+
+/* Gated linear recurrence, independent for every environment n and channel d, from t = 0 upwards (reverse: from T - 1
+ * downwards; "before" is then t + 1):
+ *     out[t] = gate[t] * before + inp[t],  before = out of the previous step in that order, state at the first one.
+ * Where reset[t, n] != 0 an episode begins: `before` does not enter step t, whatever it and the gate hold (also inf or
+ * NaN).  The carried value stays in fp32 and out[t] is its rounding.  Long sequences with few channels are split over
+ * time: a span's gates are multiplied up first, so a product of consecutive gates must be representable in fp32 (gates
+ * within [-1, 1] always are). */
+typedef struct igx_recurrence {
+    int32_t dtype;              /* IGX_F32 / IGX_F16 / IGX_BF16: type of gate, inp, out and their gradients */
+    int32_t reverse;            /* 0: t upwards, otherwise downwards */
+    int64_t steps, envs, width; /* T, N, D; any of them may be 0 */
+    const void *gate;           /* elements [T, N, D] at gate_stride[0], [1] over t and n, [2] over d: 1, or 0 = one gate
+                                   for all channels of the environment */
+    int64_t gate_stride[3];
+    const void *inp;            /* elements [T, N, D] at inp_stride over t and n; channels are adjacent */
+    int64_t inp_stride[2];
+    const int64_t *reset;       /* [T, N] at reset_stride; NULL = no episode begins */
+    int64_t reset_stride[2];
+    const float *state;         /* [N, D] the value before the first step; NULL = zeros */
+    void *out;                  /* elements [T, N, D] at out_stride, channels adjacent; must not overlap any input */
+    int64_t out_stride[2];
+    float *last;                /* [N, D] the unrounded value after the last step; NULL = not wanted.  May be state itself
+                                   (one step of a running policy in place) */
+    void *workspace;            /* igx_linear_recurrence_workspace() bytes (16-byte aligned), private to the call until it
+                                   has run; NULL when that is 0 */
+    int64_t workspace_bytes;
+} igx_recurrence;
+
+/* Bytes of device scratch that a call with these sizes, strides and type needs, forward and backward alike (no pointer
+ * of the struct is read); negative = IGX_E_*. */
+int64_t igx_linear_recurrence_workspace(const igx_recurrence *r);
+int igx_linear_recurrence(const igx_recurrence *r, igx_stream_t stream);
+
+/* Gradients: r holds the forward call's arguments (out as the forward wrote it; inp and last are not read).
+ *     d[t] = d_out[t] + gate of the following step * d of the following step (d_last behind the last one)
+ *     d_inp = d,  d_gate = d * before (0 where an episode begins),  d_state = what leaves the first step.
+ * `before` is read from `out`, at the precision it was stored in.  A gate that several channels or environments share
+ * (a stride of 0) gets its [T, N, D] gradients unsummed. */
+typedef struct igx_recurrence_grad {
+    const void *d_out;        /* elements [T, N, D] at d_out_stride, channels adjacent; NULL = zeros */
+    int64_t d_out_stride[2];
+    const float *d_last;      /* [N, D]; NULL = zeros */
+    void *d_gate;             /* elements [T, N, D] at d_gate_stride; NULL = not wanted */
+    int64_t d_gate_stride[2];
+    void *d_inp;              /* elements [T, N, D] at d_inp_stride; NULL = not wanted */
+    int64_t d_inp_stride[2];
+    float *d_state;           /* [N, D]; NULL = not wanted */
+} igx_recurrence_grad;
+
+int igx_linear_recurrence_backward(const igx_recurrence *r, const igx_recurrence_grad *g, igx_stream_t stream);
+
+/* The norms before and after a block of a residual network, with the branch's gate and residual scale, row by row
+ * (rms(v) = v / sqrt(mean(v^2) + eps) over the row's `width` elements):
+ *     out  = x + scale * act(gate) * (rms(y) * weight)      behind a block whose output is y      (y given)
+ *     next = rms(out) * next_weight                         in front of the next one              (next_weight given)
+ * with out = x where y is NULL (a norm in front of the first block), scale and gate 1 where NULL.  Statistics and the
+ * whole row's arithmetic are fp32, `next` is computed from the unrounded out, every result is rounded once.
+ * Checkpoints (optional outputs of the forward call): the 8-bit codes of y and gate - of x where y is NULL - in the
+ * form of igx_pack8, for a backward call that has the codes in place of those arrays. */
+#define IGX_GATE_NONE 0     /* act(z) = z */
+#define IGX_GATE_SIGMOID 1  /* act(z) = 1 / (1 + exp(-z)) */
+#define IGX_GATE_SILU 2     /* act(z) = z / (1 + exp(-z)) */
+#define IGX_BLOCK_NORM_MAX_WIDTH 8192
+
+typedef struct igx_block_norm {
+    int32_t dtype;       /* IGX_F32 / IGX_F16 / IGX_BF16: type of x, y, gate, out, next and their gradients */
+    int32_t activation;  /* IGX_GATE_* */
+    int64_t rows;        /* may be 0 */
+    int64_t width;       /* 1 ... IGX_BLOCK_NORM_MAX_WIDTH */
+    float eps;
+    const void *x;       /* elements [rows, width], x_stride elements (>= 0) from row to row; so are y and gate */
+    int64_t x_stride;
+    const void *y;       /* NULL: no block in front, out = x */
+    int64_t y_stride;
+    const void *gate;    /* NULL: 1 */
+    int64_t gate_stride;
+    const float *weight;      /* [width], required with y */
+    const float *scale;       /* [width]; NULL = 1 */
+    const float *next_weight; /* [width]; NULL: no norm behind; required without y */
+    void *out;           /* elements [rows, width] contiguous, required with y; not written without */
+    void *next;          /* elements [rows, width] contiguous, required with next_weight */
+    float *y_inv_rms;    /* [rows] 1 / sqrt(mean(y^2) + eps): written by the forward call where not NULL, read by backward */
+    float *out_inv_rms;  /* [rows] the same of out */
+    int8_t *y8;          /* [rows, width] codes of y, or of x without y; NULL: no checkpoint */
+    float *y8_scale;     /* [rows, ceil(width / IGX_PACK8_GROUP)] */
+    int8_t *gate8;       /* [rows, width] codes of gate; NULL: no checkpoint */
+    float *gate8_scale;
+} igx_block_norm;
+
+int igx_block_norm_forward(const igx_block_norm *b, igx_stream_t stream);
+
+/* Gradients.  b holds the forward call's arguments with y_inv_rms (with y) and out_inv_rms (with next_weight) as the
+ * forward call wrote them; out and next are not read, x only with next_weight.  Where y8 (gate8) is given it is read in
+ * place of y (gate; x where y is NULL): the gradients are then those at the values the codes stand for.  y (gate) itself
+ * says which of the operator's parts exist, so with codes it must still be non-NULL; it is not read.
+ * Column sums are added in a fixed order: the same call gives the same bits. */
+typedef struct igx_block_norm_grad {
+    const void *d_out;   /* elements [rows, width] at d_out_stride; NULL = zeros */
+    int64_t d_out_stride;
+    const void *d_next;  /* elements [rows, width] at d_next_stride; NULL = zeros */
+    int64_t d_next_stride;
+    void *d_x;           /* elements [rows, width] contiguous, as d_y and d_gate; each NULL = not wanted */
+    void *d_y;
+    void *d_gate;
+    float *d_weight;     /* [width], as d_scale and d_next_weight; each NULL = not wanted */
+    float *d_scale;
+    float *d_next_weight;
+    void *workspace;     /* igx_block_norm_workspace() bytes (16-byte aligned) where one of the three is wanted */
+    int64_t workspace_bytes;
+} igx_block_norm_grad;
+
+int64_t igx_block_norm_workspace(const igx_block_norm *b); /* bytes, or a negative IGX_E_* */
+int igx_block_norm_backward(const igx_block_norm *b, const igx_block_norm_grad *g, igx_stream_t stream);
+
+/* 8-bit checkpoints of activations: x [rows, width] in groups of IGX_PACK8_GROUP elements along a row (the last one may
+ * be shorter).  With top = the group's largest magnitude, all in fp32:
+ *     scale = top / 127,  code = nearest integer (ties to even) of x * (127 / top),  value = code * scale.
+ * A group with top < 2^-120 becomes zeros; one that holds an inf or NaN decodes to NaN throughout. */
+#define IGX_PACK8_GROUP 64
+
+int igx_pack8(const void *x, int32_t dtype, int64_t rows, int64_t width, int64_t x_stride, int8_t *codes, float *scales,
+              igx_stream_t stream);
+int igx_unpack8(const int8_t *codes, const float *scales, int32_t dtype, int64_t rows, int64_t width, void *x,
+                igx_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -404,3 +404,36 @@ def required_elements(cls, params, n_envs):
         else:
             out[name] = (k(n), True)
     return out
+
+
+# ---- sequence operators -----------------------------------------------------------------------
+IGX_F32, IGX_F16, IGX_BF16 = 0, 1, 2
+IGX_GATE_NONE, IGX_GATE_SIGMOID, IGX_GATE_SILU = 0, 1, 2
+IGX_BLOCK_NORM_MAX_WIDTH = 8192
+IGX_PACK8_GROUP = 64
+
+
+class Recurrence(_Struct):
+    _fields_ = [("dtype", i32), ("reverse", i32), ("steps", i64), ("envs", i64), ("width", i64),
+                ("gate", ptr), ("gate_stride", i64 * 3), ("inp", ptr), ("inp_stride", i64 * 2),
+                ("reset", ptr), ("reset_stride", i64 * 2), ("state", ptr), ("out", ptr), ("out_stride", i64 * 2),
+                ("last", ptr), ("workspace", ptr), ("workspace_bytes", i64)]
+
+
+class RecurrenceGrad(_Struct):
+    _fields_ = [("d_out", ptr), ("d_out_stride", i64 * 2), ("d_last", ptr), ("d_gate", ptr), ("d_gate_stride", i64 * 2),
+                ("d_inp", ptr), ("d_inp_stride", i64 * 2), ("d_state", ptr)]
+
+
+class BlockNorm(_Struct):
+    _fields_ = [("dtype", i32), ("activation", i32), ("rows", i64), ("width", i64), ("eps", f32),
+                ("x", ptr), ("x_stride", i64), ("y", ptr), ("y_stride", i64), ("gate", ptr), ("gate_stride", i64),
+                ("weight", ptr), ("scale", ptr), ("next_weight", ptr), ("out", ptr), ("next", ptr),
+                ("y_inv_rms", ptr), ("out_inv_rms", ptr), ("y8", ptr), ("y8_scale", ptr), ("gate8", ptr),
+                ("gate8_scale", ptr)]
+
+
+class BlockNormGrad(_Struct):
+    _fields_ = [("d_out", ptr), ("d_out_stride", i64), ("d_next", ptr), ("d_next_stride", i64), ("d_x", ptr), ("d_y", ptr),
+                ("d_gate", ptr), ("d_weight", ptr), ("d_scale", ptr), ("d_next_weight", ptr), ("workspace", ptr),
+                ("workspace_bytes", i64)]

@@ -109,6 +109,17 @@ SYMBOLS["igx_quat_axis"] = (C.c_int, [_P, C.c_int32, _P, _I64, _P])
 SYMBOLS["igx_extract_positions_from_rigid_body_states"] = (C.c_int, [_P, _I64, C.c_int32, _P, _I64, _P])
 SYMBOLS["igx_torch_rand_float"] = (C.c_int, [C.c_double, C.c_double, _P, C.c_uint64, C.c_uint64, _P, _I64, _P])
 SYMBOLS["igx_compute_heading_and_up"] = (C.c_int, [_P] * 5 + [C.c_int32] + [_P] * 5 + [_I64, _P])
+# sequence operators
+SYMBOLS.update({
+    "igx_linear_recurrence_workspace": (_I64, [_P]),
+    "igx_linear_recurrence": (C.c_int, [_P, _P]),
+    "igx_linear_recurrence_backward": (C.c_int, [_P, _P, _P]),
+    "igx_block_norm_workspace": (_I64, [_P]),
+    "igx_block_norm_forward": (C.c_int, [_P, _P]),
+    "igx_block_norm_backward": (C.c_int, [_P, _P, _P]),
+    "igx_pack8": (C.c_int, [_P, C.c_int32, _I64, _I64, _I64, _P, _P, _P]),
+    "igx_unpack8": (C.c_int, [_P, _P, C.c_int32, _I64, _I64, _P, _P]),
+})
 
 
 class IgxError(RuntimeError):

@@ -687,3 +687,224 @@ class WindowQuantile:
             break
         self.fallbacks += 1
         return False
+
+
+# ---- sequence operators (isaacgym_amd.sequence differentiates through them) ----------------------
+_ELEMENTS = {torch.float32: _abi.IGX_F32, torch.float16: _abi.IGX_F16, torch.bfloat16: _abi.IGX_BF16}
+_ACTIVATIONS = {"none": _abi.IGX_GATE_NONE, "sigmoid": _abi.IGX_GATE_SIGMOID, "silu": _abi.IGX_GATE_SILU}
+
+
+def _element(t, name):
+    """The ABI's number of a tensor's element type."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s: expected a torch.Tensor, got %r" % (name, type(t)))
+    if t.dtype not in _ELEMENTS:
+        raise TypeError("%s: expected float32, float16 or bfloat16, got %s" % (name, t.dtype))
+    return _ELEMENTS[t.dtype]
+
+
+def _same(t, name, shape, dtype, dev):
+    """t is a device tensor of that shape, type and device."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s: expected a torch.Tensor, got %r" % (name, type(t)))
+    if not t.is_cuda:
+        raise ValueError("libigx works on device tensors only (%s is a %s tensor)" % (name, t.device))
+    if t.dtype != dtype:
+        raise TypeError("%s: expected dtype %s, got %s" % (name, dtype, t.dtype))
+    if t.device != dev:
+        raise ValueError("%s is on %s, others on %s" % (name, t.device, dev))
+    if t.shape != shape:
+        raise ValueError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+
+
+def _packed(t, name, shape, dtype, dev):
+    """The address of a contiguous tensor (None: NULL)."""
+    if t is None:
+        return None
+    _same(t, name, shape, dtype, dev)
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)
+    return t.data_ptr()
+
+
+def _rollout(t, name, shape, dtype, dev, written=False):
+    """(address, (stride over steps, stride over environments)) of a [T, N, D] tensor with adjacent channels, any
+    strides otherwise; one that is written must not map two elements to one address."""
+    if t is None:
+        return None, (0, 0)
+    _same(t, name, shape, dtype, dev)
+    st, sn, sd = t.stride()
+    if shape[2] > 1 and sd != 1:
+        raise ValueError("%s: the channels (last dimension) must be adjacent, their stride is %d" % (name, sd))
+    if written and t.numel() and not t.is_contiguous():
+        reach = 0
+        for s, n in sorted((s, n) for s, n in zip(t.stride(), shape) if n > 1):
+            if s <= reach:
+                raise ValueError("%s: several elements share one address" % name)
+            reach += s * (n - 1)
+    return t.data_ptr(), (st, sn)
+
+
+def _recurrence(gate, inp_like, state, reset, reverse):
+    """igx_recurrence with the arguments that forward and backward share; inp_like gives shape, type and device."""
+    if not isinstance(inp_like, torch.Tensor) or inp_like.dim() != 3:
+        raise ValueError("linear_recurrence: rollouts are [steps, environments, channels] tensors")
+    shape, dtype, dev = inp_like.shape, inp_like.dtype, inp_like.device
+    r = _abi.Recurrence(dtype=_element(inp_like, "inp"), reverse=int(bool(reverse)), steps=shape[0], envs=shape[1],
+                        width=shape[2])
+    _same(gate, "gate", shape, dtype, dev)
+    sd = gate.stride(2) if shape[2] > 1 else 1
+    if sd not in (0, 1):
+        raise ValueError("gate: the channels (last dimension) must be adjacent or share one gate, their stride is %d" % sd)
+    r.gate = gate.data_ptr()
+    r.gate_stride[:] = (gate.stride(0), gate.stride(1), sd)
+    r.state = _packed(state, "state", shape[1:], torch.float32, dev)
+    if reset is not None:
+        _same(reset, "reset", shape[:2], torch.int64, dev)
+        r.reset = reset.data_ptr()
+        r.reset_stride[:] = reset.stride()
+    return r, shape, dtype, dev
+
+
+def _recurrence_workspace(r, dev):
+    size = int(_lib.lib().igx_linear_recurrence_workspace(C.byref(r)))
+    if size < 0:
+        _lib.check(size)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    r.workspace, r.workspace_bytes = (ws.data_ptr(), size) if size else (None, 0)
+    return ws
+
+
+def linear_recurrence(gate, inp, out, state=None, reset=None, last=None, reverse=False):
+    """out[t] = gate[t] * (out before it) + inp[t] over [T, N, D] (igx_linear_recurrence).  gate, inp and out share a type
+    and need adjacent channels (gate also one value for all channels of an environment); state and last are fp32 [N, D]
+    (last may be state), reset int64 [T, N].  out must not overlap an input."""
+    r, shape, dtype, dev = _recurrence(gate, inp, state, reset, reverse)
+    r.inp, r.inp_stride[:] = _rollout(inp, "inp", shape, dtype, dev)
+    r.out, r.out_stride[:] = _rollout(out, "out", shape, dtype, dev, written=True)
+    if out is None:
+        raise TypeError("out: expected a torch.Tensor, got None")
+    if out.numel() and out.data_ptr() in (gate.data_ptr(), inp.data_ptr()):
+        raise ValueError("out must not overlap an input")
+    r.last = _packed(last, "last", shape[1:], torch.float32, dev)
+    ws = _recurrence_workspace(r, dev)  # noqa: F841 (freed to the stream's pool after the launch)
+    _lib.check(_lib._launch(_lib.lib().igx_linear_recurrence, dev, C.byref(r)))
+    return out
+
+
+def linear_recurrence_backward(gate, out, d_out=None, d_last=None, d_gate=None, d_inp=None, d_state=None, state=None,
+                               reset=None, reverse=False):
+    """The gradients of linear_recurrence (igx_linear_recurrence_backward): those of d_gate, d_inp [T, N, D] and d_state
+    [N, D] that are given are filled in; d_out and d_last None stand for zeros."""
+    r, shape, dtype, dev = _recurrence(gate, out, state, reset, reverse)
+    r.out, r.out_stride[:] = _rollout(out, "out", shape, dtype, dev)
+    g = _abi.RecurrenceGrad()
+    g.d_out, g.d_out_stride[:] = _rollout(d_out, "d_out", shape, dtype, dev)
+    g.d_gate, g.d_gate_stride[:] = _rollout(d_gate, "d_gate", shape, dtype, dev, written=True)
+    g.d_inp, g.d_inp_stride[:] = _rollout(d_inp, "d_inp", shape, dtype, dev, written=True)
+    g.d_last = _packed(d_last, "d_last", shape[1:], torch.float32, dev)
+    g.d_state = _packed(d_state, "d_state", shape[1:], torch.float32, dev)
+    ws = _recurrence_workspace(r, dev)  # noqa: F841
+    _lib.check(_lib._launch(_lib.lib().igx_linear_recurrence_backward, dev, C.byref(r), C.byref(g)))
+
+
+def _row_array(t, name, shape, dtype, dev):
+    """(address, stride) of a [rows, width] tensor whose columns are adjacent."""
+    if t is None:
+        return None, 0
+    _same(t, name, shape, dtype, dev)
+    if shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError("%s: the columns must be adjacent, their stride is %d" % (name, t.stride(1)))
+    return t.data_ptr(), t.stride(0) if shape[0] > 1 else shape[1]
+
+
+def _block_norm(x_like, weight, gate, scale, next_weight, activation, eps, y_inv_rms, out_inv_rms, codes):
+    if not isinstance(x_like, torch.Tensor) or x_like.dim() != 2:
+        raise ValueError("block_norm: rows are [rows, width] tensors")
+    if activation not in _ACTIVATIONS:
+        raise ValueError("activation must be one of %s, got %r" % (sorted(_ACTIVATIONS), activation))
+    shape, dev = x_like.shape, x_like.device
+    b = _abi.BlockNorm(dtype=_element(x_like, "x"), activation=_ACTIVATIONS[activation], rows=shape[0], width=shape[1],
+                       eps=float(eps))
+    f = torch.float32
+    for k, t in (("weight", weight), ("scale", scale), ("next_weight", next_weight)):
+        setattr(b, k, _packed(t, k, shape[1:], f, dev))
+    for k, t in (("y_inv_rms", y_inv_rms), ("out_inv_rms", out_inv_rms)):
+        setattr(b, k, _packed(t, k, shape[:1], f, dev))
+    groups = -(-shape[1] // _abi.IGX_PACK8_GROUP)
+    for k, pair in zip(("y8", "gate8"), codes):
+        if pair is not None:
+            setattr(b, k, _packed(pair[0], k, shape, torch.int8, dev))
+            setattr(b, k + "_scale", _packed(pair[1], k + "_scale", (shape[0], groups), f, dev))
+    return b, shape, x_like.dtype, dev
+
+
+def block_norm(x, y=None, weight=None, gate=None, scale=None, next_weight=None, out=None, next=None, y_inv_rms=None,
+               out_inv_rms=None, y_codes=None, gate_codes=None, activation="silu", eps=1e-5):
+    """out = x + scale * act(gate) * (rms(y) * weight) and next = rms(out) * next_weight, row by row (igx_block_norm_forward;
+    without y: out = x).  x, y, gate are [rows, width] with adjacent columns, out and next contiguous; parameters fp32
+    [width]; y_codes / gate_codes: (codes, scales) to fill in."""
+    b, shape, dtype, dev = _block_norm(x, weight, gate, scale, next_weight, activation, eps, y_inv_rms, out_inv_rms,
+                                       (y_codes, gate_codes))
+    b.x, b.x_stride = _row_array(x, "x", shape, dtype, dev)
+    b.y, b.y_stride = _row_array(y, "y", shape, dtype, dev)
+    b.gate, b.gate_stride = _row_array(gate, "gate", shape, dtype, dev)
+    b.out = _packed(out, "out", shape, dtype, dev)
+    b.next = _packed(next, "next", shape, dtype, dev)
+    _lib.check(_lib._launch(_lib.lib().igx_block_norm_forward, dev, C.byref(b)))
+
+
+def block_norm_backward(rows_like, x=None, y=None, weight=None, gate=None, scale=None, next_weight=None, y_inv_rms=None,
+                        out_inv_rms=None, y_codes=None, gate_codes=None, activation="silu", eps=1e-5, d_out=None,
+                        d_next=None, d_x=None, d_y=None, d_gate=None, d_weight=None, d_scale=None, d_next_weight=None):
+    """The gradients of block_norm (igx_block_norm_backward): those given are filled in.  rows_like: a [rows, width] tensor of
+    the rows' type and device.  y_codes (gate_codes) in place of y (gate; of x in a call without a block): the gradients at
+    the values the codes stand for."""
+    b, shape, dtype, dev = _block_norm(rows_like, weight, gate, scale, next_weight, activation, eps, y_inv_rms, out_inv_rms,
+                                       (y_codes, gate_codes))
+    b.x, b.x_stride = _row_array(x, "x", shape, dtype, dev)
+    b.y, b.y_stride = _row_array(y, "y", shape, dtype, dev)
+    b.gate, b.gate_stride = _row_array(gate, "gate", shape, dtype, dev)
+    if weight is not None and y is None and y_codes is not None:
+        b.y = b.y8  # says that there is a block; not read
+    if gate is None and gate_codes is not None:
+        b.gate = b.gate8
+    g = _abi.BlockNormGrad()
+    g.d_out, g.d_out_stride = _row_array(d_out, "d_out", shape, dtype, dev)
+    g.d_next, g.d_next_stride = _row_array(d_next, "d_next", shape, dtype, dev)
+    for k, t in (("d_x", d_x), ("d_y", d_y), ("d_gate", d_gate)):
+        setattr(g, k, _packed(t, k, shape, dtype, dev))
+    for k, t in (("d_weight", d_weight), ("d_scale", d_scale), ("d_next_weight", d_next_weight)):
+        setattr(g, k, _packed(t, k, shape[1:], torch.float32, dev))
+    ws = None
+    if d_weight is not None or d_scale is not None or d_next_weight is not None:
+        size = int(_lib.lib().igx_block_norm_workspace(C.byref(b)))
+        if size < 0:
+            _lib.check(size)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        g.workspace, g.workspace_bytes = ws.data_ptr(), size
+    _lib.check(_lib._launch(_lib.lib().igx_block_norm_backward, dev, C.byref(b), C.byref(g)))
+
+
+def pack8(x, codes, scales):
+    """codes int8 [rows, width] and scales fp32 [rows, ceil(width / 64)] of x [rows, width] (igx_pack8)."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("pack8: x must be a [rows, width] tensor")
+    shape, dev = x.shape, x.device
+    dt = _element(x, "x")
+    p, stride = _row_array(x, "x", shape, x.dtype, dev)
+    q = _packed(codes, "codes", shape, torch.int8, dev)
+    s = _packed(scales, "scales", (shape[0], -(-shape[1] // _abi.IGX_PACK8_GROUP)), torch.float32, dev)
+    _lib.check(_lib._launch(_lib.lib().igx_pack8, dev, p, dt, shape[0], shape[1], stride, q, s))
+
+
+def unpack8(codes, scales, out):
+    """out [rows, width] = the values that codes and scales stand for (igx_unpack8)."""
+    if not isinstance(out, torch.Tensor) or out.dim() != 2:
+        raise ValueError("unpack8: out must be a [rows, width] tensor")
+    shape, dev = out.shape, out.device
+    dt = _element(out, "out")
+    q = _packed(codes, "codes", shape, torch.int8, dev)
+    s = _packed(scales, "scales", (shape[0], -(-shape[1] // _abi.IGX_PACK8_GROUP)), torch.float32, dev)
+    o = _packed(out, "out", shape, out.dtype, dev)
+    _lib.check(_lib._launch(_lib.lib().igx_unpack8, dev, q, s, dt, shape[0], shape[1], o))

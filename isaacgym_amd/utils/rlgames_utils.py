@@ -13,6 +13,7 @@ length bookkeeping around it in the agent loop (learning/common_agent.py:284-296
   `episode` infos, mean / min / max of every window, the direct scalars - written through
   `writer.add_scalar(tag, value, step)` exactly as the reference names them.  This is the one
   place that reads device memory (once per epoch).
+* `discount_values`: the advantages of a rollout, as one reversed linear recurrence.
 * `AverageMeter`: the windowed mean rl_games keeps for `game_rewards` / `game_lengths`
   (rl_games.algos_torch.torch_ext.AverageMeter; rl_games is not part of the reference tree, its
   published update rule is restated here).  `GameStats` feeds two of them from the per-step
@@ -24,7 +25,7 @@ from collections import OrderedDict
 import numpy as np
 import torch
 
-from .. import _abi, _lib
+from .. import _abi, _lib, sequence
 from ..episode_stats import EpisodeStats
 
 
@@ -109,6 +110,21 @@ class GameStats:
             self.game_rewards.update_batch(n, float(sums[i, 0]))
             self.game_lengths.update_batch(n, float(sums[i, 1]))
         self._pending = 0
+
+
+def discount_values(fdones, values, rewards, next_values, gamma, tau):
+    """Advantages of a rollout as the agent's discount_values computes them, step by step from the last one:
+        delta = rewards + gamma * next_values - values,  adv[t] = delta[t] + gamma * tau * (1 - fdones[t]) * adv[t + 1]
+    - the reversed linear recurrence with one gate for everything (one launch instead of a Python loop over the horizon).
+    fdones [T, N]: the reset flags the steps returned (int64; the agents' floats are taken too), the others
+    [T, N] or [T, N, D] float32 (one episode end for all D values).  Returns the advantages without gradients."""
+    with torch.no_grad():
+        delta = torch.add(rewards, next_values, alpha=float(gamma)).sub_(values)
+        rows = delta if delta.dim() == 3 else delta.unsqueeze(-1)
+        gate = torch.full((1, 1, 1), float(gamma) * float(tau), dtype=rows.dtype, device=rows.device)
+        done = fdones if fdones.dtype == torch.int64 else (fdones != 0).to(torch.int64)
+        adv, _ = sequence.linear_recurrence(gate, rows, reset=done, reverse=True)
+        return adv.view(delta.shape)
 
 
 class RLGPUAlgoObserver:

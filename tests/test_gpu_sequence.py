@@ -1,0 +1,664 @@
+"""The sequence operators against their plain 64-bit forms (tests/seq_cases.py), within the error that their types allow:
+lengths from none to long, odd widths, every layout that is accepted, resets, non-finite values where they must not
+count, gradients against formula and differences, streams, graphs and in-place steps."""
+import gc
+
+import pytest
+import torch
+
+from isaacgym_amd import ops, sequence
+from tests import seq_cases as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def lay(t, layout):
+    """t [T, N, D] (CPU) on the device with its elements laid out in the given way."""
+    T, N, D = t.shape
+    if layout == "time":
+        return t.to(DEV).contiguous()
+    if layout == "env":
+        return t.transpose(0, 1).contiguous().to(DEV).transpose(0, 1)
+    if layout == "slice":  # columns 3 ... of wider rows: neither aligned nor adjacent rows
+        big = torch.full((T, N, D + 5), float("nan"), dtype=t.dtype, device=DEV)
+        big[:, :, 3:3 + D] = t.to(DEV)
+        return big[:, :, 3:3 + D]
+    if layout == "steps":  # every second step of a longer rollout
+        big = torch.full((2 * T, N, D), float("nan"), dtype=t.dtype, device=DEV)
+        big[::2] = t.to(DEV)
+        return big[::2]
+    raise AssertionError(layout)
+
+
+def rollout(T, N, D, dtype, seed, resets=0.0, gate_shape=None):
+    g = gen(seed)
+    gate = torch.sigmoid(torch.randn(gate_shape or (T, N, D), generator=g) * 2 + 1).to(dtype)
+    inp = torch.randn(T, N, D, generator=g).to(dtype)
+    state = torch.randn(N, D, generator=g)
+    reset = (torch.rand(T, N, generator=g) < resets).to(torch.int64) * 3
+    d_out = torch.randn(T, N, D, generator=g).to(dtype)
+    d_last = torch.randn(N, D, generator=g)
+    return gate, inp, state, reset, d_out, d_last
+
+
+def check_recurrence(gate, inp, state, reset, d_out, d_last, reverse=False, layout="time", grad_layout="time"):
+    """Forward and backward through autograd on the device, against the plain form of the same values."""
+    full = gate.shape == inp.shape
+    a = lay(gate, layout) if full else gate.to(DEV)
+    b = lay(inp, layout)
+    h = None if state is None else state.to(DEV)
+    f = None if reset is None else reset.to(DEV)
+    leaves = [t.requires_grad_(True) for t in (a, b, h) if t is not None]
+    out, last = sequence.linear_recurrence(a, b, state=h, reset=f, reverse=reverse)
+    assert out.shape == b.shape and out.dtype == b.dtype and last.dtype == F32
+    ref = S.recurrence(gate, inp, state, reset, reverse, d_out, d_last)
+    S.close(out, *ref["out"], "out")
+    S.close(last, *ref["last"], "last")
+    grads = torch.autograd.grad((out, last), leaves, (lay(d_out, grad_layout), d_last.to(DEV)))
+    names = ["d_gate", "d_inp"] + (["d_state"] if h is not None else [])
+    for name, got in zip(names, grads):
+        if name == "d_gate" and not full:
+            continue
+        S.close(got, *ref[name], name)
+    return out, last, grads
+
+
+SHAPES = [(1, 1, 1), (1, 5, 3), (2, 3, 8), (7, 2, 60), (8, 37, 5), (9, 4, 105), (31, 1, 64), (33, 3, 211), (64, 130, 4),
+          (129, 2, 17), (300, 1, 7), (1000, 3, 33), (1025, 1, 129), (4100, 1, 3), (2500, 1, 260)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_recurrence_shapes(shape, dtype):
+    T, N, D = shape
+    check_recurrence(*rollout(T, N, D, dtype, 1, resets=min(0.3, 4.0 / T)))
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("layout", ["time", "env", "slice", "steps"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_recurrence_layouts(layout, dtype, reverse):
+    other = {"time": "env", "env": "slice", "slice": "time", "steps": "env"}[layout]
+    for T, N, D in ((150, 3, 12), (17, 6, 1), (20, 5, 9)):
+        check_recurrence(*rollout(T, N, D, dtype, 2, resets=0.05), reverse=reverse, layout=layout, grad_layout=other)
+
+
+@pytest.mark.parametrize("T,N,D", [(16, 5, 24), (400, 1, 8), (5, 6, 1)])
+@pytest.mark.parametrize("shape", ["one", "per_step", "per_env", "per_channel", "per_step_env"])
+def test_recurrence_broadcast_gate(T, N, D, shape):
+    gs = {"one": (1, 1, 1), "per_step": (T, 1, 1), "per_env": (1, N, 1), "per_channel": (1, 1, D), "per_step_env": (T, N, 1)}[shape]
+    gate, inp, state, reset, d_out, d_last = rollout(T, N, D, F32, 3, resets=0.05, gate_shape=gs)
+    _, _, grads = check_recurrence(gate, inp, state, reset, d_out, d_last)
+    ref, bound = S.recurrence(gate, inp, state, reset, False, d_out, d_last)["d_gate"]
+    dims = [i for i in range(3) if gs[i] == 1 and ref.shape[i] > 1]
+    assert grads[0].shape == gs
+    total = ref.sum(dims, keepdim=True) if dims else ref
+    count = ref.numel() // total.numel()
+    slack = ((bound + count * S.U * ref.abs()).sum(dims, keepdim=True)) if dims else bound
+    S.close(grads[0], total, slack, "summed d_gate")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_recurrence_optional_arguments(dtype):
+    gate, inp, state, reset, d_out, d_last = rollout(21, 4, 10, dtype, 4, resets=0.1)
+    check_recurrence(gate, inp, None, reset, d_out, d_last)
+    check_recurrence(gate, inp, state, None, d_out, d_last)
+    check_recurrence(gate, inp, None, None, d_out, d_last, reverse=True)
+    # only one of the outputs used, only one of the inputs differentiated
+    a, b, h, f = gate.to(DEV), inp.to(DEV), state.to(DEV), reset.to(DEV)
+    for use_out in (True, False):
+        ref = S.recurrence(gate, inp, state, reset, False, d_out if use_out else None, None if use_out else d_last)
+        for i, name in enumerate(("d_gate", "d_inp", "d_state")):
+            args = [a.clone(), b.clone(), h.clone()]
+            args[i].requires_grad_(True)
+            out, last = sequence.linear_recurrence(args[0], args[1], state=args[2], reset=f)
+            head = (out, d_out.to(DEV)) if use_out else (last, d_last.to(DEV))
+            got, = torch.autograd.grad(head[0], args[i], head[1])
+            S.close(got, *ref[name], "%s alone" % name)
+    # a gradient that autograd hands in with stride 0
+    args = [t.clone().requires_grad_(True) for t in (a, b, h)]
+    sequence.linear_recurrence(*args, reset=f)[0].sum().backward()
+    ref = S.recurrence(gate, inp, state, reset, False, torch.ones(inp.shape), None)
+    for t, name in zip(args, ("d_gate", "d_inp", "d_state")):
+        S.close(t.grad, *ref[name], "%s of a sum" % name)
+
+
+@pytest.mark.parametrize("T,N,D", [(6, 4, 8), (700, 1, 12), (40, 3, 3)])
+def test_recurrence_nothing_passes_an_episode_start(T, N, D):
+    """Gates, state and earlier values that are inf or NaN must not reach what lies behind a reset."""
+    gate, inp, state, _, d_out, d_last = rollout(T, N, D, F32, 5)
+    reset = torch.zeros(T, N, dtype=torch.int64)
+    at = T // 2
+    reset[at] = 1
+    reset[0] = -7
+    gate[0], gate[at] = float("nan"), float("inf")
+    state[:] = float("nan")
+    inp[at - 1] = float("inf")
+    clean_gate, clean_inp, clean_state = gate.clone(), inp.clone(), torch.zeros_like(state)
+    clean_gate[0] = clean_gate[at] = 0.0
+    ref = S.recurrence(clean_gate, clean_inp, clean_state, reset)
+    out, last = sequence.linear_recurrence(gate.to(DEV), inp.to(DEV), state=state.to(DEV), reset=reset.to(DEV))
+    S.close(out[:at - 1], ref["out"][0][:at - 1], ref["out"][1][:at - 1], "before")
+    S.close(out[at:], ref["out"][0][at:], ref["out"][1][at:], "behind")
+    assert torch.isinf(out[at - 1]).all()
+    d_gate, d_inp, d_state = torch.empty_like(out), torch.empty_like(out), torch.empty_like(last)
+    d_out[at:] = float("nan")  # what lies behind must not flow back over the start either
+    ops.linear_recurrence_backward(gate.to(DEV), out, d_out=d_out.to(DEV), d_last=d_last.to(DEV), d_gate=d_gate, d_inp=d_inp,
+                                   d_state=d_state, state=state.to(DEV), reset=reset.to(DEV))
+    assert torch.isfinite(d_inp[:at]).all() and torch.isnan(d_inp[at:]).all()
+    assert (d_gate[0] == 0).all() and (d_gate[at] == 0).all() and (d_state == 0).all()
+
+
+def test_recurrence_every_step_reset_and_zero_state():
+    gate, inp, state, _, d_out, d_last = rollout(200, 2, 8, BF16, 6)
+    reset = torch.ones(200, 2, dtype=torch.int64)
+    out, last, grads = check_recurrence(gate, inp, state, reset, d_out, d_last)
+    assert torch.equal(out.cpu(), inp) and (grads[0] == 0).all() and (grads[2] == 0).all()
+
+
+def test_recurrence_growing_gates_from_a_zero_state():
+    """Gates of 2 over 300 steps: their product overflows fp32, the state stays 0 until the last step."""
+    for T in (300, 3000):
+        inp = torch.zeros(T, 1, 8)
+        inp[-1] = 1.0
+        out, last = sequence.linear_recurrence(torch.full((T, 1, 8), 2.0, device=DEV), inp.to(DEV))
+        assert torch.equal(out.cpu(), inp) and (last == 1).all()
+
+
+@pytest.mark.parametrize("T,N,D", [(0, 3, 4), (5, 0, 4), (5, 3, 0), (0, 0, 0)])
+def test_recurrence_empty(T, N, D):
+    a = torch.empty(T, N, D, device=DEV, requires_grad=True)
+    b = torch.empty(T, N, D, device=DEV, requires_grad=True)
+    h = torch.randn(N, D, device=DEV, requires_grad=True)
+    out, last = sequence.linear_recurrence(a, b, state=h, reset=torch.zeros(T, N, dtype=torch.int64, device=DEV))
+    assert out.shape == (T, N, D)
+    if T == 0:
+        assert torch.equal(last, h)
+        g = torch.randn_like(last)
+        assert torch.equal(torch.autograd.grad(last, h, g)[0], g)
+        assert (sequence.linear_recurrence(a.detach(), b.detach())[1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("N,D", [(1, 1), (5, 3), (130, 60), (4096, 64)])
+def test_recurrence_step(N, D, dtype):
+    gate, inp, state, reset, _, _ = rollout(1, N, D, dtype, 7, resets=0.2)
+    ref = S.recurrence(gate, inp, state, reset)
+    a, b, h, f = gate[0].to(DEV), inp[0].to(DEV), state.to(DEV), reset[0].to(DEV)
+    kept, to = h.clone(), torch.full_like(h, float("nan"))
+    out = sequence.linear_recurrence_step(a, b, h, reset=f, state_out=to)
+    S.close(out, ref["out"][0][0], ref["out"][1][0], "out")
+    S.close(to, *ref["last"], "state_out")
+    assert torch.equal(h, kept)
+    again = sequence.linear_recurrence_step(a, b, h, reset=f)
+    assert torch.equal(h, to) and torch.equal(again, out)  # in place: the same bits
+
+
+def test_recurrence_step_in_place_where_lanes_share_channels():
+    """A width that the 16-byte vector does not divide: the last lane of a row overlaps the one before."""
+    for N, D in ((1, 13), (3001, 5), (1, 100003)):
+        gate, inp, state, _, _, _ = rollout(1, N, D, BF16, 8)
+        wide = torch.zeros(N, D + 3, dtype=BF16, device=DEV)  # rows apart: lanes per environment
+        wide[:, 1:1 + D] = inp[0].to(DEV)
+        for b in (inp[0].to(DEV), wide[:, 1:1 + D]):
+            h, to = state.to(DEV), torch.empty(N, D, device=DEV)
+            sequence.linear_recurrence_step(gate[0].to(DEV), b, h, state_out=to)
+            sequence.linear_recurrence_step(gate[0].to(DEV), b, h)
+            assert torch.equal(h, to)
+
+
+def test_recurrence_writes_only_its_elements():
+    gate, inp, state, reset, _, _ = rollout(70, 3, 13, F16, 9, resets=0.1)
+    big = torch.full((140, 3, 20), 7.0, dtype=F16, device=DEV)
+    out = big[::2, :, 4:17]
+    ops.linear_recurrence(gate.to(DEV), inp.to(DEV), out, state=state.to(DEV), reset=reset.to(DEV))
+    ref = S.recurrence(gate, inp, state, reset)
+    S.close(out, *ref["out"], "out")
+    assert (big[1::2] == 7).all() and (big[:, :, :4] == 7).all() and (big[:, :, 17:] == 7).all()
+
+
+def test_recurrence_offsets_past_32_bits():
+    """Steps and environments more than 2^32 bytes apart."""
+    far = torch.zeros(3 * (1 << 30) + 64, dtype=F32, device=DEV)
+    gate, inp, state, _, _, _ = rollout(3, 2, 8, F32, 10)
+    for strides in (((1 << 30), 16, 1), (16, (1 << 30) + (1 << 29), 1)):
+        b = far.as_strided((3, 2, 8), strides)
+        b.copy_(inp)
+        out = torch.empty(3, 2, 8, device=DEV)
+        ops.linear_recurrence(gate.to(DEV), b, out, state=state.to(DEV))
+        S.close(out, *S.recurrence(gate, inp, state)["out"], "out")
+        ops.linear_recurrence(gate.to(DEV), inp.to(DEV), b, state=state.to(DEV))
+        assert torch.equal(b, out)
+
+
+def test_recurrence_gradient_against_differences():
+    """<gradient, v> against (f(x + e v) - f(x - e v)) / 2e of the 64-bit plain form, e = 1e-6: the difference's own error
+    is 2^-53 |f| / e + e^2 |f'''| < 1e-8 of the magnitudes, below the fp32 gradient's."""
+    gate, inp, state, reset, d_out, d_last = rollout(40, 2, 6, F32, 11, resets=0.05)
+    gate, inp, state, d_out, d_last = (t.double() for t in (gate, inp, state, d_out, d_last))
+    _, _, grads = check_recurrence(gate.float(), inp.float(), state.float(), reset, d_out.float(), d_last.float())
+
+    def f(a, b, h):
+        r = S.recurrence(a, b, h, reset)
+        return float((r["out"][0] * d_out).sum() + (r["last"][0] * d_last).sum())
+
+    e = 1e-6
+    for i, x in enumerate((gate, inp, state)):
+        v = torch.randn(x.shape, generator=gen(12 + i), dtype=torch.float64)
+        plus, minus = ([y + s * e * v if y is x else y for y in (gate, inp, state)] for s in (1, -1))
+        diff = (f(*plus) - f(*minus)) / (2 * e)
+        g = grads[i].double().cpu()
+        # every element of the gradient is within 40 steps' roundings of 3 u each; magnitudes from |g| plus one per step
+        assert abs(float((g * v).sum()) - diff) <= 1e-5 * float((g.abs() * v.abs()).sum() + v.abs().sum())
+
+
+# ---- norms ----------------------------------------------------------------------------------------------------------
+
+def norm_inputs(R, D, dtype, seed, gate=True, scale=True, next=True, spread=True):
+    g = gen(seed)
+    x, y, z, do, dn = (torch.randn(R, D, generator=g) for _ in range(5))
+    if spread and R:  # rows of very different sizes, one of them empty
+        y = y * torch.logspace(-3, 2, R)[:, None]
+        y[R // 2] = 0
+    w, s, w2 = (1 + 0.2 * torch.randn(D, generator=g) for _ in range(3))
+    t = dict(x=x.to(dtype), y=y.to(dtype), gate=(2 * z).to(dtype) if gate else None, weight=w, scale=s if scale else None,
+             next_weight=w2 if next else None)
+    return t, do.to(dtype), dn.to(dtype)
+
+
+def check_norm(t, d_out, d_next, activation="silu", checkpoint=False, place=None):
+    """residual_norm (or rms_norm where there is no y) forward and backward against the plain form."""
+    place = place or (lambda v: v.to(DEV))
+    dev = {k: (place(v) if v.dim() == 2 else v.to(DEV)).requires_grad_(True) for k, v in t.items() if v is not None}
+    if t.get("y") is None:
+        outs = (sequence.rms_norm(dev["x"], dev["next_weight"], checkpoint=checkpoint),)
+        heads, names = (place(d_next),), ("next",)
+        d_out = None
+    else:
+        outs = sequence.residual_norm(**dev, activation=activation, checkpoint=checkpoint)
+        outs = outs if "next_weight" in dev else (outs,)
+        heads, names = (place(d_out), place(d_next))[:len(outs)], ("out", "next")
+    ref = S.block_norm(**t, activation=activation, d_out=d_out, d_next=d_next if t["next_weight"] is not None else None,
+                       checkpoint=checkpoint)
+    for name, got in zip(names, outs):
+        S.close(got, *ref[name], name)
+    keys = list(dev)
+    grads = torch.autograd.grad(outs, [dev[k] for k in keys], heads)
+    for k, got in zip(keys, grads):
+        assert got.dtype == dev[k].dtype and got.shape == dev[k].shape
+        S.close(got, *ref["d_" + k], "d_" + k)
+    return outs, dict(zip(keys, grads))
+
+
+NORM_SHAPES = [(1, 1), (3, 2), (5, 7), (64, 8), (33, 60), (7, 64), (130, 65), (19, 105), (6, 128), (300, 211), (5, 256),
+               (9, 500), (4, 512), (3, 513), (5, 1025), (2, 2048), (3, 4099), (2, 8192)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", NORM_SHAPES)
+def test_residual_norm_shapes(shape, dtype):
+    t, do, dn = norm_inputs(*shape, dtype, 20)
+    check_norm(t, do, dn)
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", [(1, 1), (70, 33), (40, 64), (9, 130), (5, 700), (3, 2049), (2, 5000)])
+def test_rms_norm(shape, dtype, checkpoint):
+    t, _, dn = norm_inputs(*shape, dtype, 21)
+    check_norm(dict(x=t["y"], y=None, next_weight=t["next_weight"]), None, dn, checkpoint=checkpoint)
+
+
+@pytest.mark.parametrize("activation", ["silu", "sigmoid", "none"])
+@pytest.mark.parametrize("gate,scale,nxt", [(True, True, False), (True, False, True), (False, True, True), (False, False, False)])
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_residual_norm_parts(gate, scale, nxt, activation, checkpoint):
+    for (R, D), dtype in (((50, 60), F32), ((37, 264), BF16), ((6, 1100), F16)):
+        t, do, dn = norm_inputs(R, D, dtype, 22, gate=gate, scale=scale, next=nxt)
+        check_norm(t, do, dn, activation=activation, checkpoint=checkpoint)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_residual_norm_strided_rows(dtype):
+    def place(v):  # rows of a wider array, from an odd column
+        big = torch.full((v.shape[0], v.shape[1] + 9), float("nan"), dtype=v.dtype, device=DEV)
+        big[:, 5:5 + v.shape[1]] = v.to(DEV)
+        return big[:, 5:5 + v.shape[1]]
+
+    for R, D in ((20, 60), (11, 211), (4, 1030)):
+        t, do, dn = norm_inputs(R, D, dtype, 23)
+        check_norm(t, do, dn, place=place)
+
+
+def test_residual_norm_many_rows():
+    """More rows than there are lane groups on the card: the groups walk, the column sums are joined."""
+    t, do, dn = norm_inputs(40001, 24, F32, 24, spread=False)
+    check_norm(t, do, dn)
+    t, do, dn = norm_inputs(9001, 600, BF16, 25, spread=False)
+    check_norm(t, do, dn)
+
+
+def test_residual_norm_leading_dimensions_and_unused_outputs():
+    t, do, dn = norm_inputs(24, 40, F32, 26)
+    dev = {k: (v.view(2, 3, 4, 40) if v.dim() == 2 else v).to(DEV).requires_grad_(True) for k, v in t.items()}
+    out, nxt = sequence.residual_norm(**dev)
+    assert out.shape == nxt.shape == (2, 3, 4, 40)
+    for used, head, args in ((out, do, dict(d_out=do)), (nxt, dn, dict(d_next=dn))):
+        ref = S.block_norm(**t, **args)
+        grads = torch.autograd.grad(used, [dev[k] for k in t], head.view(2, 3, 4, 40).to(DEV), retain_graph=True,
+                                    allow_unused=True)
+        for k, got in zip(t, grads):
+            S.close(got.reshape(ref["d_" + k][0].shape), *ref["d_" + k], "d_" + k)
+    # one leaf alone
+    for k in t:
+        args = {j: (v.detach().requires_grad_(j == k)) for j, v in dev.items()}
+        o, n = sequence.residual_norm(**args)
+        got, = torch.autograd.grad((o, n), args[k], (do.view(o.shape).to(DEV), dn.view(o.shape).to(DEV)))
+        ref = S.block_norm(**t, d_out=do, d_next=dn)["d_" + k]
+        S.close(got.reshape(ref[0].shape), *ref, "d_%s alone" % k)
+
+
+def test_norms_empty():
+    for R in (0,):
+        x = torch.empty(R, 30, device=DEV, requires_grad=True)
+        w = torch.ones(30, device=DEV, requires_grad=True)
+        out = sequence.rms_norm(x, w)
+        assert out.shape == (R, 30)
+        gx, gw = torch.autograd.grad(out, (x, w), torch.empty_like(out))
+        assert gx.shape == x.shape and (gw == 0).all()
+        out, nxt = sequence.residual_norm(x, x, w, gate=x, scale=w, next_weight=w)
+        gw, = torch.autograd.grad((out, nxt), w, (torch.empty_like(out), torch.empty_like(nxt)))
+        assert (gw == 0).all()
+
+
+def test_norms_a_row_does_not_touch_its_neighbours():
+    """NaN and inf in one row stay in it (and in the column sums); the others keep their bits."""
+    t, do, dn = norm_inputs(65, 50, F32, 27)
+    clean = {k: v.to(DEV) for k, v in t.items()}
+    bad = {k: v.clone() for k, v in clean.items()}
+    bad["y"][17], bad["x"][40], bad["gate"][3, 5] = float("nan"), float("inf"), float("nan")
+    keep = torch.ones(65, dtype=torch.bool)
+    keep[[17, 40, 3]] = False
+    for a, b in zip(sequence.residual_norm(**clean), sequence.residual_norm(**bad)):
+        assert torch.equal(a[keep], b[keep])
+        assert torch.isnan(b[17]).all()
+
+
+def test_norms_offsets_past_32_bits():
+    far = torch.zeros(2 * (1 << 30) + 4096, dtype=F32, device=DEV)
+    t, do, dn = norm_inputs(3, 40, F32, 28)
+    x = far.as_strided((3, 40), (1 << 30, 1))
+    x.copy_(t["x"])
+    got = sequence.residual_norm(x, t["y"].to(DEV), t["weight"].to(DEV), gate=t["gate"].to(DEV), scale=t["scale"].to(DEV))
+    t["next_weight"] = None
+    S.close(got, *S.block_norm(**t)["out"], "out")
+    codes, scales = torch.empty(3, 40, dtype=torch.int8, device=DEV), torch.empty(3, 1, device=DEV)
+    ops.pack8(x, codes, scales)
+    assert torch.equal(codes.cpu().float(), S.through8(t["x"])[1])
+
+
+def test_norm_gradient_against_differences():
+    """As for the recurrence: the 64-bit plain form's central differences, e = 1e-6."""
+    t, do, dn = norm_inputs(12, 20, F32, 29, spread=False)
+    _, grads = check_norm(t, do, dn)
+    t = {k: v.double() for k, v in t.items()}
+
+    def f(t):
+        r = S.block_norm(**t)
+        return float((r["out"][0] * do.double()).sum() + (r["next"][0] * dn.double()).sum())
+
+    e = 1e-6
+    for i, k in enumerate(t):
+        v = torch.randn(t[k].shape, generator=gen(30 + i), dtype=torch.float64)
+        diff = (f({**t, k: t[k] + e * v}) - f({**t, k: t[k] - e * v})) / (2 * e)
+        g = grads[k].double().cpu()
+        assert abs(float((g * v).sum()) - diff) <= 1e-5 * float((g.abs() * v.abs()).sum() + v.abs().sum()), k
+
+
+# ---- 8-bit checkpoints ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 5), (17, 63), (9, 64), (11, 65), (40, 105), (5, 128), (2, 1000), (3001, 211)])
+def test_pack8_is_the_definition_bit_for_bit(shape, dtype):
+    x = (torch.randn(*shape, generator=gen(40)) * torch.logspace(-4, 4, shape[0])[:, None]).to(dtype)
+    value, code, scale = S.through8(x)
+    codes, scales = sequence.pack8(x.to(DEV))
+    assert torch.equal(codes.cpu().float(), code) and torch.equal(scales.cpu(), scale)
+    for to in (dtype, F32):
+        assert torch.equal(sequence.unpack8(codes, scales, dtype=to).cpu(), value.to(to))
+
+
+def test_pack8_ends_of_the_range():
+    """Zeros, subnormals, values at the type's ends, ties, and non-finite values, which mark their group."""
+    x = torch.zeros(9, 130)
+    x[1] = 1e-40
+    x[2, 3] = 2.0 ** -120
+    x[3] = torch.linspace(-127, 127, 130)
+    x[4, :64] = torch.arange(64) + 0.5
+    x[4, 0] = 127.0
+    x[5] = 3.0e38
+    x[6, 70], x[7, 1], x[8, 129] = float("nan"), float("inf"), float("-inf")
+    value, code, scale = S.through8(x)
+    codes, scales = sequence.pack8(x.to(DEV))
+    assert torch.equal(codes.cpu().float(), code)
+    got = sequence.unpack8(codes, scales).cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(value)) and torch.equal(got.nan_to_num(7.0), value.nan_to_num(7.0))
+    assert torch.isfinite(got[6, :64]).all() and torch.isnan(got[6, 64:128]).all() and torch.isnan(got[8, 128:]).all()
+
+
+def test_pack8_shapes_and_empty():
+    x = torch.randn(2, 3, 70, device=DEV)
+    codes, scales = sequence.pack8(x)
+    assert codes.shape == (2, 3, 70) and scales.shape == (2, 3, 2)
+    assert torch.equal(sequence.unpack8(codes, scales), S.through8(x.cpu().view(6, 70))[0].view(2, 3, 70).to(DEV))
+    codes, scales = sequence.pack8(torch.empty(0, 70, device=DEV))
+    assert sequence.unpack8(codes, scales).shape == (0, 70)
+
+
+def test_checkpoint_frees_what_it_replaces():
+    """With checkpoint=True the graph holds codes, not the block's output and gate."""
+    R, D = 8192, 512
+    x = torch.randn(R, D, device=DEV, dtype=BF16, requires_grad=True)
+    w = torch.ones(D, device=DEV)
+    size = R * D * 2
+
+    def held(checkpoint):
+        gc.collect()
+        torch.cuda.synchronize()
+        start = torch.cuda.memory_allocated()
+        out = sequence.residual_norm(x, x * 2, w, gate=x + 1, checkpoint=checkpoint)
+        gc.collect()
+        return torch.cuda.memory_allocated() - start, out
+
+    plain, o1 = held(False)
+    del o1
+    packed, o2 = held(True)
+    assert plain >= 3 * size and packed <= 2.2 * size
+
+
+# ---- streams, graphs, repeatability ---------------------------------------------------------------------------------
+
+def block(x, p, state, reset):
+    """norm -> recurrence -> gated norm on the residual stream: one block of a recurrent policy."""
+    n = sequence.rms_norm(x, p["w_in"])
+    h, last = sequence.linear_recurrence(torch.sigmoid(n), n, state=state, reset=reset)
+    out, nxt = sequence.residual_norm(x, h, p["w_out"], gate=n, scale=p["s"], next_weight=p["w_next"], checkpoint=True)
+    return out, nxt, last
+
+
+def block_inputs(T, N, D, dtype=F32, seed=50):
+    g = gen(seed)
+    x = torch.randn(T, N, D, generator=g).to(dtype).to(DEV)
+    p = {k: (1 + 0.1 * torch.randn(D, generator=g)).to(DEV) for k in ("w_in", "w_out", "s", "w_next")}
+    state = torch.randn(N, D, generator=g).to(DEV)
+    reset = (torch.rand(T, N, generator=g) < 0.1).to(torch.int64).to(DEV)
+    heads = [torch.randn(T, N, D, generator=g).to(dtype).to(DEV) for _ in range(2)]
+    return x, p, state, reset, heads
+
+
+def block_pass(x, p, state, reset, heads):
+    leaves = [x, state] + list(p.values())
+    for t in leaves:
+        t.requires_grad_(True)
+    out, nxt, last = block(x, p, state, reset)
+    grads = torch.autograd.grad((out, nxt), leaves, heads)
+    return [out.detach(), nxt.detach(), last.detach()] + list(grads)
+
+
+def test_same_call_same_bits():
+    args = block_inputs(300, 5, 100)
+    first = block_pass(*args)
+    for _ in range(3):
+        for a, b in zip(first, block_pass(*args)):
+            assert torch.equal(a, b)
+
+
+def test_side_stream():
+    args = block_inputs(64, 7, 72, BF16)
+    want = block_pass(*args)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = block_pass(*args)
+    torch.cuda.current_stream().wait_stream(s)
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+def test_two_captured_graphs_replayed_with_eager_work_between():
+    """Forward and backward of a block in two graphs, on new inputs every replay, against the eager pass."""
+    graphs = []
+    for i, (T, N, D) in enumerate(((2000, 1, 40), (40, 6, 130))):
+        x, p, state, reset, heads = block_inputs(T, N, D, seed=60 + i)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                block_pass(x, p, state, reset, heads)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = block_pass(x, p, state, reset, heads)
+        graphs.append((graph, (x, p, state, reset, heads), outs, (T, N, D)))
+    for turn in range(4):
+        for graph, args, outs, shape in graphs:
+            x, p, state, reset, heads = args
+            fresh = block_inputs(*shape, seed=70 + turn)
+            with torch.no_grad():
+                x.copy_(fresh[0])
+                state.copy_(fresh[2])
+                for k in p:
+                    p[k].copy_(fresh[1][k])
+                reset.copy_(fresh[3])
+                for h, f in zip(heads, fresh[4]):
+                    h.copy_(f)
+            graph.replay()
+            want = block_pass(*fresh)
+            torch.cuda.synchronize()
+            for a, b in zip(outs, want):
+                assert torch.equal(a, b)
+            del want
+
+
+def test_capture_with_a_live_eager_graph_of_the_same_leaf_is_refused():
+    x, p, state, reset, heads = block_inputs(8, 2, 16)
+    x.requires_grad_(True)
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    alive = sequence.rms_norm(x, w)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager autograd graph"):
+        with torch.cuda.graph(graph):
+            torch.zeros(1, device=DEV).add_(1)
+            sequence.rms_norm(x, w)
+    del alive, graph
+    torch.cuda.synchronize()
+    out = sequence.rms_norm(x, w)  # eager work goes on as before
+    S.close(out.view(16, 16), *S.block_norm(x.detach().view(16, 16), next_weight=w)["next"], "next")
+
+
+# ---- as they are used: a policy on an environment's rollout ------------------------------------------------------------
+
+def test_policy_block_on_a_task_rollout():
+    """A recurrent policy runs a task step by step; the rollout is then trained on as a whole.  The training pass gives
+    the running policy's outputs again, its gradients are the plain form's, and the advantages are the agent's loop."""
+    from isaacgym_amd import tasks
+    from isaacgym_amd.utils.rlgames_utils import discount_values
+
+    T, N = 24, 64
+    env = tasks.make("Ant", num_envs=N, device=DEV)
+    D = env.num_obs
+    g = gen(80)
+    w_in, w_out, s, w_next = ((1 + 0.1 * torch.randn(D, generator=g)).to(DEV) for _ in range(4))
+    k = torch.randn(D, generator=g).to(DEV)
+    env.reset_done()
+    state = torch.zeros(N, D, device=DEV)
+    start = state.clone()
+    begins = torch.ones(N, dtype=torch.int64, device=DEV)  # the first step starts every episode
+    xs, flags, outs, rewards, dones = [], [], [], [], []
+    obs = env.obs_buf.clone()
+    env.progress_buf[::5] = 990  # some episodes end inside the rollout
+    for t in range(T):
+        n = sequence.rms_norm(obs, w_in)
+        h = sequence.linear_recurrence_step(torch.sigmoid(n * k), n, state, reset=begins)
+        out, nxt = sequence.residual_norm(obs, h, w_out, gate=n, scale=s, next_weight=w_next)
+        xs.append(obs)
+        flags.append(begins)
+        outs.append((out, nxt))
+        obs_dict, rew, reset, _ = env.step(nxt[:, :env.num_actions].tanh())
+        obs, begins = obs_dict["obs"].clone(), reset.clone()
+        rewards.append(rew.clone())
+        dones.append(begins)
+    assert sum(int(f.sum()) for f in flags[1:]) > 0
+    x, reset = torch.stack(xs), torch.stack(flags)
+    leaves = [t.requires_grad_(True) for t in (x, w_in, w_out, s, w_next)]
+    n = sequence.rms_norm(x, w_in)
+    gates = torch.sigmoid(n * k)
+    h, last = sequence.linear_recurrence(gates, n, state=start, reset=reset)
+    out, nxt = sequence.residual_norm(x, h, w_out, gate=n, scale=s, next_weight=w_next)
+    # one step or many: a chain of at most T + 3 fp32 operators, about 100 u each (the norms' own bounds), on either side
+    chain = (T + 3) * 100 * S.U
+    for t in range(T):
+        for a, b in ((out.detach()[t], outs[t][0]), (nxt.detach()[t], outs[t][1])):
+            assert float((a - b).abs().max()) <= 2 * chain * float(out.detach().abs().max())
+    assert float((last.detach() - state).abs().max()) <= 2 * chain * float(h.detach().abs().max())
+
+    d = [torch.randn(out.shape, generator=g).to(DEV) for _ in range(2)]
+    grads = torch.autograd.grad((out, nxt), leaves, d)
+    # the whole block in 64 bits, differentiated by torch
+    q = [t.detach().double().cpu().requires_grad_(True) for t in leaves]
+    X, W, WO, SS, WN = q
+
+    def rms(v):
+        return v / (v.square().mean(-1, keepdim=True) + 1e-5).sqrt()
+
+    NN = rms(X) * W
+    A = torch.sigmoid(NN * k.double().cpu())
+    H, hs = torch.zeros(N, D, dtype=torch.float64), []
+    for t in range(T):
+        H = torch.where(reset[t].cpu().bool()[:, None], torch.zeros_like(H), A[t] * H) + NN[t]
+        hs.append(H)
+    O = X + SS * (NN * torch.sigmoid(NN)) * rms(torch.stack(hs)) * WO
+    ref = torch.autograd.grad((O, rms(O) * WN), q, [t.double().cpu() for t in d])
+    for got, want in zip(grads, ref):
+        assert float((got.double().cpu() - want).abs().max()) <= chain * float(want.abs().max())
+
+    rew, done = torch.stack(rewards), torch.stack(dones)
+    values, nxt_values = torch.randn(2, T, N, generator=g).to(DEV)
+    adv = discount_values(done, values, rew, nxt_values, 0.99, 0.95)
+    r64, v64, n64 = rew.double(), values.double(), nxt_values.double()
+    want, mag = torch.zeros(T, N, dtype=torch.float64, device=DEV), torch.zeros(T, N, dtype=torch.float64, device=DEV)
+    a, m = 0.0, 0.0
+    for t in range(T - 1, -1, -1):
+        live = 0.99 * 0.95 * (1.0 - done[t].double())
+        a = r64[t] + 0.99 * n64[t] - v64[t] + live * a
+        m = r64[t].abs() + n64[t].abs() + v64[t].abs() + live * m
+        want[t], mag[t] = a, m
+    # two roundings of the difference, one of the gate (twice: gamma * tau, its product) and one of the sum, every step
+    assert ((adv.double() - want).abs() <= 5 * T * S.U * mag).all()
