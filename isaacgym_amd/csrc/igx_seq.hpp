@@ -103,6 +103,6 @@ template <int V> __device__ __forceinline__ void load_codes(const int8_t *p, flo
 inline int element_size(int dtype) { return dtype == IGX_F32 ? 4 : 2; }
 inline bool known_dtype(int dtype) { return dtype == IGX_F32 || dtype == IGX_F16 || dtype == IGX_BF16; }
 
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+__host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace igx

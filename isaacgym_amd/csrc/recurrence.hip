@@ -1,55 +1,65 @@
 // Gated linear recurrence h[t] = gate[t] h[t-1] + inp[t] over rollouts [T, N, D], and its gradients.
 //
 // Channels are independent and adjacent in memory, so a lane owns one 16-byte vector of channels and walks the steps
-// with the state in fp32 registers.  A call moves 3 elements per (t, n, d) forward and 5 backward and does 2 - 3
-// operations on each: HBM bounds it.
+// with the carried value in fp32 registers; the loads of kUnroll steps are in flight together, since they do not depend
+// on it.  A call moves 3 elements per (t, n, d) forward and 5 backward and does 2 - 3 operations on each: HBM bounds it
+// where there are enough channels to fill the card.
+//
+// With fewer channels the time is split, for the recurrence is a composition of maps h -> A h + B that is associative:
+//   - within a workgroup SEG groups of lanes take kUnroll consecutive steps each of the same channels, reduce them to
+//     (A, B) in registers, exchange those through LDS, and then walk their steps from the value that reaches them, so
+//     every element is still read and written once;
+//   - across workgroups a first kernel reduces every span of the time to its (A, B) in a workspace, and each workgroup of
+//     the second composes the spans before its own.  That reads gate and inp twice (the second time mostly from the
+//     caches), so it is done only where the channels alone leave CUs without work.
 #include "igx_seq.hpp"
 
 namespace igx {
 namespace {
 
-constexpr int kUnroll = 8;   // steps whose loads are in flight together: they do not depend on the state
 constexpr int kBlock = 256;
 
-enum Flags { kNoFlags = 0, kOneFlag = 1, kFlagEach = 2 };
+// reset flags a lane needs for a step: its channels belong to one environment, to two, or to any number
+enum Flags { kNoFlags = 0, kOneFlag = 1, kTwoFlags = 2, kFlagEach = 3 };
 
 // One call as the kernels see it.  The steps are numbered in the order they are computed (the host turns an array
-// round by pointing at its last step and negating its stride), strides are in bytes.
+// round by pointing at its last step and negating its stride), strides are in bytes.  Forward reads gate and `add` = inp;
+// backward runs the other way, add = d_out, before = out one step further on.
 struct RecArgs {
-    const char *gate, *inp, *reset, *out_r;
-    char *out;
-    const float *state;
-    float *last;
-    const char *d_out;
-    char *d_gate, *d_inp;
-    const float *d_last;
-    float *d_state;
-    int64_t gate_t, gate_n, inp_t, inp_n, reset_t, reset_n, out_t, out_n;
-    int64_t d_out_t, d_out_n, d_gate_t, d_gate_n, d_inp_t, d_inp_n;
-    int64_t T, D;
-    int64_t run;      // channels that are adjacent in every array: N * D where the environments follow each other, else D
-    int64_t per_run;  // vectors in a run
-    int64_t vectors;  // vectors in all
-    int splat;        // one gate for all channels of a run
+    const char *gate, *add, *reset, *before;
+    char *to, *d_gate;          // forward: out; backward: d_inp, d_gate (NULL: not wanted)
+    const float *start;         // forward: state, backward: d_last; NULL: zeros
+    float *end;                 // forward: last, backward: d_state; NULL: not wanted
+    const float *state;         // backward: what stands before the first step; NULL: zeros
+    float *spans;               // [0]: start; [1 + 2 s], [2 + 2 s]: A and B of span s; rows of `vectors` lane vectors
+    int64_t gate_t, gate_n, add_t, add_n, reset_t, reset_n, before_t, before_n, to_t, to_n, d_gate_t, d_gate_n;
+    int64_t T, span;            // steps in all, and in a span
+    uint32_t D;
+    uint32_t run;      // channels that are adjacent in every array: N * D where the environments follow each other, else D
+    uint32_t per_run;  // vectors in a run
+    uint32_t vectors;  // vectors in all
+    int splat;         // one gate for all channels of a run
 };
 
 // Which channels a lane owns: V of them from `col` of run `row`.  The last vector of a run that V does not divide is
 // moved back to end with the run: its first `skip` channels belong to the lane before and are computed but not stored.
 struct Lane {
-    int64_t row, col;
+    uint32_t row, col;
     int skip;
+    int64_t channel;  // of state, last and their gradients
 };
 
-template <int V> __device__ __forceinline__ Lane lane_of(const RecArgs &a, int64_t v)
+template <int V> __device__ __forceinline__ Lane lane_of(const RecArgs &a, uint32_t v)
 {
     Lane l;
     l.row = a.per_run == a.vectors ? 0 : v / a.per_run;
     l.col = (v - l.row * a.per_run) * V;
     l.skip = 0;
-    if (l.col + V > a.run) {
-        l.skip = (int)(l.col + V - a.run);
+    if (V > 1 && a.run - l.col < V) {
+        l.skip = (int)(V - (a.run - l.col));
         l.col = a.run - V;
     }
+    l.channel = (int64_t)l.row * a.run + l.col;
     return l;
 }
 
@@ -64,34 +74,45 @@ template <typename T, int V> __device__ __forceinline__ void store_from(char *p,
     }
 }
 
-// Reset flags of the lane's channels for one step: one environment for all of them (a single flag), or one each.
+// Reset flags of the lane's channels for one step: one environment's, that of the first and the last (the environment
+// changes at channel `cut`), or each channel's.
 template <int V, int FL> struct LaneFlags {
-    const char *p[FL == kFlagEach ? V : 1];
+    static constexpr int kCount = FL == kFlagEach ? V : FL == kTwoFlags ? 2 : 1;
+    const char *p[kCount];
+    int cut;
     __device__ __forceinline__ LaneFlags(const RecArgs &a, const Lane &l)
     {
         if constexpr (FL == kNoFlags) return;
-        const int64_t first = l.row * (a.run / a.D);  // run = D: the run's environment; run = N * D: row is 0
-        if constexpr (FL == kOneFlag) {
-            p[0] = a.reset + (first + l.col / a.D) * a.reset_n;
-        } else if constexpr (FL == kFlagEach) {
+        // a run of D channels is one environment; the only run of N * D holds them all
 #pragma unroll
-            for (int i = 0; i < V; i++) p[i] = a.reset + (first + (l.col + i) / a.D) * a.reset_n;
+        for (int i = 0; i < kCount; i++) {
+            const uint32_t env = l.row + (l.col + (FL == kTwoFlags && i ? V - 1 : i)) / a.D;
+            p[i] = a.reset + (int64_t)env * a.reset_n;
+            if (FL == kTwoFlags && i) cut = (int)((env - l.row) * a.D - l.col);
         }
     }
 };
 
+// steps whose loads a lane has in flight; a flag for every channel takes as many registers as the channels do
+constexpr int kUnroll = 8;
+template <int V, int FL> constexpr int unroll_of() { return FL == kFlagEach && V == 8 ? kUnroll / 2 : kUnroll; }
+
 template <int V, int FL> struct StepFlags {
-    int64_t f[FL == kFlagEach ? V : 1];
-    __device__ __forceinline__ void load(const LaneFlags<V, FL> &lf, int64_t off)
+    using Places = LaneFlags<V, FL>;
+    int64_t f[Places::kCount];
+    int cut;
+    __device__ __forceinline__ void load(const Places &lf, int64_t off)
     {
         if constexpr (FL != kNoFlags) {
 #pragma unroll
-            for (int i = 0; i < (FL == kFlagEach ? V : 1); i++) f[i] = *reinterpret_cast<const int64_t *>(lf.p[i] + off);
+            for (int i = 0; i < Places::kCount; i++) f[i] = *reinterpret_cast<const int64_t *>(lf.p[i] + off);
+            if (FL == kTwoFlags) cut = lf.cut;
         }
     }
     __device__ __forceinline__ bool begins(int i) const
     {
         if constexpr (FL == kNoFlags) return false;
+        if constexpr (FL == kTwoFlags) return i < cut ? f[0] != 0 : f[1] != 0;
         return f[FL == kFlagEach ? i : 0] != 0;
     }
 };
@@ -107,110 +128,335 @@ template <typename T, int V> __device__ __forceinline__ void load_gate(Raw<T, V>
     }
 }
 
-template <typename T, int V, int FL> __global__ __launch_bounds__(kBlock) void recurrence_kernel(RecArgs a)
+// The map of some steps, h -> A h + B.  Behind an episode's start nothing of h is left, not even an inf or NaN times 0:
+// such a map has kDropped for A, a NaN that arithmetic does not produce.  And where nothing is carried in, the result is
+// B whatever A has grown to.
+constexpr uint32_t kDropped = 0x7fc0d209u;
+__device__ __forceinline__ bool dropped(float A) { return __float_as_uint(A) == kDropped; }
+__device__ __forceinline__ float through(float A, float B, float h) { return h == 0.0f || dropped(A) ? B : fmaf(A, h, B); }
+
+// K consecutive steps of a lane's channels in registers.  `count` of them exist, the others repeat the last one and are
+// neutral; whole steps of a full group cost no test (CHECK false).
+template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK> struct Steps {
+    Raw<T, V> g[K], x[K], hb[K];
+    StepFlags<V, FL> f[K];
+    int count;
+
+    __device__ __forceinline__ void load(const RecArgs &a, const LaneFlags<V, FL> &lf, const char *gate, const char *add,
+                                         const char *before, int64_t t0, int64_t t1)
+    {
+        count = CHECK ? (t1 - t0 < K ? (int)(t1 - t0) : K) : K;
+        const int64_t most = t1 - 1;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int64_t t = CHECK && t0 + k > most ? most : t0 + k;
+            load_gate<T, V>(g[k], gate + t * a.gate_t, a.splat);
+            f[k].load(lf, t * a.reset_t);
+        }
+        if (!BACKWARD || add) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                const int64_t t = CHECK && t0 + k > most ? most : t0 + k;
+                x[k] = load_raw<T, V>(add + t * a.add_t);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; k++) x[k] = {};
+        }
+        if (BACKWARD && before) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {  // before the first step stands `state`, which is not in out
+                const int64_t t = CHECK && t0 + k > most ? most : t0 + k;
+                if (t < a.T - 1) hb[k] = load_raw<T, V>(before + t * a.before_t);
+            }
+        }
+    }
+    __device__ __forceinline__ bool there(int k) const { return !CHECK || k < count; }
+
+    // the steps as one map (A, B) after those already in it; `starts`: channels in which an episode began
+    __device__ __forceinline__ void reduce(float (&A)[V], float (&B)[V], bool (&starts)[V]) const
+    {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const bool begins = f[k].begins(i);
+                const float gate = raw_at(g[k], i), x1 = raw_at(x[k], i);
+                const float b = BACKWARD ? (begins ? 0.0f : gate * (B[i] + x1)) : (begins ? x1 : fmaf(gate, B[i], x1));
+                A[i] = there(k) ? gate * A[i] : A[i];
+                B[i] = there(k) ? b : B[i];
+                starts[i] = starts[i] || (there(k) && begins);
+            }
+        }
+    }
+
+    // forward: h = gate h + inp -> out.  backward: d = d_out + h -> d_inp, d * before -> d_gate, h = gate d
+    __device__ __forceinline__ void walk(const RecArgs &a, const Lane &l, bool store, char *to, char *d_gate, int64_t t0,
+                                         float (&h)[V]) const
+    {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            if (CHECK && !there(k)) break;
+            const int64_t t = t0 + k;
+            if constexpr (!BACKWARD) {
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const float x1 = raw_at(x[k], i);
+                    h[i] = f[k].begins(i) ? x1 : fmaf(raw_at(g[k], i), h[i], x1);
+                }
+                if (store) store_from<T, V>(to + t * a.to_t, h, l.skip);
+            } else {
+                float d[V], dg[V];
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    d[i] = raw_at(x[k], i) + h[i];
+                    dg[i] = 0.0f;
+                    h[i] = f[k].begins(i) ? 0.0f : raw_at(g[k], i) * d[i];
+                }
+                if (d_gate) {
+                    if (t < a.T - 1) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) dg[i] = f[k].begins(i) ? 0.0f : d[i] * raw_at(hb[k], i);
+                    } else if (a.state) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) dg[i] = f[k].begins(i) ? 0.0f : d[i] * a.state[l.channel + i];
+                    }
+                    if (store) store_from<T, V>(d_gate + t * a.d_gate_t, dg, l.skip);
+                }
+                if (to && store) store_from<T, V>(to + t * a.to_t, d, l.skip);
+            }
+        }
+    }
+};
+
+template <int V> __device__ __forceinline__ void identity(float (&A)[V], float (&B)[V], bool (&starts)[V])
 {
-    const int64_t v = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < V; i++) A[i] = 1.0f, B[i] = 0.0f, starts[i] = false;
+}
+
+// A as the maps hold it
+template <int V> __device__ __forceinline__ void mark(float (&A)[V], const bool (&starts)[V])
+{
+#pragma unroll
+    for (int i = 0; i < V; i++) A[i] = __uint_as_float(starts[i] ? kDropped : A[i] != A[i] ? 0x7fc00000u : __float_as_uint(A[i]));
+}
+
+// where a lane's channels lie in the arrays
+template <typename T> struct Places {
+    const char *gate, *add, *before;
+    char *to, *d_gate;
+    __device__ __forceinline__ Places(const RecArgs &a, const Lane &l)
+    {
+        const int64_t at = (int64_t)l.col * sizeof(T);
+        gate = a.gate + l.row * a.gate_n + (a.splat ? 0 : at);
+        add = a.add ? a.add + l.row * a.add_n + at : nullptr;
+        before = a.before ? a.before + l.row * a.before_n + at : nullptr;
+        to = a.to ? a.to + l.row * a.to_n + at : nullptr;
+        d_gate = a.d_gate ? a.d_gate + l.row * a.d_gate_n + at : nullptr;
+    }
+};
+
+template <int V> __device__ __forceinline__ void store_end(const RecArgs &a, const Lane &l, const float (&h)[V])
+{
+    if (!a.end) return;
+#pragma unroll
+    for (int i = 0; i < V; i++)
+        if (i >= l.skip) a.end[l.channel + i] = h[i];
+}
+
+// enough channels: a lane walks all the steps
+template <typename T, int V, int FL, bool BACKWARD>
+__global__ __launch_bounds__(kBlock) void recurrence_kernel(RecArgs a)
+{
+    const uint32_t v = blockIdx.x * kBlock + threadIdx.x;
     if (v >= a.vectors) return;
     const Lane l = lane_of<V>(a, v);
     const LaneFlags<V, FL> lf(a, l);
-    const char *gate = a.gate + l.row * a.gate_n + (a.splat ? 0 : l.col * (int64_t)sizeof(T));
-    const char *inp = a.inp + l.row * a.inp_n + l.col * sizeof(T);
-    char *out = a.out + l.row * a.out_n + l.col * sizeof(T);
-    const int64_t c = l.row * a.run + l.col;
+    const Places<T> p(a, l);
     float h[V];
 #pragma unroll
-    for (int i = 0; i < V; i++) h[i] = a.state ? a.state[c + i] : 0.0f;
-    for (int64_t t0 = 0; t0 < a.T; t0 += kUnroll) {
-        Raw<T, V> g[kUnroll], x[kUnroll];
-        StepFlags<V, FL> f[kUnroll];
+    for (int i = 0; i < V; i++) h[i] = a.start ? a.start[l.channel + i] : 0.0f;
+    int64_t t = 0;
+    auto group = [&](auto count) {
+        constexpr int K = decltype(count)::value;
+        Steps<T, V, FL, K, BACKWARD, false> s;
+        s.load(a, lf, p.gate, p.add, p.before, t, t + K);
+        s.walk(a, l, true, p.to, p.d_gate, t, h);
+        t += K;
+    };
+    constexpr int kSteps = unroll_of<V, FL>();
+    while (t + kSteps <= a.T) group(std::integral_constant<int, kSteps>());
+    if (kSteps > 4 && a.T - t >= 4) group(std::integral_constant<int, 4>());
+    if (a.T - t >= 2) group(std::integral_constant<int, 2>());
+    if (a.T - t >= 1) group(std::integral_constant<int, 1>());
+    store_end<V>(a, l, h);
+}
+
+// V floats of each of a workgroup's lanes, as 16-byte columns without bank conflicts
+template <int V, int LANES> struct Exchange {
+    static constexpr int Q = V >= 4 ? V / 4 : 1, W = V >= 4 ? 4 : V;
+    typedef typename Pack<float, W>::type Word __attribute__((aligned(4 * W)));
+    Word w[Q][LANES];
+    __device__ __forceinline__ void put(int lane, const float (&f)[V])
+    {
+        if constexpr (V == 1) {
+            w[0][lane] = f[0];
+        } else {
 #pragma unroll
-        for (int k = 0; k < kUnroll; k++) {
-            const int64_t t = t0 + k < a.T ? t0 + k : a.T - 1;
-            load_gate<T, V>(g[k], gate + t * a.gate_t, a.splat);
-            x[k] = load_raw<T, V>(inp + t * a.inp_t);
-            f[k].load(lf, t * a.reset_t);
-        }
-#pragma unroll
-        for (int k = 0; k < kUnroll; k++) {
-            if (t0 + k >= a.T) break;
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                const float add = raw_at(x[k], i);
-                h[i] = f[k].begins(i) ? add : fmaf(raw_at(g[k], i), h[i], add);
-            }
-            store_from<T, V>(out + (t0 + k) * a.out_t, h, l.skip);
+            for (int q = 0; q < Q; q++) w[q][lane] = {f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]};
         }
     }
-    if (a.last) {
+    __device__ __forceinline__ void get(int lane, float (&f)[V]) const
+    {
+        if constexpr (V == 1) {
+            f[0] = w[0][lane];
+        } else {
 #pragma unroll
-        for (int i = 0; i < V; i++)
-            if (i >= l.skip) a.last[c + i] = h[i];
+            for (int q = 0; q < Q; q++) {
+                const Word x = w[q][lane];
+#pragma unroll
+                for (int i = 0; i < 4; i++) f[4 * q + i] = x[i];
+            }
+        }
+    }
+};
+
+// the map (A, B) behind (A1, B1), into the latter
+template <int V> __device__ __forceinline__ void compose(float (&A1)[V], float (&B1)[V], const float (&A)[V], const float (&B)[V])
+{
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const bool none = dropped(A[i]) || dropped(A1[i]);
+        const float product = A[i] * A1[i];
+        B1[i] = through(A[i], B[i], B1[i]);
+        A1[i] = __uint_as_float(none ? kDropped : product != product ? 0x7fc00000u : __float_as_uint(product));
     }
 }
 
-// Backward: the steps are numbered from the last computed one, `carry` is what the later steps hand back.
-//     d = d_out + carry;  d_inp = d;  d_gate = d * before;  carry = gate * d
-template <typename T, int V, int FL> __global__ __launch_bounds__(kBlock) void recurrence_backward_kernel(RecArgs a)
+template <int V> __device__ __forceinline__ void load_span(const RecArgs &a, int64_t row, uint32_t v, float (&f)[V])
 {
-    const int64_t v = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (v >= a.vectors) return;
+    const float *p = a.spans + (row * a.vectors + v) * V;
+    if constexpr (V == 1) f[0] = *p;
+    else widen(load_raw<float, V>(p), f);
+}
+
+// Time split: SEG groups of 256 / SEG lanes take kUnroll steps each of the same channels; blockIdx.y is the span.
+template <typename T, int V, int FL, bool BACKWARD, int SEG>
+__global__ __launch_bounds__(kBlock) void recurrence_split_kernel(RecArgs a)
+{
+    constexpr int LANES = kBlock / SEG;
+    __shared__ Exchange<V, LANES> maps[2][SEG][2];
+    const int lane = threadIdx.x % LANES, seg = threadIdx.x / LANES;
+    const uint32_t mine = blockIdx.x * LANES + lane, v = mine < a.vectors ? mine : a.vectors - 1;
+    const bool store = mine < a.vectors;  // the other lanes of the last workgroup repeat its last vector
     const Lane l = lane_of<V>(a, v);
     const LaneFlags<V, FL> lf(a, l);
-    const char *gate = a.gate + l.row * a.gate_n + (a.splat ? 0 : l.col * (int64_t)sizeof(T));
-    const char *before = a.out_r + l.row * a.out_n + l.col * sizeof(T);
-    const char *d_out = a.d_out ? a.d_out + l.row * a.d_out_n + l.col * sizeof(T) : nullptr;
-    char *d_gate = a.d_gate ? a.d_gate + l.row * a.d_gate_n + l.col * sizeof(T) : nullptr;
-    char *d_inp = a.d_inp ? a.d_inp + l.row * a.d_inp_n + l.col * sizeof(T) : nullptr;
-    const int64_t c = l.row * a.run + l.col;
-    float carry[V];
+    const Places<T> p(a, l);
+    const int64_t first = (int64_t)blockIdx.y * a.span, t1 = first + a.span < a.T ? first + a.span : a.T;
+    float h[V];
+    if (gridDim.y == 1) {
 #pragma unroll
-    for (int i = 0; i < V; i++) carry[i] = a.d_last ? a.d_last[c + i] : 0.0f;
-    for (int64_t t0 = 0; t0 < a.T; t0 += kUnroll) {
-        Raw<T, V> g[kUnroll], y[kUnroll], hb[kUnroll];
-        StepFlags<V, FL> f[kUnroll];
+        for (int i = 0; i < V; i++) h[i] = a.start ? a.start[l.channel + i] : 0.0f;
+    } else {  // each group composes its part of the spans before this one, then all go through the parts
+        const int64_t spans = blockIdx.y, part = ceil_div(spans, SEG);
+        float A[V], B[V];
 #pragma unroll
-        for (int k = 0; k < kUnroll; k++) {
-            const int64_t t = t0 + k < a.T ? t0 + k : a.T - 1;
-            load_gate<T, V>(g[k], gate + t * a.gate_t, a.splat);
-            f[k].load(lf, t * a.reset_t);
+        for (int i = 0; i < V; i++) A[i] = 1.0f, B[i] = 0.0f;
+        const int64_t end = (seg + 1) * part < spans ? (seg + 1) * part : spans;
+#pragma unroll 2
+        for (int64_t s = seg * part; s < end; s++) {
+            float A2[V], B2[V];
+            load_span<V>(a, 1 + 2 * s, v, A2);
+            load_span<V>(a, 2 + 2 * s, v, B2);
+            compose<V>(A, B, A2, B2);
         }
-        if (d_out) {
+        maps[1][seg][0].put(lane, A);
+        maps[1][seg][1].put(lane, B);
+        load_span<V>(a, 0, v, h);
+        __syncthreads();
+#pragma unroll 2
+        for (int s = 0; s < SEG; s++) {
+            float A2[V], B2[V];
+            maps[1][s][0].get(lane, A2);
+            maps[1][s][1].get(lane, B2);
 #pragma unroll
-            for (int k = 0; k < kUnroll; k++) {
-                const int64_t t = t0 + k < a.T ? t0 + k : a.T - 1;
-                y[k] = load_raw<T, V>(d_out + t * a.d_out_t);
-            }
-        }
-        if (d_gate) {
-#pragma unroll
-            for (int k = 0; k < kUnroll; k++) {  // the value before the first step is `state`, not in out
-                const int64_t t = t0 + k < a.T - 1 ? t0 + k : a.T - 2;
-                if (a.T > 1) hb[k] = load_raw<T, V>(before + t * a.out_t);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < kUnroll; k++) {
-            if (t0 + k >= a.T) break;
-            float d[V], dg[V];
-            const bool first = t0 + k == a.T - 1;
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                d[i] = (d_out ? raw_at(y[k], i) : 0.0f) + carry[i];
-                const bool begins = f[k].begins(i);
-                if (d_gate) {
-                    const float h = first ? (a.state ? a.state[c + i] : 0.0f) : raw_at(hb[k], i);
-                    dg[i] = begins ? 0.0f : d[i] * h;
-                }
-                carry[i] = begins ? 0.0f : raw_at(g[k], i) * d[i];
-            }
-            if (d_inp) store_from<T, V>(d_inp + (t0 + k) * a.d_inp_t, d, l.skip);
-            if (d_gate) store_from<T, V>(d_gate + (t0 + k) * a.d_gate_t, dg, l.skip);
+            for (int i = 0; i < V; i++) h[i] = through(A2[i], B2[i], h[i]);
         }
     }
-    if (a.d_state) {
+    int turn = 0;
+    constexpr int kSteps = unroll_of<V, FL>();
+    for (int64_t t0 = first; t0 < t1; t0 += SEG * kSteps, turn ^= 1) {
+        const int64_t ts = t0 + seg * kSteps;
+        Steps<T, V, FL, kSteps, BACKWARD, true> s;
+        s.load(a, lf, p.gate, p.add, p.before, ts, t1);
+        float A[V], B[V], from[V] = {};
+        bool starts[V];
+        identity<V>(A, B, starts);
+        s.reduce(A, B, starts);
+        mark<V>(A, starts);
+        maps[turn][seg][0].put(lane, A);
+        maps[turn][seg][1].put(lane, B);
+        __syncthreads();
+#pragma unroll 2
+        for (int q = 0; q < SEG; q++) {
+            float A2[V], B2[V];
+            maps[turn][q][0].get(lane, A2);
+            maps[turn][q][1].get(lane, B2);
 #pragma unroll
-        for (int i = 0; i < V; i++)
-            if (i >= l.skip) a.d_state[c + i] = carry[i];
+            for (int i = 0; i < V; i++) {
+                from[i] = q == seg ? h[i] : from[i];
+                h[i] = through(A2[i], B2[i], h[i]);
+            }
+        }
+        s.walk(a, l, store, p.to, p.d_gate, ts, from);
+    }
+    if (store && seg == 0 && blockIdx.y == gridDim.y - 1) store_end<V>(a, l, h);
+}
+
+// The (A, B) of every span: SEG groups of lanes reduce consecutive parts of it, joined through LDS.
+template <typename T, int V, int FL, bool BACKWARD>
+__global__ __launch_bounds__(kBlock) void recurrence_spans_kernel(RecArgs a)
+{
+    constexpr int SEG = 16, LANES = kBlock / SEG;
+    __shared__ Exchange<V, LANES> maps[SEG][2];
+    const int lane = threadIdx.x % LANES, seg = threadIdx.x / LANES;
+    const uint32_t mine = blockIdx.x * LANES + lane, v = mine < a.vectors ? mine : a.vectors - 1;
+    const Lane l = lane_of<V>(a, v);
+    const LaneFlags<V, FL> lf(a, l);
+    const Places<T> p(a, l);
+    const int64_t first = (int64_t)blockIdx.y * a.span, last = first + a.span < a.T ? first + a.span : a.T;
+    const int64_t part = ceil_div(a.span, SEG);
+    const int64_t from = first + seg * part, to = from + part < last ? from + part : last;
+    float A[V], B[V];
+    bool starts[V];
+    identity<V>(A, B, starts);
+    constexpr int kSteps = unroll_of<V, FL>();
+    for (int64_t t = from; t < to; t += kSteps) {
+        Steps<T, V, FL, kSteps, BACKWARD, true> s;
+        s.load(a, lf, p.gate, p.add, nullptr, t, to);
+        s.reduce(A, B, starts);
+    }
+    mark<V>(A, starts);
+    maps[seg][0].put(lane, A);
+    maps[seg][1].put(lane, B);
+    __syncthreads();
+    if (seg != 0 || mine >= a.vectors) return;
+#pragma unroll 2
+    for (int q = 1; q < SEG; q++) {
+        float A2[V], B2[V];
+        maps[q][0].get(lane, A2);
+        maps[q][1].get(lane, B2);
+        compose<V>(A, B, A2, B2);
+    }
+    const int64_t at = (int64_t)a.vectors * V;
+    float *to_span = a.spans + (int64_t)v * V;
+    store_vec<float, V>(to_span + (1 + 2 * (int64_t)blockIdx.y) * at, A);
+    store_vec<float, V>(to_span + (2 + 2 * (int64_t)blockIdx.y) * at, B);
+    if (blockIdx.y == 0) {  // the second kernel takes the start from here: `end` may be the array it comes from
+#pragma unroll
+        for (int i = 0; i < V; i++) A[i] = a.start ? a.start[l.channel + i] : 0.0f;
+        store_vec<float, V>(to_span, A);
     }
 }
 
@@ -225,6 +471,9 @@ struct Plan {
     RecArgs a;
     int vec;    // channels per lane: the type's 16 bytes, or 1 where a run is shorter than that
     int flags;
+    int seg;    // groups of lanes that share a workgroup's channels; 1: a lane walks all steps
+    int64_t spans;
+    int64_t workspace() const { return spans > 1 ? (1 + 2 * spans) * a.vectors * vec * (int64_t)sizeof(float) : 0; }
 };
 
 int check(const igx_recurrence *r, const char *who)
@@ -245,6 +494,24 @@ int check(const igx_recurrence *r, const char *who)
 // are environments n and n + 1 adjacent in this array?
 bool follows(const igx_recurrence *r, int64_t stride_n) { return r->envs == 1 || stride_n == r->width; }
 
+// How the time is split.  Lanes for the whole card (256 workgroups and more) walk the steps alone; down to 64 lanes a
+// workgroup its four groups share short rollouts; below, sixteen groups share the steps, and as long as that leaves CUs
+// without a workgroup the spans of a long sequence go to workgroups of their own.
+void split(Plan &p)
+{
+    const int64_t vectors = p.a.vectors, T = p.a.T;
+    p.spans = 1;
+    p.a.span = T;
+    p.seg = T <= kUnroll || vectors >= 131072 ? 1 : vectors >= 16384 ? 4 : 16;
+    if (p.seg != 16) return;
+    const int64_t strips = ceil_div(vectors, kBlock / 16), tile = 16 * kUnroll;
+    if (strips >= 256 || T <= tile) return;
+    const int64_t want = ceil_div(512, strips), most = ceil_div(T, tile);
+    const int64_t spans = want < most ? want : most;
+    p.a.span = ceil_div(ceil_div(T, spans), tile) * tile;
+    p.spans = ceil_div(T, p.a.span);
+}
+
 void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, Plan &p)
 {
     RecArgs &a = p.a;
@@ -262,13 +529,15 @@ void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, Plan &p)
     const bool one_gate = (r->gate_stride[1] == 0 || N == 1) && (r->gate_stride[2] == 0 || D == 1);
     flat = flat && (one_gate || (!shared && follows(r, r->gate_stride[1])));
     a.T = T;
-    a.D = D;
-    a.run = flat ? N * D : D;
+    a.D = (uint32_t)D;
+    a.run = (uint32_t)(flat ? N * D : D);
     a.splat = one_gate || shared;
-    p.vec = a.run >= (r->dtype == IGX_F32 ? 4 : 8) ? (r->dtype == IGX_F32 ? 4 : 8) : 1;
-    a.per_run = ceil_div(a.run, p.vec);
-    a.vectors = (flat ? 1 : N) * a.per_run;
-    p.flags = !r->reset ? kNoFlags : (p.vec == 1 || !flat || D % p.vec == 0 || N == 1) ? kOneFlag : kFlagEach;
+    const int vec = r->dtype == IGX_F32 ? 4 : 8;
+    p.vec = a.run >= (uint32_t)vec ? vec : 1;
+    a.per_run = (uint32_t)ceil_div(a.run, p.vec);
+    a.vectors = (uint32_t)(flat ? 1 : N) * a.per_run;
+    p.flags = !r->reset ? kNoFlags : (p.vec == 1 || !flat || D % p.vec == 0 || N == 1) ? kOneFlag : D >= p.vec ? kTwoFlags : kFlagEach;
+    split(p);
 
     // forward order: as stored, or turned round for reverse; the backward pass goes the other way through the same order
     const bool down = (r->reverse != 0) != (g != nullptr);
@@ -280,49 +549,71 @@ void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, Plan &p)
     };
     a.gate = turn(r->gate, r->gate_stride[0], r->gate_stride[1], e, a.gate_t, a.gate_n);
     a.reset = turn(r->reset, r->reset_stride[0], r->reset_stride[1], 8, a.reset_t, a.reset_n);
-    a.state = r->state;
     if (!g) {
-        a.inp = turn(r->inp, r->inp_stride[0], r->inp_stride[1], e, a.inp_t, a.inp_n);
-        a.out = const_cast<char *>(turn(r->out, r->out_stride[0], r->out_stride[1], e, a.out_t, a.out_n));
-        a.last = r->last;
+        a.add = turn(r->inp, r->inp_stride[0], r->inp_stride[1], e, a.add_t, a.add_n);
+        a.to = const_cast<char *>(turn(r->out, r->out_stride[0], r->out_stride[1], e, a.to_t, a.to_n));
+        a.start = r->state;
+        a.end = r->last;
     } else {
-        // the value before the step that comes first backwards (the last computed) is one step further on in out
-        a.out_r = turn(r->out, r->out_stride[0], r->out_stride[1], e, a.out_t, a.out_n);
-        if (a.out_r) a.out_r += a.out_t;
-        a.d_out = turn(g->d_out, g->d_out_stride[0], g->d_out_stride[1], e, a.d_out_t, a.d_out_n);
+        a.add = turn(g->d_out, g->d_out_stride[0], g->d_out_stride[1], e, a.add_t, a.add_n);
+        a.to = const_cast<char *>(turn(g->d_inp, g->d_inp_stride[0], g->d_inp_stride[1], e, a.to_t, a.to_n));
         a.d_gate = const_cast<char *>(turn(g->d_gate, g->d_gate_stride[0], g->d_gate_stride[1], e, a.d_gate_t, a.d_gate_n));
-        a.d_inp = const_cast<char *>(turn(g->d_inp, g->d_inp_stride[0], g->d_inp_stride[1], e, a.d_inp_t, a.d_inp_n));
-        a.d_last = g->d_last;
-        a.d_state = g->d_state;
+        if (a.d_gate) {  // the value before a step is one step further on in out, counted backwards
+            a.before = turn(r->out, r->out_stride[0], r->out_stride[1], e, a.before_t, a.before_n);
+            a.before += a.before_t;
+            a.state = r->state;
+        }
+        a.start = g->d_last;
+        a.end = g->d_state;
     }
 }
 
-template <int DT> void launch(const Plan &p, bool backward, hipStream_t s)
+template <typename T, int V, int FL, bool BACKWARD> void launch_as(const Plan &p, hipStream_t s)
+{
+    const dim3 block(kBlock);
+    const uint32_t v = p.a.vectors;
+    if (p.spans > 1)
+        recurrence_spans_kernel<T, V, FL, BACKWARD><<<dim3((unsigned)ceil_div(v, kBlock / 16), (unsigned)p.spans), block, 0, s>>>(p.a);
+    if (p.seg == 1) {
+        recurrence_kernel<T, V, FL, BACKWARD><<<dim3((unsigned)ceil_div(v, kBlock)), block, 0, s>>>(p.a);
+    } else if (p.seg == 4) {
+        recurrence_split_kernel<T, V, FL, BACKWARD, 4><<<dim3((unsigned)ceil_div(v, kBlock / 4)), block, 0, s>>>(p.a);
+    } else {
+        const dim3 grid((unsigned)ceil_div(v, kBlock / 16), (unsigned)p.spans);
+        recurrence_split_kernel<T, V, FL, BACKWARD, 16><<<grid, block, 0, s>>>(p.a);
+    }
+}
+
+template <int DT, bool BACKWARD> void launch_type(const Plan &p, hipStream_t s)
 {
     using T = typename Elem<DT>::type;
     constexpr int V = Elem<DT>::vec;
-    const dim3 grid((unsigned)ceil_div(p.a.vectors, kBlock)), block(kBlock);
-#define IGX_REC_GO(VV, FF)                                                                       \
-    do {                                                                                         \
-        if (backward) recurrence_backward_kernel<T, VV, FF><<<grid, block, 0, s>>>(p.a);         \
-        else recurrence_kernel<T, VV, FF><<<grid, block, 0, s>>>(p.a);                           \
-    } while (0)
     if (p.vec == 1) {
-        if (p.flags == kNoFlags) IGX_REC_GO(1, kNoFlags);
-        else IGX_REC_GO(1, kOneFlag);
+        if (p.flags == kNoFlags) launch_as<T, 1, kNoFlags, BACKWARD>(p, s);
+        else launch_as<T, 1, kOneFlag, BACKWARD>(p, s);
     } else {
-        if (p.flags == kNoFlags) IGX_REC_GO(V, kNoFlags);
-        else if (p.flags == kOneFlag) IGX_REC_GO(V, kOneFlag);
-        else IGX_REC_GO(V, kFlagEach);
+        if (p.flags == kNoFlags) launch_as<T, V, kNoFlags, BACKWARD>(p, s);
+        else if (p.flags == kOneFlag) launch_as<T, V, kOneFlag, BACKWARD>(p, s);
+        else if (p.flags == kTwoFlags) launch_as<T, V, kTwoFlags, BACKWARD>(p, s);
+        else launch_as<T, V, kFlagEach, BACKWARD>(p, s);
     }
-#undef IGX_REC_GO
 }
 
-void launch_any(int dtype, const Plan &p, bool backward, hipStream_t s)
+template <bool BACKWARD> int launch(const igx_recurrence *r, Plan &p, hipStream_t s, const char *who)
 {
-    if (dtype == IGX_F32) launch<IGX_F32>(p, backward, s);
-    else if (dtype == IGX_F16) launch<IGX_F16>(p, backward, s);
-    else launch<IGX_BF16>(p, backward, s);
+    const int64_t need = p.workspace();
+    if (need) {
+        if (!r->workspace) return fail(IGX_E_NULL, "%s: workspace is NULL", who);
+        if (!aligned16(r->workspace)) return fail(IGX_E_ALIGN, "%s: workspace must be 16-byte aligned", who);
+        if (r->workspace_bytes < need)
+            return fail(IGX_E_SIZE, "%s: workspace of %lld bytes is smaller than igx_linear_recurrence_workspace()", who,
+                        (long long)r->workspace_bytes);
+        p.a.spans = static_cast<float *>(r->workspace);
+    }
+    if (r->dtype == IGX_F32) launch_type<IGX_F32, BACKWARD>(p, s);
+    else if (r->dtype == IGX_F16) launch_type<IGX_F16, BACKWARD>(p, s);
+    else launch_type<IGX_BF16, BACKWARD>(p, s);
+    return launch_status(who);
 }
 
 int carry_through(const float *from, float *to, int64_t n, hipStream_t s, const char *who)
@@ -338,7 +629,19 @@ int carry_through(const float *from, float *to, int64_t n, hipStream_t s, const 
 extern "C" int64_t igx_linear_recurrence_workspace(const igx_recurrence *r)
 {
     const int rc = igx::check(r, __func__);
-    return rc ? rc : 0;
+    if (rc) return rc;
+    // which environments follow each other decides how many lanes there are, and that differs with the arrays of the two
+    // passes: the most that either could need, from lanes per environment and lanes over all of them
+    int64_t most = 0;
+    if (r->steps == 0 || r->envs == 0 || r->width == 0) return 0;
+    igx_recurrence q = *r;
+    for (int apart = 0; apart < 2; apart++) {
+        q.inp_stride[1] = q.out_stride[1] = r->width + apart;
+        igx::Plan p;
+        igx::make_plan(&q, nullptr, p);
+        if (p.workspace() > most) most = p.workspace();
+    }
+    return most;
 }
 
 extern "C" int igx_linear_recurrence(const igx_recurrence *r, igx_stream_t stream)
@@ -354,8 +657,7 @@ extern "C" int igx_linear_recurrence(const igx_recurrence *r, igx_stream_t strea
     IGX_REQUIRE_PTR(r->out, "out");
     igx::Plan p;
     igx::make_plan(r, nullptr, p);
-    igx::launch_any(r->dtype, p, false, s);
-    return igx::launch_status(__func__);
+    return igx::launch<false>(r, p, s, __func__);
 }
 
 extern "C" int igx_linear_recurrence_backward(const igx_recurrence *r, const igx_recurrence_grad *g, igx_stream_t stream)
@@ -371,6 +673,5 @@ extern "C" int igx_linear_recurrence_backward(const igx_recurrence *r, const igx
     if (g->d_gate) IGX_REQUIRE_PTR(r->out, "out");
     igx::Plan p;
     igx::make_plan(r, g, p);
-    igx::launch_any(r->dtype, p, true, s);
-    return igx::launch_status(__func__);
+    return igx::launch<true>(r, p, s, __func__);
 }
