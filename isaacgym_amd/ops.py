@@ -692,51 +692,66 @@ class WindowQuantile:
 # ---- sequence operators (isaacgym_amd.sequence differentiates through them) ----------------------
 _ELEMENTS = {torch.float32: _abi.IGX_F32, torch.float16: _abi.IGX_F16, torch.bfloat16: _abi.IGX_BF16}
 _ACTIVATIONS = {"none": _abi.IGX_GATE_NONE, "sigmoid": _abi.IGX_GATE_SIGMOID, "silu": _abi.IGX_GATE_SILU}
+_GROUP = _abi.IGX_PACK8_GROUP
 
 
 def _element(t, name):
-    """The ABI's number of a tensor's element type."""
+    """The ABI's number of a device tensor's element type."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s: expected a torch.Tensor, got %r" % (name, type(t)))
-    if t.dtype not in _ELEMENTS:
+    e = _ELEMENTS.get(t.dtype)
+    if e is None:
         raise TypeError("%s: expected float32, float16 or bfloat16, got %s" % (name, t.dtype))
-    return _ELEMENTS[t.dtype]
+    if not t.is_cuda:
+        raise ValueError("libigx works on device tensors only (%s is a %s tensor)" % (name, t.device))
+    return e
 
 
-def _same(t, name, shape, dtype, dev):
-    """t is a device tensor of that shape, type and device."""
+def _same(t, name, shape, dtype, like):
+    """t is a tensor of that shape and type on the device of the device tensor `like`."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == like.get_device():
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s: expected a torch.Tensor, got %r" % (name, type(t)))
     if not t.is_cuda:
         raise ValueError("libigx works on device tensors only (%s is a %s tensor)" % (name, t.device))
     if t.dtype != dtype:
         raise TypeError("%s: expected dtype %s, got %s" % (name, dtype, t.dtype))
-    if t.device != dev:
-        raise ValueError("%s is on %s, others on %s" % (name, t.device, dev))
-    if t.shape != shape:
-        raise ValueError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    if t.device != like.device:
+        raise ValueError("%s is on %s, others on %s" % (name, t.device, like.device))
+    raise ValueError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
 
 
-def _packed(t, name, shape, dtype, dev):
+def _packed(t, name, shape, dtype, like):
     """The address of a contiguous tensor (None: NULL)."""
     if t is None:
         return None
-    _same(t, name, shape, dtype, dev)
+    _same(t, name, shape, dtype, like)
     if not t.is_contiguous():
         raise ValueError("%s must be contiguous" % name)
     return t.data_ptr()
 
 
-def _rollout(t, name, shape, dtype, dev, written=False):
+def _scratch(size, device):
+    """(tensor, address, bytes) of a call's workspace; the tensor goes back to the stream's pool after the launch."""
+    if size < 0:
+        _lib.check(size)
+    if size == 0:
+        return None, None, 0
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), size
+
+
+def _rollout(t, name, shape, like, written=False):
     """(address, (stride over steps, stride over environments)) of a [T, N, D] tensor with adjacent channels, any
     strides otherwise; one that is written must not map two elements to one address."""
     if t is None:
         return None, (0, 0)
-    _same(t, name, shape, dtype, dev)
+    _same(t, name, shape, like.dtype, like)
     st, sn, sd = t.stride()
-    if shape[2] > 1 and sd != 1:
+    if sd != 1 and shape[2] > 1:
         raise ValueError("%s: the channels (last dimension) must be adjacent, their stride is %d" % (name, sd))
-    if written and t.numel() and not t.is_contiguous():
+    if written and not t.is_contiguous() and t.numel():
         reach = 0
         for s, n in sorted((s, n) for s, n in zip(t.stride(), shape) if n > 1):
             if s <= reach:
@@ -745,50 +760,43 @@ def _rollout(t, name, shape, dtype, dev, written=False):
     return t.data_ptr(), (st, sn)
 
 
-def _recurrence(gate, inp_like, state, reset, reverse):
-    """igx_recurrence with the arguments that forward and backward share; inp_like gives shape, type and device."""
-    if not isinstance(inp_like, torch.Tensor) or inp_like.dim() != 3:
+def _recurrence(gate, like, state, reset, reverse):
+    """igx_recurrence with the arguments that forward and backward share; `like` gives shape, type and device."""
+    if isinstance(like, torch.Tensor) and like.dim() != 3:
         raise ValueError("linear_recurrence: rollouts are [steps, environments, channels] tensors")
-    shape, dtype, dev = inp_like.shape, inp_like.dtype, inp_like.device
-    r = _abi.Recurrence(dtype=_element(inp_like, "inp"), reverse=int(bool(reverse)), steps=shape[0], envs=shape[1],
-                        width=shape[2])
-    _same(gate, "gate", shape, dtype, dev)
-    sd = gate.stride(2) if shape[2] > 1 else 1
-    if sd not in (0, 1):
+    e = _element(like, "inp")
+    shape = like.shape
+    r = _abi.Recurrence()
+    r.dtype, r.reverse, (r.steps, r.envs, r.width) = e, 1 if reverse else 0, shape
+    _same(gate, "gate", shape, like.dtype, like)
+    st, sn, sd = gate.stride()
+    if shape[2] <= 1:
+        sd = 1
+    if sd != 0 and sd != 1:
         raise ValueError("gate: the channels (last dimension) must be adjacent or share one gate, their stride is %d" % sd)
-    r.gate = gate.data_ptr()
-    r.gate_stride[:] = (gate.stride(0), gate.stride(1), sd)
-    r.state = _packed(state, "state", shape[1:], torch.float32, dev)
+    r.gate, r.gate_stride = gate.data_ptr(), (st, sn, sd)
+    r.state = _packed(state, "state", shape[1:], torch.float32, like)
     if reset is not None:
-        _same(reset, "reset", shape[:2], torch.int64, dev)
-        r.reset = reset.data_ptr()
-        r.reset_stride[:] = reset.stride()
-    return r, shape, dtype, dev
-
-
-def _recurrence_workspace(r, dev):
-    size = int(_lib.lib().igx_linear_recurrence_workspace(C.byref(r)))
-    if size < 0:
-        _lib.check(size)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    r.workspace, r.workspace_bytes = (ws.data_ptr(), size) if size else (None, 0)
-    return ws
+        _same(reset, "reset", shape[:2], torch.int64, like)
+        r.reset, r.reset_stride = reset.data_ptr(), reset.stride()
+    return r, shape
 
 
 def linear_recurrence(gate, inp, out, state=None, reset=None, last=None, reverse=False):
     """out[t] = gate[t] * (out before it) + inp[t] over [T, N, D] (igx_linear_recurrence).  gate, inp and out share a type
     and need adjacent channels (gate also one value for all channels of an environment); state and last are fp32 [N, D]
     (last may be state), reset int64 [T, N].  out must not overlap an input."""
-    r, shape, dtype, dev = _recurrence(gate, inp, state, reset, reverse)
-    r.inp, r.inp_stride[:] = _rollout(inp, "inp", shape, dtype, dev)
-    r.out, r.out_stride[:] = _rollout(out, "out", shape, dtype, dev, written=True)
+    r, shape = _recurrence(gate, inp, state, reset, reverse)
+    r.inp, r.inp_stride = _rollout(inp, "inp", shape, inp)
     if out is None:
         raise TypeError("out: expected a torch.Tensor, got None")
-    if out.numel() and out.data_ptr() in (gate.data_ptr(), inp.data_ptr()):
+    r.out, r.out_stride = _rollout(out, "out", shape, inp, written=True)
+    if r.out is not None and r.out in (r.gate, r.inp) and out.numel():
         raise ValueError("out must not overlap an input")
-    r.last = _packed(last, "last", shape[1:], torch.float32, dev)
-    ws = _recurrence_workspace(r, dev)  # noqa: F841 (freed to the stream's pool after the launch)
-    _lib.check(_lib._launch(_lib.lib().igx_linear_recurrence, dev, C.byref(r)))
+    r.last = _packed(last, "last", shape[1:], torch.float32, inp)
+    L = _lib.lib()
+    ws, r.workspace, r.workspace_bytes = _scratch(L.igx_linear_recurrence_workspace(C.byref(r)), inp.device)
+    _lib.check(_lib._launch(L.igx_linear_recurrence, inp.device, C.byref(r)))
     return out
 
 
@@ -796,115 +804,126 @@ def linear_recurrence_backward(gate, out, d_out=None, d_last=None, d_gate=None, 
                                reset=None, reverse=False):
     """The gradients of linear_recurrence (igx_linear_recurrence_backward): those of d_gate, d_inp [T, N, D] and d_state
     [N, D] that are given are filled in; d_out and d_last None stand for zeros."""
-    r, shape, dtype, dev = _recurrence(gate, out, state, reset, reverse)
-    r.out, r.out_stride[:] = _rollout(out, "out", shape, dtype, dev)
+    r, shape = _recurrence(gate, out, state, reset, reverse)
+    r.out, r.out_stride = _rollout(out, "out", shape, out)
     g = _abi.RecurrenceGrad()
-    g.d_out, g.d_out_stride[:] = _rollout(d_out, "d_out", shape, dtype, dev)
-    g.d_gate, g.d_gate_stride[:] = _rollout(d_gate, "d_gate", shape, dtype, dev, written=True)
-    g.d_inp, g.d_inp_stride[:] = _rollout(d_inp, "d_inp", shape, dtype, dev, written=True)
-    g.d_last = _packed(d_last, "d_last", shape[1:], torch.float32, dev)
-    g.d_state = _packed(d_state, "d_state", shape[1:], torch.float32, dev)
-    ws = _recurrence_workspace(r, dev)  # noqa: F841
-    _lib.check(_lib._launch(_lib.lib().igx_linear_recurrence_backward, dev, C.byref(r), C.byref(g)))
+    g.d_out, g.d_out_stride = _rollout(d_out, "d_out", shape, out)
+    g.d_gate, g.d_gate_stride = _rollout(d_gate, "d_gate", shape, out, written=True)
+    g.d_inp, g.d_inp_stride = _rollout(d_inp, "d_inp", shape, out, written=True)
+    g.d_last = _packed(d_last, "d_last", shape[1:], torch.float32, out)
+    g.d_state = _packed(d_state, "d_state", shape[1:], torch.float32, out)
+    L = _lib.lib()
+    ws, r.workspace, r.workspace_bytes = _scratch(L.igx_linear_recurrence_workspace(C.byref(r)), out.device)
+    _lib.check(_lib._launch(L.igx_linear_recurrence_backward, out.device, C.byref(r), C.byref(g)))
 
 
-def _row_array(t, name, shape, dtype, dev):
-    """(address, stride) of a [rows, width] tensor whose columns are adjacent."""
+def _row_array(t, name, shape, like):
+    """(address, stride from row to row) of a [..., width] tensor with adjacent columns and evenly spaced rows."""
     if t is None:
         return None, 0
-    _same(t, name, shape, dtype, dev)
-    if shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError("%s: the columns must be adjacent, their stride is %d" % (name, t.stride(1)))
-    return t.data_ptr(), t.stride(0) if shape[0] > 1 else shape[1]
+    _same(t, name, shape, like.dtype, like)
+    if t.is_contiguous():
+        return t.data_ptr(), shape[-1]
+    try:
+        rows = t.view(-1, shape[-1])
+    except RuntimeError:
+        raise ValueError("%s: its rows (all but the last dimension) must be evenly spaced" % name) from None
+    if shape[-1] > 1 and rows.stride(1) != 1:
+        raise ValueError("%s: the columns (last dimension) must be adjacent, their stride is %d" % (name, rows.stride(1)))
+    return rows.data_ptr(), rows.stride(0) if rows.shape[0] > 1 else shape[-1]
 
 
-def _block_norm(x_like, weight, gate, scale, next_weight, activation, eps, y_inv_rms, out_inv_rms, codes):
-    if not isinstance(x_like, torch.Tensor) or x_like.dim() != 2:
-        raise ValueError("block_norm: rows are [rows, width] tensors")
-    if activation not in _ACTIVATIONS:
+def _rows_of(t, name):
+    """(element type, rows, width, shape of the scales of its 8-bit codes) of a [..., width] tensor."""
+    e = _element(t, name)
+    if t.dim() < 1:
+        raise ValueError("%s: rows are [..., width] tensors" % name)
+    width = t.shape[-1]
+    return e, t.numel() // width if width else 0, width, t.shape[:-1] + (-(-width // _GROUP),)
+
+
+def _block_norm(like, weight, gate, scale, next_weight, inv_rms, codes, activation, eps):
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError("activation must be one of %s, got %r" % (sorted(_ACTIVATIONS), activation))
-    shape, dev = x_like.shape, x_like.device
-    b = _abi.BlockNorm(dtype=_element(x_like, "x"), activation=_ACTIVATIONS[activation], rows=shape[0], width=shape[1],
-                       eps=float(eps))
-    f = torch.float32
-    for k, t in (("weight", weight), ("scale", scale), ("next_weight", next_weight)):
-        setattr(b, k, _packed(t, k, shape[1:], f, dev))
-    for k, t in (("y_inv_rms", y_inv_rms), ("out_inv_rms", out_inv_rms)):
-        setattr(b, k, _packed(t, k, shape[:1], f, dev))
-    groups = -(-shape[1] // _abi.IGX_PACK8_GROUP)
-    for k, pair in zip(("y8", "gate8"), codes):
-        if pair is not None:
-            setattr(b, k, _packed(pair[0], k, shape, torch.int8, dev))
-            setattr(b, k + "_scale", _packed(pair[1], k + "_scale", (shape[0], groups), f, dev))
-    return b, shape, x_like.dtype, dev
+    e, rows, width, scales_shape = _rows_of(like, "x")
+    b = _abi.BlockNorm()
+    b.dtype, b.activation, b.rows, b.width, b.eps = e, act, rows, width, eps
+    vector, f = like.shape[-1:], torch.float32
+    b.weight = _packed(weight, "weight", vector, f, like)
+    b.scale = _packed(scale, "scale", vector, f, like)
+    b.next_weight = _packed(next_weight, "next_weight", vector, f, like)
+    if inv_rms is not None:
+        b.y_inv_rms = _packed(inv_rms, "inv_rms", (2, rows), f, like)
+        b.out_inv_rms = b.y_inv_rms + 4 * rows if rows else None
+    if codes is not None:
+        b.y8 = _packed(codes[0], "y codes", like.shape, torch.int8, like)
+        b.y8_scale = _packed(codes[1], "y scales", scales_shape, f, like)
+        if len(codes) == 4:
+            b.gate8 = _packed(codes[2], "gate codes", like.shape, torch.int8, like)
+            b.gate8_scale = _packed(codes[3], "gate scales", scales_shape, f, like)
+    return b
 
 
-def block_norm(x, y=None, weight=None, gate=None, scale=None, next_weight=None, out=None, next=None, y_inv_rms=None,
-               out_inv_rms=None, y_codes=None, gate_codes=None, activation="silu", eps=1e-5):
+def block_norm(x, y=None, weight=None, gate=None, scale=None, next_weight=None, out=None, next=None, inv_rms=None, codes=None,
+               activation="silu", eps=1e-5):
     """out = x + scale * act(gate) * (rms(y) * weight) and next = rms(out) * next_weight, row by row (igx_block_norm_forward;
-    without y: out = x).  x, y, gate are [rows, width] with adjacent columns, out and next contiguous; parameters fp32
-    [width]; y_codes / gate_codes: (codes, scales) to fill in."""
-    b, shape, dtype, dev = _block_norm(x, weight, gate, scale, next_weight, activation, eps, y_inv_rms, out_inv_rms,
-                                       (y_codes, gate_codes))
-    b.x, b.x_stride = _row_array(x, "x", shape, dtype, dev)
-    b.y, b.y_stride = _row_array(y, "y", shape, dtype, dev)
-    b.gate, b.gate_stride = _row_array(gate, "gate", shape, dtype, dev)
-    b.out = _packed(out, "out", shape, dtype, dev)
-    b.next = _packed(next, "next", shape, dtype, dev)
-    _lib.check(_lib._launch(_lib.lib().igx_block_norm_forward, dev, C.byref(b)))
+    without y: out = x).  x, y, gate are [..., width] with adjacent columns and evenly spaced rows, out and next
+    contiguous, parameters fp32 [width].  Filled in where given: inv_rms fp32 [2, rows], the rows' 1 / rms of y and of out
+    (what block_norm_backward needs); codes: the 8-bit checkpoint, (codes, scales) of y - of x without y - and then of
+    gate if there is one."""
+    b = _block_norm(x, weight, gate, scale, next_weight, inv_rms, codes, activation, eps)
+    shape = x.shape
+    b.x, b.x_stride = _row_array(x, "x", shape, x)
+    b.y, b.y_stride = _row_array(y, "y", shape, x)
+    b.gate, b.gate_stride = _row_array(gate, "gate", shape, x)
+    b.out = _packed(out, "out", shape, x.dtype, x)
+    b.next = _packed(next, "next", shape, x.dtype, x)
+    _lib.check(_lib._launch(_lib.lib().igx_block_norm_forward, x.device, C.byref(b)))
 
 
-def block_norm_backward(rows_like, x=None, y=None, weight=None, gate=None, scale=None, next_weight=None, y_inv_rms=None,
-                        out_inv_rms=None, y_codes=None, gate_codes=None, activation="silu", eps=1e-5, d_out=None,
-                        d_next=None, d_x=None, d_y=None, d_gate=None, d_weight=None, d_scale=None, d_next_weight=None):
-    """The gradients of block_norm (igx_block_norm_backward): those given are filled in.  rows_like: a [rows, width] tensor of
-    the rows' type and device.  y_codes (gate_codes) in place of y (gate; of x in a call without a block): the gradients at
-    the values the codes stand for."""
-    b, shape, dtype, dev = _block_norm(rows_like, weight, gate, scale, next_weight, activation, eps, y_inv_rms, out_inv_rms,
-                                       (y_codes, gate_codes))
-    b.x, b.x_stride = _row_array(x, "x", shape, dtype, dev)
-    b.y, b.y_stride = _row_array(y, "y", shape, dtype, dev)
-    b.gate, b.gate_stride = _row_array(gate, "gate", shape, dtype, dev)
-    if weight is not None and y is None and y_codes is not None:
-        b.y = b.y8  # says that there is a block; not read
-    if gate is None and gate_codes is not None:
-        b.gate = b.gate8
+def block_norm_backward(like, x=None, y=None, weight=None, gate=None, scale=None, next_weight=None, inv_rms=None, codes=None,
+                        activation="silu", eps=1e-5, d_out=None, d_next=None, d_x=None, d_y=None, d_gate=None, d_weight=None,
+                        d_scale=None, d_next_weight=None):
+    """The gradients of block_norm (igx_block_norm_backward): those given are filled in.  like: a [..., width] tensor of
+    the rows' shape, type and device.  codes in place of y and gate (of x in a call without a block): the gradients at the
+    values the codes stand for."""
+    b = _block_norm(like, weight, gate, scale, next_weight, inv_rms, codes, activation, eps)
+    shape, dtype = like.shape, like.dtype
+    b.x, b.x_stride = _row_array(x, "x", shape, like)
+    b.y, b.y_stride = _row_array(y, "y", shape, like)
+    b.gate, b.gate_stride = _row_array(gate, "gate", shape, like)
+    if codes is not None and weight is not None:  # with codes these only say which parts there are
+        b.y, b.gate = b.y8, b.gate8
     g = _abi.BlockNormGrad()
-    g.d_out, g.d_out_stride = _row_array(d_out, "d_out", shape, dtype, dev)
-    g.d_next, g.d_next_stride = _row_array(d_next, "d_next", shape, dtype, dev)
-    for k, t in (("d_x", d_x), ("d_y", d_y), ("d_gate", d_gate)):
-        setattr(g, k, _packed(t, k, shape, dtype, dev))
-    for k, t in (("d_weight", d_weight), ("d_scale", d_scale), ("d_next_weight", d_next_weight)):
-        setattr(g, k, _packed(t, k, shape[1:], torch.float32, dev))
-    ws = None
+    g.d_out, g.d_out_stride = _row_array(d_out, "d_out", shape, like)
+    g.d_next, g.d_next_stride = _row_array(d_next, "d_next", shape, like)
+    g.d_x = _packed(d_x, "d_x", shape, dtype, like)
+    g.d_y = _packed(d_y, "d_y", shape, dtype, like)
+    g.d_gate = _packed(d_gate, "d_gate", shape, dtype, like)
+    vector, f = shape[-1:], torch.float32
+    g.d_weight = _packed(d_weight, "d_weight", vector, f, like)
+    g.d_scale = _packed(d_scale, "d_scale", vector, f, like)
+    g.d_next_weight = _packed(d_next_weight, "d_next_weight", vector, f, like)
+    L = _lib.lib()
     if d_weight is not None or d_scale is not None or d_next_weight is not None:
-        size = int(_lib.lib().igx_block_norm_workspace(C.byref(b)))
-        if size < 0:
-            _lib.check(size)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        g.workspace, g.workspace_bytes = ws.data_ptr(), size
-    _lib.check(_lib._launch(_lib.lib().igx_block_norm_backward, dev, C.byref(b), C.byref(g)))
+        ws, g.workspace, g.workspace_bytes = _scratch(L.igx_block_norm_workspace(C.byref(b)), like.device)
+    _lib.check(_lib._launch(L.igx_block_norm_backward, like.device, C.byref(b), C.byref(g)))
 
 
 def pack8(x, codes, scales):
-    """codes int8 [rows, width] and scales fp32 [rows, ceil(width / 64)] of x [rows, width] (igx_pack8)."""
-    if not isinstance(x, torch.Tensor) or x.dim() != 2:
-        raise ValueError("pack8: x must be a [rows, width] tensor")
-    shape, dev = x.shape, x.device
-    dt = _element(x, "x")
-    p, stride = _row_array(x, "x", shape, x.dtype, dev)
-    q = _packed(codes, "codes", shape, torch.int8, dev)
-    s = _packed(scales, "scales", (shape[0], -(-shape[1] // _abi.IGX_PACK8_GROUP)), torch.float32, dev)
-    _lib.check(_lib._launch(_lib.lib().igx_pack8, dev, p, dt, shape[0], shape[1], stride, q, s))
+    """codes int8 [..., width] and scales fp32 [..., ceil(width / 64)] of x [..., width] (igx_pack8)."""
+    e, rows, width, scales_shape = _rows_of(x, "x")
+    p, stride = _row_array(x, "x", x.shape, x)
+    q = _packed(codes, "codes", x.shape, torch.int8, x)
+    s = _packed(scales, "scales", scales_shape, torch.float32, x)
+    _lib.check(_lib._launch(_lib.lib().igx_pack8, x.device, p, e, rows, width, stride, q, s))
 
 
 def unpack8(codes, scales, out):
-    """out [rows, width] = the values that codes and scales stand for (igx_unpack8)."""
-    if not isinstance(out, torch.Tensor) or out.dim() != 2:
-        raise ValueError("unpack8: out must be a [rows, width] tensor")
-    shape, dev = out.shape, out.device
-    dt = _element(out, "out")
-    q = _packed(codes, "codes", shape, torch.int8, dev)
-    s = _packed(scales, "scales", (shape[0], -(-shape[1] // _abi.IGX_PACK8_GROUP)), torch.float32, dev)
-    o = _packed(out, "out", shape, out.dtype, dev)
-    _lib.check(_lib._launch(_lib.lib().igx_unpack8, dev, q, s, dt, shape[0], shape[1], o))
+    """out [..., width] = the values that codes and scales stand for (igx_unpack8)."""
+    e, rows, width, scales_shape = _rows_of(out, "out")
+    q = _packed(codes, "codes", out.shape, torch.int8, out)
+    s = _packed(scales, "scales", scales_shape, torch.float32, out)
+    o = _packed(out, "out", out.shape, out.dtype, out)
+    _lib.check(_lib._launch(_lib.lib().igx_unpack8, out.device, q, s, e, rows, width, o))

@@ -17,47 +17,56 @@ fallback.  Calls only enqueue work on the current stream and can be captured int
 together; a capture while an eager graph of one of the same leaf tensors is alive is refused, because torch would add
 the captured gradient to the leaf on the eager stream.
 """
+from weakref import WeakSet
+
 import torch
 from torch.autograd.function import once_differentiable
-from torch.utils.weak import WeakIdKeyDictionary
-from weakref import WeakSet
 
 from . import _abi, ops
 
-_eager_nodes = WeakIdKeyDictionary()  # leaf -> the live autograd nodes that an eager call made with it
+_live = WeakSet()  # the autograd nodes of eager calls that hang on leaf tensors, as long as their graphs live
 
 
 def _capture_guard(ctx, tensors):
     """Eager: remember that this node hangs on its leaves.  Captured: refuse leaves on which an eager node still hangs."""
-    leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
+    leaves = [id(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf]
     if not leaves:
         return
-    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-        for t in leaves:
-            if len(_eager_nodes.get(t, ())):
+    if torch.cuda.is_current_stream_capturing():
+        for node in list(_live):
+            if not node.leaves.isdisjoint(leaves):
                 raise RuntimeError("a tensor that requires grad is still part of an eager autograd graph: release that "
                                    "graph's outputs before capturing one with the same tensor")
         return
-    for t in leaves:
-        nodes = _eager_nodes.get(t)
-        if nodes is None:
-            nodes = _eager_nodes[t] = WeakSet()
-        nodes.add(ctx)
+    ctx.leaves = frozenset(leaves)  # the graph keeps the leaves alive, so their ids stay theirs
+    _live.add(ctx)
+
+
+def _differentiated(*tensors):
+    """Whether autograd has to see the call (going past it saves half the host time of a small one)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 # ---- gated linear recurrence -------------------------------------------------------------------
+
+def _run_recurrence(gate, inp, state, reset, reverse):
+    out = torch.empty_like(inp)  # in inp's layout, so that neighbouring operators see the one they were given
+    if not _adjacent(out):
+        out = torch.empty(inp.shape, dtype=inp.dtype, device=inp.device)
+    last = torch.empty(inp.shape[1:], dtype=torch.float32, device=inp.device)
+    ops.linear_recurrence(gate, inp, out, state=state, reset=reset, last=last, reverse=reverse)
+    return out, last
+
 
 class _LinearRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, inp, state, reset, reverse):
         ctx.set_materialize_grads(False)
-        out = torch.empty_like(inp)  # in inp's layout, so that neighbouring operators see the one they were given
-        if not _adjacent(out):
-            out = torch.empty(inp.shape, dtype=inp.dtype, device=inp.device)
-        last = torch.empty(inp.shape[1:], dtype=torch.float32, device=inp.device)
-        ops.linear_recurrence(gate, inp, out, state=state, reset=reset, last=last, reverse=reverse)
-        if any(ctx.needs_input_grad[:3]):
+        needed = any(ctx.needs_input_grad)
+        if needed and inp.is_cuda:
             _capture_guard(ctx, (gate, inp, state))
+        out, last = _run_recurrence(gate, inp, state, reset, reverse)
+        if needed:
             ctx.save_for_backward(gate, out, state, reset)
             ctx.reverse = reverse
         return out, last
@@ -98,7 +107,8 @@ def linear_recurrence(gate, inp, state=None, reset=None, reverse=False):
     `out` as stored.  Products of consecutive gates have to stay within float32's range (gates in [-1, 1] always do)."""
     if gate.shape != inp.shape:
         gate = gate.expand(inp.shape)
-    return _LinearRecurrence.apply(gate, inp, state, reset, bool(reverse))
+    run = _LinearRecurrence.apply if _differentiated(gate, inp, state) else _run_recurrence
+    return run(gate, inp, state, reset, bool(reverse))
 
 
 def linear_recurrence_step(gate, inp, state, reset=None, state_out=None, out=None):
@@ -118,64 +128,43 @@ def linear_recurrence_step(gate, inp, state, reset=None, state_out=None, out=Non
 
 # ---- norms before and after a block --------------------------------------------------------------
 
-def _rows(t, name):
-    """t [..., width] as [rows, width], never copied."""
-    if not isinstance(t, torch.Tensor) or t.dim() < 1:
-        raise ValueError("%s must be a tensor of at least one dimension" % name)
-    width = t.shape[-1]
-    try:
-        return t.view(t.numel() // width if width else 0, width)
-    except RuntimeError:
-        raise ValueError("%s: its rows (all but the last dimension) must be evenly spaced" % name) from None
-
-
-def _row_grad(t, rows, width):
-    """An incoming gradient as [rows, width] with adjacent columns; autograd may hand in any strides."""
-    if t is None:
-        return None
-    t = t.reshape(rows, width)
-    return t if width <= 1 or t.stride(1) == 1 else t.contiguous()
+def _row_grad(t):
+    """An incoming gradient with adjacent columns and evenly spaced rows; autograd may hand in any strides."""
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _code_buffers(t):
-    rows, width = t.shape
-    return (torch.empty(rows, width, dtype=torch.int8, device=t.device),
-            torch.empty(rows, -(-width // _abi.IGX_PACK8_GROUP), dtype=torch.float32, device=t.device))
+    return (torch.empty(t.shape, dtype=torch.int8, device=t.device),
+            torch.empty(t.shape[:-1] + (-(-t.shape[-1] // _abi.IGX_PACK8_GROUP),), dtype=torch.float32, device=t.device))
+
+
+def _run_block_norm(x, y, weight, gate, scale, next_weight, activation, eps, inv_rms=None, codes=None):
+    """(out, next) of ops.block_norm; without y (a norm in front of the first block) out is None."""
+    out = None if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    nxt = None if next_weight is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    ops.block_norm(x, y=y, weight=weight, gate=gate, scale=scale, next_weight=next_weight, out=out, next=nxt,
+                   inv_rms=inv_rms, codes=codes, activation=activation, eps=eps)
+    return out, nxt
 
 
 class _BlockNorm(torch.autograd.Function):
-    """(out, next) of ops.block_norm; without y (a norm in front of the first block) out is None."""
-
     @staticmethod
     def forward(ctx, x, y, weight, gate, scale, next_weight, activation, eps, checkpoint):
         ctx.set_materialize_grads(False)
-        xr = _rows(x, "x")
-        yr = None if y is None else _rows(y, "y")
-        gr = None if gate is None else _rows(gate, "gate")
-        rows, width = xr.shape
         needed = any(ctx.needs_input_grad)
-        dev = x.device
-
-        def row_stat(wanted):
-            return torch.empty(rows, dtype=torch.float32, device=dev) if wanted and needed else None
-
-        out = None if y is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-        nxt = None if next_weight is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-        y_inv, out_inv = row_stat(y is not None), row_stat(next_weight is not None)
-        codes = needed and checkpoint
-        y_codes = _code_buffers(xr) if codes else None
-        gate_codes = _code_buffers(xr) if codes and gate is not None else None
-        ops.block_norm(xr, y=yr, weight=weight, gate=gr, scale=scale, next_weight=next_weight,
-                       out=None if out is None else out.view(rows, width), next=None if nxt is None else nxt.view(rows, width),
-                       y_inv_rms=y_inv, out_inv_rms=out_inv, y_codes=y_codes, gate_codes=gate_codes, activation=activation,
-                       eps=eps)
-        if needed:
+        if needed and x.is_cuda:
             _capture_guard(ctx, (x, y, weight, gate, scale, next_weight))
-            keep_x = next_weight is not None and (y is not None or not codes)
-            ctx.save_for_backward(xr if keep_x else None, None if codes else yr, None if codes else gr, weight, scale,
-                                  next_weight, y_inv, out_inv, *(y_codes or (None, None)), *(gate_codes or (None, None)))
-            ctx.shape, ctx.rows, ctx.width, ctx.dtype, ctx.device = x.shape, rows, width, x.dtype, dev
-            ctx.has_block, ctx.activation, ctx.eps = y is not None, activation, eps
+        width = x.shape[-1]
+        inv_rms = torch.empty(2, x.numel() // width if width else 0, dtype=torch.float32, device=x.device) if needed else None
+        codes = None
+        if needed and checkpoint:
+            codes = _code_buffers(x) + (_code_buffers(x) if gate is not None else ())
+        out, nxt = _run_block_norm(x, y, weight, gate, scale, next_weight, activation, eps, inv_rms, codes)
+        if needed:
+            keep_x = next_weight is not None and (y is not None or codes is None)
+            ctx.save_for_backward(x if keep_x else None, *((y, gate) if codes is None else (None, None)), weight, scale,
+                                  next_weight, inv_rms, *(codes or ()))
+            ctx.activation, ctx.eps = activation, eps
         return out, nxt
 
     @staticmethod
@@ -183,34 +172,32 @@ class _BlockNorm(torch.autograd.Function):
     def backward(ctx, d_out, d_next):
         if d_out is None and d_next is None:
             return (None,) * 9
-        x, y, gate, weight, scale, next_weight, y_inv, out_inv, y8, y8s, g8, g8s = ctx.saved_tensors
+        x, y, gate, weight, scale, next_weight, inv_rms, *codes = ctx.saved_tensors
         want_x, want_y, want_weight, want_gate, want_scale, want_next = ctx.needs_input_grad[:6]
-        rows, width = ctx.rows, ctx.width
-        do, dn = _row_grad(d_out, rows, width), _row_grad(d_next, rows, width)
+        do, dn = _row_grad(d_out), _row_grad(d_next)
+        like = dn if do is None else do
+        # without a norm behind, the gradient of x is that of out
+        passed = dn is None
+        d_x = torch.empty_like(like) if want_x and not passed else None
+        d_y = torch.empty_like(like) if want_y else None
+        d_gate = torch.empty_like(like) if want_gate else None
+        wanted = want_weight + want_scale + want_next
+        sums = iter(torch.empty(wanted, like.shape[-1], dtype=torch.float32, device=like.device).unbind(0) if wanted else ())
+        d_weight = next(sums) if want_weight else None
+        d_scale = next(sums) if want_scale else None
+        d_next_weight = next(sums) if want_next else None
+        ops.block_norm_backward(like, x=x, y=y, weight=weight, gate=gate, scale=scale, next_weight=next_weight, inv_rms=inv_rms,
+                                codes=codes or None, activation=ctx.activation, eps=ctx.eps, d_out=do, d_next=dn, d_x=d_x,
+                                d_y=d_y, d_gate=d_gate, d_weight=d_weight, d_scale=d_scale, d_next_weight=d_next_weight)
+        return d_out if want_x and passed else d_x, d_y, d_weight, d_gate, d_scale, d_next_weight, None, None, None
 
-        def rows_like():
-            return torch.empty(rows, width, dtype=ctx.dtype, device=ctx.device)
 
-        def sums_like(wanted):
-            return torch.empty(width, dtype=torch.float32, device=ctx.device) if wanted else None
-
-        # behind a block and without a norm the gradient of x is that of out
-        passed = next_weight is None or dn is None
-        d_x = rows_like() if want_x and not passed else None
-        d_y = rows_like() if want_y else None
-        d_gate = rows_like() if want_gate else None
-        d_weight, d_scale, d_next_weight = sums_like(want_weight), sums_like(want_scale), sums_like(want_next)
-        ops.block_norm_backward(do if do is not None else dn, x=x, y=y, weight=weight, gate=gate, scale=scale,
-                                next_weight=next_weight, y_inv_rms=y_inv, out_inv_rms=out_inv,
-                                y_codes=None if y8 is None else (y8, y8s), gate_codes=None if g8 is None else (g8, g8s),
-                                activation=ctx.activation, eps=ctx.eps, d_out=do, d_next=dn, d_x=d_x, d_y=d_y, d_gate=d_gate,
-                                d_weight=d_weight, d_scale=d_scale, d_next_weight=d_next_weight)
-
-        def shaped(t):
-            return None if t is None else t.view(ctx.shape)
-
-        return (d_out if want_x and passed else shaped(d_x), shaped(d_y), d_weight, shaped(d_gate), d_scale, d_next_weight,
-                None, None, None)
+def _block_norm(x, y, weight, gate, scale, next_weight, activation, eps, checkpoint):
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise ValueError("x must be a tensor of at least one dimension")
+    if _differentiated(x, y, weight, gate, scale, next_weight):
+        return _BlockNorm.apply(x, y, weight, gate, scale, next_weight, activation, eps, checkpoint)
+    return _run_block_norm(x, y, weight, gate, scale, next_weight, activation, eps)
 
 
 def rms_norm(x, weight, eps=1e-5, checkpoint=False):
@@ -218,7 +205,7 @@ def rms_norm(x, weight, eps=1e-5, checkpoint=False):
 
     x [..., D] float32 / float16 / bfloat16, weight [D] float32.  checkpoint=True: the backward pass sees x through its
     8-bit codes (`pack8`), and x itself need not be kept for it."""
-    return _BlockNorm.apply(x, None, None, None, None, weight, "none", eps, checkpoint)[1]
+    return _block_norm(x, None, None, None, None, weight, "none", eps, checkpoint)[1]
 
 
 def residual_norm(x, y, weight, gate=None, scale=None, next_weight=None, activation="silu", eps=1e-5, checkpoint=False):
@@ -228,7 +215,7 @@ def residual_norm(x, y, weight, gate=None, scale=None, next_weight=None, activat
     x, y, gate [..., D] of one shape and type; weight, scale, next_weight [D] float32; activation of the gate: "silu",
     "sigmoid" or "none".  Differentiable in all of them.  checkpoint=True: y and gate are kept for the backward pass as
     8-bit codes (`pack8`) and their gradients are those at the values the codes stand for; x is kept as it is."""
-    out, nxt = _BlockNorm.apply(x, y, weight, gate, scale, next_weight, activation, eps, checkpoint)
+    out, nxt = _block_norm(x, y, weight, gate, scale, next_weight, activation, eps, checkpoint)
     return out if next_weight is None else (out, nxt)
 
 
@@ -238,15 +225,14 @@ def pack8(x):
     """(codes int8 [..., D], scales float32 [..., ceil(D / 64)]) of x [..., D]: groups of 64 elements along the last
     dimension share scale = max|x| / 127, a code is the nearest integer of x * (127 / max|x|).  A group that holds an inf
     or NaN decodes to NaN, one whose largest magnitude is below 2^-120 to zeros.  Not differentiable."""
-    xr = _rows(x.detach(), "x")
-    codes, scales = _code_buffers(xr)
-    ops.pack8(xr, codes, scales)
-    return codes.view(x.shape), scales.view(x.shape[:-1] + scales.shape[1:])
+    x = x.detach()
+    codes, scales = _code_buffers(x)
+    ops.pack8(x, codes, scales)
+    return codes, scales
 
 
 def unpack8(codes, scales, dtype=torch.float32):
     """The values that pack8's codes and scales stand for."""
     out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
-    q = _rows(codes, "codes")
-    ops.unpack8(q, _rows(scales, "scales"), _rows(out, "out"))
+    ops.unpack8(codes, scales, out)
     return out

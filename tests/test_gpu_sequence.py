@@ -482,6 +482,40 @@ def test_checkpoint_frees_what_it_replaces():
     assert plain >= 3 * size and packed <= 2.2 * size
 
 
+def test_layouts_that_are_refused():
+    x = torch.zeros(3, 4, 5, 6, device=DEV)
+    w = torch.ones(6, device=DEV)
+    with pytest.raises(ValueError, match="evenly spaced"):
+        sequence.rms_norm(x[:, ::2], w)
+    with pytest.raises(ValueError, match="adjacent"):
+        sequence.rms_norm(torch.zeros(6, 5, device=DEV).t(), w)
+    with pytest.raises(ValueError, match="evenly spaced"):
+        sequence.rms_norm(x.transpose(2, 3), torch.ones(5, device=DEV))
+    with pytest.raises(ValueError, match="expected shape"):
+        sequence.residual_norm(x, x[0], w)
+    with pytest.raises(TypeError, match="expected dtype"):
+        sequence.residual_norm(x, x.half(), w)
+    with pytest.raises(TypeError, match="expected dtype"):
+        sequence.rms_norm(x, w.half())
+    with pytest.raises(ValueError, match="device tensors only"):
+        sequence.rms_norm(x, w.cpu())
+    with pytest.raises(ValueError, match="contiguous"):
+        sequence.rms_norm(x, torch.ones(12, device=DEV)[::2])
+    r = torch.zeros(3, 4, 6, device=DEV)
+    with pytest.raises(ValueError, match="adjacent"):
+        sequence.linear_recurrence(r, torch.zeros(3, 6, 4, device=DEV).transpose(1, 2))
+    with pytest.raises(TypeError, match="expected dtype"):
+        sequence.linear_recurrence(r, r, reset=torch.zeros(3, 4, device=DEV))
+    with pytest.raises(ValueError, match="expected shape"):
+        sequence.linear_recurrence(r, r, state=torch.zeros(4, 5, device=DEV))
+    with pytest.raises(ValueError, match="overlap"):
+        ops.linear_recurrence(r, r, r)
+    with pytest.raises(ValueError, match="share one address"):
+        ops.linear_recurrence(r, r, torch.zeros(4, 6, device=DEV).expand(3, 4, 6))
+    with pytest.raises(Exception, match="8192"):
+        sequence.rms_norm(torch.zeros(2, 8193, device=DEV), torch.ones(8193, device=DEV))
+
+
 # ---- streams, graphs, repeatability ---------------------------------------------------------------------------------
 
 def block(x, p, state, reset):

@@ -141,8 +141,6 @@ def test_host_tensors_wrong_types_and_shapes_are_refused():
         sequence.linear_recurrence_step(x, x, x)
     with pytest.raises(ValueError, match="activation"):
         sequence.residual_norm(x, x, torch.ones(4), activation="tanh")
-    with pytest.raises(ValueError, match="evenly spaced"):
-        sequence.rms_norm(torch.zeros(3, 4, 5, 6)[:, ::2], torch.ones(6))
     with pytest.raises(RuntimeError):
         sequence.linear_recurrence(torch.zeros(3, 3, 4), x)  # does not broadcast
 
@@ -155,6 +153,7 @@ def test_capture_guard_counts_live_eager_nodes(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
     a = torch.zeros(3, 2, 4, requires_grad=True)
     b = torch.zeros(3, 2, 4)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
     first = sequence.linear_recurrence(a, b)
     second = sequence.linear_recurrence(a * 1.0, b)  # not a leaf of the operator
     capturing[0] = True
