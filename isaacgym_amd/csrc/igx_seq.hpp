@@ -19,9 +19,12 @@ template <typename T> struct Pack<T, 1> { typedef T type; };
 
 template <typename T, int V> struct Raw { typename Pack<T, V>::type v; };
 
-template <typename T, int V> __device__ __forceinline__ Raw<T, V> load_raw(const void *p)
+// STREAM: past the caches' replacement, for what is not read again soon
+template <typename T, int V, bool STREAM = false> __device__ __forceinline__ Raw<T, V> load_raw(const void *p)
 {
-    return {*reinterpret_cast<const typename Pack<T, V>::type *>(p)};
+    const typename Pack<T, V>::type *q = reinterpret_cast<const typename Pack<T, V>::type *>(p);
+    if constexpr (STREAM && V > 1) return {__builtin_nontemporal_load(q)};
+    else return {*q};
 }
 
 template <typename T, int V> __device__ __forceinline__ float raw_at(const Raw<T, V> &r, int i)
@@ -37,7 +40,7 @@ template <typename T, int V> __device__ __forceinline__ void widen(const Raw<T, 
 }
 
 // one rounding to nearest even, the hardware's conversion
-template <typename T, int V> __device__ __forceinline__ void store_vec(void *p, const float (&f)[V])
+template <typename T, int V, bool STREAM = false> __device__ __forceinline__ void store_vec(void *p, const float (&f)[V])
 {
     if constexpr (V == 1) {
         *reinterpret_cast<T *>(p) = (T)f[0];
@@ -45,7 +48,8 @@ template <typename T, int V> __device__ __forceinline__ void store_vec(void *p, 
         typename Pack<T, V>::type v;
 #pragma unroll
         for (int i = 0; i < V; i++) v[i] = (T)f[i];
-        *reinterpret_cast<typename Pack<T, V>::type *>(p) = v;
+        if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<typename Pack<T, V>::type *>(p));
+        else *reinterpret_cast<typename Pack<T, V>::type *>(p) = v;
     }
 }
 

@@ -1,17 +1,21 @@
 // Gated linear recurrence h[t] = gate[t] h[t-1] + inp[t] over rollouts [T, N, D], and its gradients.
 //
-// Channels are independent and adjacent in memory, so a lane owns one 16-byte vector of channels and walks the steps
-// with the carried value in fp32 registers; the loads of kUnroll steps are in flight together, since they do not depend
-// on it.  A call moves 3 elements per (t, n, d) forward and 5 backward and does 2 - 3 operations on each: HBM bounds it
-// where there are enough channels to fill the card.
+// Channels are independent and adjacent in memory, so a lane owns a vector of channels (16 bytes) and walks the steps with
+// the carried value in fp32 registers.  A call moves 3 elements per (t, n, d) forward and 5 backward and does 2 - 3
+// operations on each: HBM bounds it where there are enough channels to fill the card (32 x 65 536 x 64 bf16 forward and
+// backward: 2.15 GB in 406 us, 5.3 TB/s; one step of 262 144 x 64 with its fp32 state: 235 MB in 38 us, 6.2 TB/s).  Arrays
+// that nothing reads again soon go past the caches' replacement (non-temporal; loads too where a lane walks alone: 406 us
+// against 444).
 //
 // With fewer channels the time is split, for the recurrence is a composition of maps h -> A h + B that is associative:
-//   - within a workgroup SEG groups of lanes take kUnroll consecutive steps each of the same channels, reduce them to
+//   - within a workgroup SEG groups of lanes take a few consecutive steps each of the same channels, reduce them to
 //     (A, B) in registers, exchange those through LDS, and then walk their steps from the value that reaches them, so
 //     every element is still read and written once;
 //   - across workgroups a first kernel reduces every span of the time to its (A, B) in a workspace, and each workgroup of
-//     the second composes the spans before its own.  That reads gate and inp twice (the second time mostly from the
-//     caches), so it is done only where the channels alone leave CUs without work.
+//     the second composes the spans before its own, while its first steps are on their way.  That reads gate and inp twice
+//     (the second time mostly from the caches), so it is done only where the channels alone leave CUs without work: 8 192
+//     steps of 512 channels in bf16 take 23 us forward and 23 us backward, bound by the latency of two launches and the
+//     exchange (a lane for every 8 channels needs 7 565 us).
 #include "igx_seq.hpp"
 
 namespace igx {
@@ -63,10 +67,10 @@ template <int V> __device__ __forceinline__ Lane lane_of(const RecArgs &a, uint3
     return l;
 }
 
-template <typename T, int V> __device__ __forceinline__ void store_from(char *p, const float (&f)[V], int skip)
+template <typename T, int V, bool STREAM = false> __device__ __forceinline__ void store_from(char *p, const float (&f)[V], int skip)
 {
     if (V == 1 || skip == 0) {
-        store_vec<T, V>(p, f);
+        store_vec<T, V, STREAM>(p, f);
     } else {
 #pragma unroll
         for (int i = 0; i < V; i++)
@@ -93,9 +97,11 @@ template <int V, int FL> struct LaneFlags {
     }
 };
 
-// steps whose loads a lane has in flight; a flag for every channel takes as many registers as the channels do
-constexpr int kUnroll = 8;
-template <int V, int FL> constexpr int unroll_of() { return FL == kFlagEach && V == 8 ? kUnroll / 2 : kUnroll; }
+// Steps whose loads a lane has in flight, by the groups that share a workgroup's channels (measured, forward + backward):
+// with a lane for all steps 1, since thousands of waves are in flight and fewer rows [N, D] open at a time suit HBM better
+// (32 x 65 536 x 64 bf16: 406 us with 1, 415 with 2, 431 with 4, 475 with 8); with four groups 2 (32 x 4 096 x 64 fp32:
+// 49 us, 51 with 4, 55 with 8); with sixteen, where waves are few, 8 (2 048 x 16 x 1 024 bf16: 172 us, 237 with 4).
+constexpr int steps_of(int seg) { return seg == 1 ? 1 : seg == 4 ? 2 : 8; }
 
 template <int V, int FL> struct StepFlags {
     using Places = LaneFlags<V, FL>;
@@ -117,10 +123,10 @@ template <int V, int FL> struct StepFlags {
     }
 };
 
-template <typename T, int V> __device__ __forceinline__ void load_gate(Raw<T, V> &g, const char *p, int splat)
+template <typename T, int V, bool STREAM> __device__ __forceinline__ void load_gate(Raw<T, V> &g, const char *p, int splat)
 {
     if (V == 1 || !splat) {
-        g = load_raw<T, V>(p);
+        g = load_raw<T, V, STREAM>(p);
     } else if constexpr (V > 1) {
         const T one = *reinterpret_cast<const T *>(p);
 #pragma unroll
@@ -137,7 +143,7 @@ __device__ __forceinline__ float through(float A, float B, float h) { return h =
 
 // K consecutive steps of a lane's channels in registers.  `count` of them exist, the others repeat the last one and are
 // neutral; whole steps of a full group cost no test (CHECK false).
-template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK> struct Steps {
+template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STREAM> struct Steps {
     Raw<T, V> g[K], x[K], hb[K];
     StepFlags<V, FL> f[K];
     int count;
@@ -150,14 +156,14 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK> struct St
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const int64_t t = CHECK && t0 + k > most ? most : t0 + k;
-            load_gate<T, V>(g[k], gate + t * a.gate_t, a.splat);
+            load_gate<T, V, STREAM>(g[k], gate + t * a.gate_t, a.splat);
             f[k].load(lf, t * a.reset_t);
         }
         if (!BACKWARD || add) {
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 const int64_t t = CHECK && t0 + k > most ? most : t0 + k;
-                x[k] = load_raw<T, V>(add + t * a.add_t);
+                x[k] = load_raw<T, V, STREAM>(add + t * a.add_t);
             }
         } else {
 #pragma unroll
@@ -167,7 +173,7 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK> struct St
 #pragma unroll
             for (int k = 0; k < K; k++) {  // before the first step stands `state`, which is not in out
                 const int64_t t = CHECK && t0 + k > most ? most : t0 + k;
-                if (t < a.T - 1) hb[k] = load_raw<T, V>(before + t * a.before_t);
+                if (t < a.T - 1) hb[k] = load_raw<T, V, STREAM>(before + t * a.before_t);
             }
         }
     }
@@ -204,7 +210,7 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK> struct St
                     const float x1 = raw_at(x[k], i);
                     h[i] = f[k].begins(i) ? x1 : fmaf(raw_at(g[k], i), h[i], x1);
                 }
-                if (store) store_from<T, V>(to + t * a.to_t, h, l.skip);
+                if (store) store_from<T, V, true>(to + t * a.to_t, h, l.skip);
             } else {
                 float d[V], dg[V];
 #pragma unroll
@@ -221,9 +227,9 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK> struct St
 #pragma unroll
                         for (int i = 0; i < V; i++) dg[i] = f[k].begins(i) ? 0.0f : d[i] * a.state[l.channel + i];
                     }
-                    if (store) store_from<T, V>(d_gate + t * a.d_gate_t, dg, l.skip);
+                    if (store) store_from<T, V, true>(d_gate + t * a.d_gate_t, dg, l.skip);
                 }
-                if (to && store) store_from<T, V>(to + t * a.to_t, d, l.skip);
+                if (to && store) store_from<T, V, true>(to + t * a.to_t, d, l.skip);
             }
         }
     }
@@ -257,12 +263,20 @@ template <typename T> struct Places {
     }
 };
 
+// the carried values of a lane's channels, [N, D] fp32
+template <int V> __device__ __forceinline__ void load_start(const float *p, const Lane &l, float (&h)[V])
+{
+    if (p) {
+        widen(load_raw<float, V>(p + l.channel), h);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) h[i] = 0.0f;
+    }
+}
+
 template <int V> __device__ __forceinline__ void store_end(const RecArgs &a, const Lane &l, const float (&h)[V])
 {
-    if (!a.end) return;
-#pragma unroll
-    for (int i = 0; i < V; i++)
-        if (i >= l.skip) a.end[l.channel + i] = h[i];
+    if (a.end) store_from<float, V>(reinterpret_cast<char *>(a.end + l.channel), h, l.skip);
 }
 
 // enough channels: a lane walks all the steps
@@ -275,21 +289,12 @@ __global__ __launch_bounds__(kBlock) void recurrence_kernel(RecArgs a)
     const LaneFlags<V, FL> lf(a, l);
     const Places<T> p(a, l);
     float h[V];
-#pragma unroll
-    for (int i = 0; i < V; i++) h[i] = a.start ? a.start[l.channel + i] : 0.0f;
-    int64_t t = 0;
-    auto group = [&](auto count) {
-        constexpr int K = decltype(count)::value;
-        Steps<T, V, FL, K, BACKWARD, false> s;
-        s.load(a, lf, p.gate, p.add, p.before, t, t + K);
+    load_start<V>(a.start, l, h);
+    for (int64_t t = 0; t < a.T; t++) {
+        Steps<T, V, FL, steps_of(1), BACKWARD, false, true> s;
+        s.load(a, lf, p.gate, p.add, p.before, t, t + 1);
         s.walk(a, l, true, p.to, p.d_gate, t, h);
-        t += K;
-    };
-    constexpr int kSteps = unroll_of<V, FL>();
-    while (t + kSteps <= a.T) group(std::integral_constant<int, kSteps>());
-    if (kSteps > 4 && a.T - t >= 4) group(std::integral_constant<int, 4>());
-    if (a.T - t >= 2) group(std::integral_constant<int, 2>());
-    if (a.T - t >= 1) group(std::integral_constant<int, 1>());
+    }
     store_end<V>(a, l, h);
 }
 
@@ -341,7 +346,7 @@ template <int V> __device__ __forceinline__ void load_span(const RecArgs &a, int
     else widen(load_raw<float, V>(p), f);
 }
 
-// Time split: SEG groups of 256 / SEG lanes take kUnroll steps each of the same channels; blockIdx.y is the span.
+// Time split: SEG groups of 256 / SEG lanes take steps_of(SEG) steps each of the same channels; blockIdx.y is the span.
 template <typename T, int V, int FL, bool BACKWARD, int SEG>
 __global__ __launch_bounds__(kBlock) void recurrence_split_kernel(RecArgs a)
 {
@@ -354,10 +359,12 @@ __global__ __launch_bounds__(kBlock) void recurrence_split_kernel(RecArgs a)
     const LaneFlags<V, FL> lf(a, l);
     const Places<T> p(a, l);
     const int64_t first = (int64_t)blockIdx.y * a.span, t1 = first + a.span < a.T ? first + a.span : a.T;
+    constexpr int kSteps = steps_of(SEG);
+    Steps<T, V, FL, kSteps, BACKWARD, true, false> s;
+    s.load(a, lf, p.gate, p.add, p.before, first + seg * kSteps, t1);  // on its way while the spans are composed
     float h[V];
     if (gridDim.y == 1) {
-#pragma unroll
-        for (int i = 0; i < V; i++) h[i] = a.start ? a.start[l.channel + i] : 0.0f;
+        load_start<V>(a.start, l, h);
     } else {  // each group composes its part of the spans before this one, then all go through the parts
         const int64_t spans = blockIdx.y, part = ceil_div(spans, SEG);
         float A[V], B[V];
@@ -365,10 +372,10 @@ __global__ __launch_bounds__(kBlock) void recurrence_split_kernel(RecArgs a)
         for (int i = 0; i < V; i++) A[i] = 1.0f, B[i] = 0.0f;
         const int64_t end = (seg + 1) * part < spans ? (seg + 1) * part : spans;
 #pragma unroll 2
-        for (int64_t s = seg * part; s < end; s++) {
+        for (int64_t q = seg * part; q < end; q++) {
             float A2[V], B2[V];
-            load_span<V>(a, 1 + 2 * s, v, A2);
-            load_span<V>(a, 2 + 2 * s, v, B2);
+            load_span<V>(a, 1 + 2 * q, v, A2);
+            load_span<V>(a, 2 + 2 * q, v, B2);
             compose<V>(A, B, A2, B2);
         }
         maps[1][seg][0].put(lane, A);
@@ -376,20 +383,17 @@ __global__ __launch_bounds__(kBlock) void recurrence_split_kernel(RecArgs a)
         load_span<V>(a, 0, v, h);
         __syncthreads();
 #pragma unroll 2
-        for (int s = 0; s < SEG; s++) {
+        for (int q = 0; q < SEG; q++) {
             float A2[V], B2[V];
-            maps[1][s][0].get(lane, A2);
-            maps[1][s][1].get(lane, B2);
+            maps[1][q][0].get(lane, A2);
+            maps[1][q][1].get(lane, B2);
 #pragma unroll
             for (int i = 0; i < V; i++) h[i] = through(A2[i], B2[i], h[i]);
         }
     }
     int turn = 0;
-    constexpr int kSteps = unroll_of<V, FL>();
     for (int64_t t0 = first; t0 < t1; t0 += SEG * kSteps, turn ^= 1) {
-        const int64_t ts = t0 + seg * kSteps;
-        Steps<T, V, FL, kSteps, BACKWARD, true> s;
-        s.load(a, lf, p.gate, p.add, p.before, ts, t1);
+        const int64_t ts = t0 + seg * kSteps, next = t0 + SEG * kSteps;
         float A[V], B[V], from[V] = {};
         bool starts[V];
         identity<V>(A, B, starts);
@@ -410,6 +414,7 @@ __global__ __launch_bounds__(kBlock) void recurrence_split_kernel(RecArgs a)
             }
         }
         s.walk(a, l, store, p.to, p.d_gate, ts, from);
+        if (next < t1) s.load(a, lf, p.gate, p.add, p.before, next + seg * kSteps, t1);
     }
     if (store && seg == 0 && blockIdx.y == gridDim.y - 1) store_end<V>(a, l, h);
 }
@@ -431,9 +436,9 @@ __global__ __launch_bounds__(kBlock) void recurrence_spans_kernel(RecArgs a)
     float A[V], B[V];
     bool starts[V];
     identity<V>(A, B, starts);
-    constexpr int kSteps = unroll_of<V, FL>();
+    constexpr int kSteps = steps_of(16);
     for (int64_t t = from; t < to; t += kSteps) {
-        Steps<T, V, FL, kSteps, BACKWARD, true> s;
+        Steps<T, V, FL, kSteps, BACKWARD, true, false> s;
         s.load(a, lf, p.gate, p.add, nullptr, t, to);
         s.reduce(A, B, starts);
     }
@@ -454,8 +459,7 @@ __global__ __launch_bounds__(kBlock) void recurrence_spans_kernel(RecArgs a)
     store_vec<float, V>(to_span + (1 + 2 * (int64_t)blockIdx.y) * at, A);
     store_vec<float, V>(to_span + (2 + 2 * (int64_t)blockIdx.y) * at, B);
     if (blockIdx.y == 0) {  // the second kernel takes the start from here: `end` may be the array it comes from
-#pragma unroll
-        for (int i = 0; i < V; i++) A[i] = a.start ? a.start[l.channel + i] : 0.0f;
+        load_start<V>(a.start, l, A);
         store_vec<float, V>(to_span, A);
     }
 }
@@ -469,7 +473,7 @@ __global__ void carry_through_kernel(const float *from, float *to, int64_t n)
 
 struct Plan {
     RecArgs a;
-    int vec;    // channels per lane: the type's 16 bytes, or 1 where a run is shorter than that
+    int vec;    // channels per lane: the type's 16 bytes, or 4, or 1 where a run is shorter than that
     int flags;
     int seg;    // groups of lanes that share a workgroup's channels; 1: a lane walks all steps
     int64_t spans;
@@ -494,17 +498,19 @@ int check(const igx_recurrence *r, const char *who)
 // are environments n and n + 1 adjacent in this array?
 bool follows(const igx_recurrence *r, int64_t stride_n) { return r->envs == 1 || stride_n == r->width; }
 
-// How the time is split.  Lanes for the whole card (256 workgroups and more) walk the steps alone; down to 64 lanes a
-// workgroup its four groups share short rollouts; below, sixteen groups share the steps, and as long as that leaves CUs
-// without a workgroup the spans of a long sequence go to workgroups of their own.
+// How the time is split (both sides measured, forward + backward).  131 072 lanes and more walk the steps alone (64 x 16 384 x
+// 64 fp32: 364 us, 452 in four groups).  With fewer, four groups share a workgroup's steps (32 x 4 096 x 64 fp32, 65 536
+// lanes: 49 us, 82 alone), below 16 384 lanes sixteen.  A sequence goes to several workgroups in spans only where the
+// channels fill fewer than 256 of them, one for each CU (1 024 x 64 x 256 fp32 fills 256: 118 us in one span, 153 in two,
+// for gate and inp are then read twice); 512 workgroups in all are enough.
 void split(Plan &p)
 {
     const int64_t vectors = p.a.vectors, T = p.a.T;
     p.spans = 1;
     p.a.span = T;
-    p.seg = T <= kUnroll || vectors >= 131072 ? 1 : vectors >= 16384 ? 4 : 16;
+    p.seg = T <= steps_of(16) || vectors >= 131072 ? 1 : vectors >= 16384 ? 4 : 16;
     if (p.seg != 16) return;
-    const int64_t strips = ceil_div(vectors, kBlock / 16), tile = 16 * kUnroll;
+    const int64_t strips = ceil_div(vectors, kBlock / 16), tile = 16 * steps_of(16);
     if (strips >= 256 || T <= tile) return;
     const int64_t want = ceil_div(512, strips), most = ceil_div(T, tile);
     const int64_t spans = want < most ? want : most;
@@ -532,12 +538,18 @@ void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, Plan &p)
     a.D = (uint32_t)D;
     a.run = (uint32_t)(flat ? N * D : D);
     a.splat = one_gate || shared;
-    const int vec = r->dtype == IGX_F32 ? 4 : 8;
-    p.vec = a.run >= (uint32_t)vec ? vec : 1;
-    a.per_run = (uint32_t)ceil_div(a.run, p.vec);
-    a.vectors = (uint32_t)(flat ? 1 : N) * a.per_run;
+    auto lanes = [&](int vec) {
+        p.vec = a.run >= (uint32_t)vec ? vec : 1;
+        a.per_run = (uint32_t)ceil_div(a.run, p.vec);
+        a.vectors = (uint32_t)(flat ? 1 : N) * a.per_run;
+        split(p);
+    };
+    lanes(r->dtype == IGX_F32 ? 4 : 8);
+    if (r->dtype != IGX_F32 && p.seg > 1) {  // too few lanes: twice as many with half the bytes (8 192 x 1 x 512 bf16: 64 -> 43 us)
+        lanes(4);
+        if (p.seg == 1) p.seg = 4;
+    }
     p.flags = !r->reset ? kNoFlags : (p.vec == 1 || !flat || D % p.vec == 0 || N == 1) ? kOneFlag : D >= p.vec ? kTwoFlags : kFlagEach;
-    split(p);
 
     // forward order: as stored, or turned round for reverse; the backward pass goes the other way through the same order
     const bool down = (r->reverse != 0) != (g != nullptr);
@@ -588,7 +600,12 @@ template <int DT, bool BACKWARD> void launch_type(const Plan &p, hipStream_t s)
 {
     using T = typename Elem<DT>::type;
     constexpr int V = Elem<DT>::vec;
-    if (p.vec == 1) {
+    if (p.vec == 4 && V != 4) {
+        if (p.flags == kNoFlags) launch_as<T, 4, kNoFlags, BACKWARD>(p, s);
+        else if (p.flags == kOneFlag) launch_as<T, 4, kOneFlag, BACKWARD>(p, s);
+        else if (p.flags == kTwoFlags) launch_as<T, 4, kTwoFlags, BACKWARD>(p, s);
+        else launch_as<T, 4, kFlagEach, BACKWARD>(p, s);
+    } else if (p.vec == 1) {
         if (p.flags == kNoFlags) launch_as<T, 1, kNoFlags, BACKWARD>(p, s);
         else launch_as<T, 1, kOneFlag, BACKWARD>(p, s);
     } else {

@@ -80,6 +80,24 @@ def test_recurrence_shapes(shape, dtype):
     check_recurrence(*rollout(T, N, D, dtype, 1, resets=min(0.3, 4.0 / T)))
 
 
+MANY = [(13, 1100, 64), (11, 700, 105), (12, 25000, 3), (11, 5000, 105), (10, 9001, 64), (9, 180000, 3)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", MANY)
+def test_recurrence_many_channels(shape, dtype):
+    """Enough channels that a few groups of lanes share the steps, or that every lane walks alone."""
+    T, N, D = shape
+    check_recurrence(*rollout(T, N, D, dtype, 13, resets=0.1))
+
+
+@pytest.mark.parametrize("layout", ["env", "slice"])
+def test_recurrence_many_short_rows(layout):
+    """Environments that do not follow each other, narrower than a lane's vector or not divided by it."""
+    for T, N, D in ((11, 20000, 3), (10, 4000, 21)):
+        check_recurrence(*rollout(T, N, D, F32, 14, resets=0.1), layout=layout, grad_layout="time")
+
+
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("layout", ["time", "env", "slice", "steps"])
 @pytest.mark.parametrize("dtype", [F32, BF16])
