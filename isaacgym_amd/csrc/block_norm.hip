@@ -6,128 +6,11 @@
 // waves of a whole workgroup, whichever the width fills - so every array is read and written once and the statistics
 // need no second pass.  Groups of lanes walk over the rows, which keeps the parameter vectors in registers and lets
 // backward add up the column sums there: one partial row per workgroup, joined in a fixed order by a second kernel.
-#include "igx_seq.hpp"
+// STREAM variants go past the caches' replacement, for calls that move more than the last-level cache holds.
+#include "igx_block_norm.hpp"
 
 namespace igx {
 namespace {
-
-constexpr int kBlock = 256;   // of the kernels whose row fits one wave
-constexpr int kColumns = 8;   // of a lane
-
-struct NormArgs {
-    const char *x, *y, *gate, *d_out, *d_next;
-    const char *x_end, *y_end, *gate_end, *d_out_end, *d_next_end;  // behind each array's last element
-    int64_t x_row, y_row, gate_row, d_out_row, d_next_row;          // bytes from row to row
-    char *out, *next, *d_x, *d_y, *d_gate;
-    const float *weight, *scale, *next_weight;
-    float *y_inv, *out_inv;
-    int8_t *y8, *gate8;
-    float *y8_scale, *gate8_scale;
-    float *partial;  // [sums][workgroups][width]
-    int64_t rows;
-    int width, groups, act;
-    float eps;
-    bool sum_weight, sum_scale, sum_next;
-};
-
-__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
-
-__device__ __forceinline__ float activate(float z, int act)
-{
-    if (act == IGX_GATE_NONE) return z;
-    const float p = sigmoid(z);
-    return act == IGX_GATE_SIGMOID ? p : z * p;
-}
-
-__device__ __forceinline__ void activate_slope(float z, int act, float &f, float &slope)
-{
-    if (act == IGX_GATE_NONE) {
-        f = z;
-        slope = 1.0f;
-        return;
-    }
-    const float p = sigmoid(z), q = p * (1.0f - p);
-    f = act == IGX_GATE_SIGMOID ? p : z * p;
-    slope = act == IGX_GATE_SIGMOID ? q : fmaf(z, q, p);
-}
-
-// The lanes that share a row.  LANES 8 ... 64: that many lanes of a wave, kWorkgroup: the whole workgroup of up to 512,
-// kLargest: one of 1024, which leaves a lane half as many registers.
-constexpr int kWorkgroup = 0, kLargest = -1;
-constexpr int block_of(int lanes) { return lanes > 0 ? kBlock : lanes == kWorkgroup ? 512 : 1024; }
-
-template <typename T, int LANES> struct RowLanes {
-    static constexpr int V = Elem<std::is_same<T, float>::value ? IGX_F32 : std::is_same<T, _Float16>::value ? IGX_F16 : IGX_BF16>::vec;
-    static constexpr int K = kColumns / V;
-    static constexpr bool kWide = LANES <= 0;
-    int lane, lanes, rows_per_block, sub;
-    __device__ __forceinline__ RowLanes()
-    {
-        lanes = kWide ? blockDim.x : LANES;
-        lane = kWide ? threadIdx.x : threadIdx.x % (kWide ? 1 : LANES);
-        sub = kWide ? 0 : threadIdx.x / (kWide ? 1 : LANES);
-        rows_per_block = kWide ? 1 : kBlock / (kWide ? 1 : LANES);
-    }
-    __device__ __forceinline__ int col(int k) const { return (k * lanes + lane) * V; }
-
-    // sum over the row's lanes, the same value in all of them; `slots`: LDS for the wide form, two halves used in turn so
-    // that one barrier a sum is enough
-    __device__ __forceinline__ float sum(float v, float *slots, int &turn) const
-    {
-#pragma unroll
-        for (int m = 1; m < (kWide ? 64 : LANES); m *= 2) v += __shfl_xor(v, m);
-        if constexpr (kWide) {
-            float *s = slots + 16 * turn;
-            turn ^= 1;
-            if (threadIdx.x % 64 == 0) s[threadIdx.x / 64] = v;
-            __syncthreads();
-            v = 0.0f;
-            for (int w = 0; w < (int)(blockDim.x / 64); w++) v += s[w];
-        }
-        return v;
-    }
-};
-
-// A lane's vector of a row: `left` of its V columns exist.  Reading on into the next row is fine, past the array is not.
-template <typename T, int V> __device__ __forceinline__ Raw<T, V> load_row(const char *p, const char *end, int left)
-{
-    Raw<T, V> r = {};
-    if (left <= 0) return r;
-    if (p + V * sizeof(T) <= end) {
-        r = load_raw<T, V>(p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i++)
-            if (i < left) r.v[i] = reinterpret_cast<const T *>(p)[i];
-    }
-    return r;
-}
-
-template <typename T, int V> __device__ __forceinline__ void widen_row(const Raw<T, V> &r, int left, float (&f)[V])
-{
-    widen(r, f);
-    if (left < V) {
-#pragma unroll
-        for (int i = 0; i < V; i++) f[i] = i < left ? f[i] : 0.0f;
-    }
-}
-
-template <typename T, int V> __device__ __forceinline__ void store_row(char *p, const float (&f)[V], int left)
-{
-    if (left >= V) {
-        store_vec<T, V>(p, f);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i++)
-            if (i < left) reinterpret_cast<T *>(p)[i] = (T)f[i];
-    }
-}
-
-template <int V> __device__ __forceinline__ void load_param(const float *p, int col, int left, float absent, float (&f)[V])
-{
-#pragma unroll
-    for (int i = 0; i < V; i++) f[i] = i < left ? (p ? p[col + i] : absent) : 0.0f;
-}
 
 // the row's 8-bit codes: a group's lanes sit next to each other (with 8 lanes of 4 columns, in both of their vectors)
 template <int V, int K, int LANES>
@@ -167,7 +50,7 @@ __device__ __forceinline__ void checkpoint_row(const float (&f)[K][V], const int
 }
 
 // POST: there is a block output y; NEXT: there is a norm behind
-template <typename T, int LANES, bool POST, bool NEXT>
+template <typename T, int LANES, bool POST, bool NEXT, bool STREAM>
 __global__ __launch_bounds__(block_of(LANES)) void block_norm_kernel(NormArgs a)
 {
     using Row = RowLanes<T, LANES>;
@@ -176,41 +59,48 @@ __global__ __launch_bounds__(block_of(LANES)) void block_norm_kernel(NormArgs a)
     const Row rl;
     int turn = 0;
     int col[K], left[K];
-    float weight[K][V], scale[K][V], next_weight[K][V];
+    float factor[K][V], next_weight[K][V];  // scale * weight
 #pragma unroll
     for (int k = 0; k < K; k++) {
         col[k] = rl.col(k);
         left[k] = a.width - col[k];
-        if constexpr (POST) {
-            load_param<V>(a.weight, col[k], left[k], 1.0f, weight[k]);
-            load_param<V>(a.scale, col[k], left[k], 1.0f, scale[k]);
-        }
-        if constexpr (NEXT) load_param<V>(a.next_weight, col[k], left[k], 1.0f, next_weight[k]);
+        if constexpr (POST) load_factor<V>(a, col[k], left[k], factor[k]);
+        if constexpr (NEXT) load_param<V>(a.next_weight, col[k], left[k], next_weight[k]);
     }
-    for (int64_t base = (int64_t)blockIdx.x * rl.rows_per_block; base < a.rows; base += (int64_t)gridDim.x * rl.rows_per_block) {
-        const int64_t row = base + rl.sub;
-        const bool there = row < a.rows;
-        Raw<T, V> xr[K], yr[K], gr[K];
-        int have[K];
+    struct Arrays {
+        Raw<T, V> x[K], y[K], gate[K];
+    };
+    auto fetch = [&](int64_t row, Arrays &r) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            have[k] = there ? left[k] : 0;
+            const int have = row < a.rows ? left[k] : 0;
             const int64_t at = col[k] * (int64_t)sizeof(T);
-            xr[k] = load_row<T, V>(a.x + row * a.x_row + at, a.x_end, have[k]);
+            r.x[k] = load_row<T, V, STREAM>(a.x + row * a.x_row + at, a.x_end, have);
             if constexpr (POST) {
-                yr[k] = load_row<T, V>(a.y + row * a.y_row + at, a.y_end, have[k]);
-                if (a.gate) gr[k] = load_row<T, V>(a.gate + row * a.gate_row + at, a.gate_end, have[k]);
+                r.y[k] = load_row<T, V, STREAM>(a.y + row * a.y_row + at, a.y_end, have);
+                if (a.gate) r.gate[k] = load_row<T, V, STREAM>(a.gate + row * a.gate_row + at, a.gate_end, have);
             }
         }
+    };
+    const int64_t step = (int64_t)gridDim.x * rl.rows_per_block;
+    int64_t base = (int64_t)blockIdx.x * rl.rows_per_block;
+    Arrays in;
+    fetch(base + rl.sub, in);
+    for (; base < a.rows; base += step) {
+        const int64_t row = base + rl.sub;
+        const bool there = row < a.rows;
+        int have[K];
+#pragma unroll
+        for (int k = 0; k < K; k++) have[k] = there ? left[k] : 0;
         const int64_t at_row = row * (int64_t)a.width;
         float o[K][V];
 #pragma unroll
-        for (int k = 0; k < K; k++) widen_row<T, V>(xr[k], have[k], o[k]);
+        for (int k = 0; k < K; k++) widen_row<T, V>(in.x[k], have[k], o[k]);
         if constexpr (POST) {
             float y[K][V], ss = 0.0f;
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                widen_row<T, V>(yr[k], have[k], y[k]);
+                widen_row<T, V>(in.y[k], have[k], y[k]);
 #pragma unroll
                 for (int i = 0; i < V; i++) ss = fmaf(y[k][i], y[k][i], ss);
             }
@@ -219,7 +109,7 @@ __global__ __launch_bounds__(block_of(LANES)) void block_norm_kernel(NormArgs a)
             float z[K][V];
             if (a.gate) {
 #pragma unroll
-                for (int k = 0; k < K; k++) widen_row<T, V>(gr[k], have[k], z[k]);
+                for (int k = 0; k < K; k++) widen_row<T, V>(in.gate[k], have[k], z[k]);
             }
             if (a.y8) checkpoint_row<V, K, LANES>(y, have, col, a.y8 + at_row, a.y8_scale + row * a.groups);
             if (a.gate && a.gate8) checkpoint_row<V, K, LANES>(z, have, col, a.gate8 + at_row, a.gate8_scale + row * a.groups);
@@ -228,9 +118,9 @@ __global__ __launch_bounds__(block_of(LANES)) void block_norm_kernel(NormArgs a)
 #pragma unroll
                 for (int i = 0; i < V; i++) {
                     const float f = a.gate ? activate(z[k][i], a.act) : 1.0f;
-                    o[k][i] = fmaf(scale[k][i] * f, y[k][i] * inv * weight[k][i], o[k][i]);
+                    o[k][i] = fmaf(f * (y[k][i] * inv), factor[k][i], o[k][i]);
                 }
-                if (have[k] > 0) store_row<T, V>(a.out + (at_row + col[k]) * sizeof(T), o[k], have[k]);
+                if (have[k] > 0) store_row<T, V, STREAM>(a.out + (at_row + col[k]) * sizeof(T), o[k], have[k]);
             }
         } else {
             if (a.y8) checkpoint_row<V, K, LANES>(o, have, col, a.y8 + at_row, a.y8_scale + row * a.groups);
@@ -240,242 +130,73 @@ __global__ __launch_bounds__(block_of(LANES)) void block_norm_kernel(NormArgs a)
 #pragma unroll
             for (int k = 0; k < K; k++)
 #pragma unroll
-                for (int i = 0; i < V; i++) ss = i < have[k] ? fmaf(o[k][i], o[k][i], ss) : ss;
+                for (int i = 0; i < V; i++) ss = fmaf(o[k][i], o[k][i], ss);
             const float inv = rsqrtf(rl.sum(ss, slots, turn) / (float)a.width + a.eps);
             if (a.out_inv && there && rl.lane == 0) a.out_inv[row] = inv;
 #pragma unroll
             for (int k = 0; k < K; k++) {
 #pragma unroll
                 for (int i = 0; i < V; i++) o[k][i] *= inv * next_weight[k][i];
-                if (have[k] > 0) store_row<T, V>(a.next + (at_row + col[k]) * sizeof(T), o[k], have[k]);
+                if (have[k] > 0) store_row<T, V, STREAM>(a.next + (at_row + col[k]) * sizeof(T), o[k], have[k]);
             }
         }
+        fetch(row + step, in);
     }
 }
 
-// a vector of an array that may be kept as codes
-template <typename T, int V, bool CODES> struct Saved;
-template <typename T, int V> struct Saved<T, V, false> {
-    Raw<T, V> r;
-    __device__ __forceinline__ void load(const char *p, const char *end, const int8_t *, const float *, int, int left)
-    {
-        r = load_row<T, V>(p, end, left);
-    }
-    __device__ __forceinline__ void get(float (&f)[V], int left) const { widen_row<T, V>(r, left, f); }
-};
-template <typename T, int V> struct Saved<T, V, true> {
-    uint32_t w[V / 4];
-    float scale;
-    __device__ __forceinline__ void load(const char *, const char *, const int8_t *codes, const float *scales, int col, int left)
-    {
-        scale = 0.0f;
-#pragma unroll
-        for (int j = 0; j < V / 4; j++) w[j] = 0;
-        if (left <= 0) return;
-        scale = scales[col / IGX_PACK8_GROUP];
-        if (left >= V) {
-            __builtin_memcpy(w, codes + col, V);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; i++)
-                if (i < left) w[i / 4] |= (uint32_t)(uint8_t)codes[col + i] << (8 * (i % 4));
-        }
-    }
-    __device__ __forceinline__ void get(float (&f)[V], int left) const
-    {
-#pragma unroll
-        for (int i = 0; i < V; i++) f[i] = i < left ? (float)(int8_t)(w[i / 4] >> (8 * (i % 4))) * scale : 0.0f;
-    }
-};
-
-template <typename T, int LANES, bool POST, bool NEXT, bool CODES>
-__global__ __launch_bounds__(block_of(LANES)) void block_norm_backward_kernel(NormArgs a)
+template <typename T, int LANES, bool STREAM> void launch_as(const NormArgs &a, dim3 grid, dim3 block, hipStream_t s)
 {
-    using Row = RowLanes<T, LANES>;
-    constexpr int V = Row::V, K = Row::K;
-    __shared__ float slots[32];
-    __shared__ float joined[LANES > 0 ? kBlock * kColumns : 1];
-    const Row rl;
-    int turn = 0;
-    int col[K], left[K];
-    float weight[K][V], scale[K][V], next_weight[K][V];
-    float sw[K][V], ss[K][V], sn[K][V];
-    const float per = 1.0f / (float)a.width;
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        col[k] = rl.col(k);
-        left[k] = a.width - col[k];
-        if constexpr (POST) {
-            load_param<V>(a.weight, col[k], left[k], 1.0f, weight[k]);
-            load_param<V>(a.scale, col[k], left[k], 1.0f, scale[k]);
-        }
-        if constexpr (NEXT) load_param<V>(a.next_weight, col[k], left[k], 1.0f, next_weight[k]);
-#pragma unroll
-        for (int i = 0; i < V; i++) sw[k][i] = ss[k][i] = sn[k][i] = 0.0f;
-    }
-    for (int64_t base = (int64_t)blockIdx.x * rl.rows_per_block; base < a.rows; base += (int64_t)gridDim.x * rl.rows_per_block) {
-        const int64_t row = base + rl.sub;
-        const bool there = row < a.rows;
-        const int64_t at_row = row * (int64_t)a.width;
-        Raw<T, V> dor[K], dnr[K];
-        Saved<T, V, CODES && !POST> xs[K];
-        Saved<T, V, CODES> ys[K], gs[K];
-        int have[K];
-        float inv_y = 0.0f, inv_o = 0.0f;
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            have[k] = there ? left[k] : 0;
-            const int64_t at = col[k] * (int64_t)sizeof(T);
-            if (a.d_out) dor[k] = load_row<T, V>(a.d_out + row * a.d_out_row + at, a.d_out_end, have[k]);
-            if constexpr (NEXT) {
-                if (a.d_next) dnr[k] = load_row<T, V>(a.d_next + row * a.d_next_row + at, a.d_next_end, have[k]);
-                if constexpr (POST) xs[k].load(a.x + row * a.x_row + at, a.x_end, nullptr, nullptr, 0, have[k]);
-                else xs[k].load(a.x + row * a.x_row + at, a.x_end, a.y8 + at_row, a.y8_scale + row * a.groups, col[k], have[k]);
-            }
-            if constexpr (POST) {
-                ys[k].load(a.y + row * a.y_row + at, a.y_end, a.y8 + at_row, a.y8_scale + row * a.groups, col[k], have[k]);
-                if (a.gate)
-                    gs[k].load(a.gate + row * a.gate_row + at, a.gate_end, a.gate8 + at_row, a.gate8_scale + row * a.groups,
-                               col[k], have[k]);
-            }
-        }
-        if (there) {
-            if constexpr (POST) inv_y = a.y_inv[row];
-            if constexpr (NEXT) inv_o = a.out_inv[row];
-        }
-        float d[K][V];
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            if (a.d_out) {
-                widen_row<T, V>(dor[k], have[k], d[k]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; i++) d[k][i] = 0.0f;
-            }
-        }
-        float unit[K][V], f[K][V], slope[K][V];  // rms(y), act(gate) and its derivative
-        if constexpr (POST) {
-#pragma unroll
-            for (int k = 0; k < K; k++) {
-                ys[k].get(unit[k], have[k]);
-                float z[V];
-                if (a.gate) gs[k].get(z, have[k]);
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    unit[k][i] *= inv_y;
-                    f[k][i] = 1.0f;
-                    slope[k][i] = 0.0f;
-                    if (a.gate) activate_slope(z[i], a.act, f[k][i], slope[k][i]);
-                }
-            }
-        }
-        if constexpr (NEXT) {
-            float u[K][V], t[K][V], dot = 0.0f;  // rms(out), what reaches it
-#pragma unroll
-            for (int k = 0; k < K; k++) {
-                xs[k].get(u[k], have[k]);
-                if (a.d_next) {
-                    widen_row<T, V>(dnr[k], have[k], t[k]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; i++) t[k][i] = 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    if constexpr (POST) u[k][i] = fmaf(scale[k][i] * f[k][i], unit[k][i] * weight[k][i], u[k][i]);
-                    u[k][i] *= inv_o;
-                    sn[k][i] = fmaf(t[k][i], u[k][i], sn[k][i]);
-                    t[k][i] *= next_weight[k][i];
-                    dot = fmaf(t[k][i], u[k][i], dot);
-                }
-            }
-            dot = rl.sum(dot, slots, turn) * per;
-#pragma unroll
-            for (int k = 0; k < K; k++)
-#pragma unroll
-                for (int i = 0; i < V; i++) d[k][i] = fmaf(inv_o, fmaf(-u[k][i], dot, t[k][i]), d[k][i]);
-        }
-        if (a.d_x) {
-#pragma unroll
-            for (int k = 0; k < K; k++)
-                if (have[k] > 0) store_row<T, V>(a.d_x + (at_row + col[k]) * sizeof(T), d[k], have[k]);
-        }
-        if constexpr (POST) {
-            float t[K][V], dot = 0.0f;
-#pragma unroll
-            for (int k = 0; k < K; k++) {
-                float dg[V];
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    const float normed = unit[k][i] * weight[k][i];
-                    dg[i] = d[k][i] * scale[k][i] * normed * slope[k][i];
-                    ss[k][i] = fmaf(d[k][i] * f[k][i], normed, ss[k][i]);
-                    t[k][i] = d[k][i] * scale[k][i] * f[k][i];
-                    sw[k][i] = fmaf(t[k][i], unit[k][i], sw[k][i]);
-                    t[k][i] *= weight[k][i];
-                    dot = fmaf(t[k][i], unit[k][i], dot);
-                }
-                if (a.d_gate && have[k] > 0) store_row<T, V>(a.d_gate + (at_row + col[k]) * sizeof(T), dg, have[k]);
-            }
-            dot = rl.sum(dot, slots, turn) * per;
-            if (a.d_y) {
-#pragma unroll
-                for (int k = 0; k < K; k++) {
-#pragma unroll
-                    for (int i = 0; i < V; i++) t[k][i] = inv_y * fmaf(-unit[k][i], dot, t[k][i]);
-                    if (have[k] > 0) store_row<T, V>(a.d_y + (at_row + col[k]) * sizeof(T), t[k], have[k]);
-                }
-            }
-        }
-    }
-    // the workgroup's column sums
-    int64_t at = 0;
-    auto join = [&](const float (&s)[K][V], bool wanted) {
-        if (!wanted) return;
-        float *to = a.partial + at + (int64_t)blockIdx.x * a.width;
-        at += (int64_t)gridDim.x * a.width;
-        if constexpr (LANES <= 0) {
-#pragma unroll
-            for (int k = 0; k < K; k++)
-#pragma unroll
-                for (int i = 0; i < V; i++)
-                    if (i < left[k]) to[col[k] + i] = s[k][i];
-        } else {
-            constexpr int kSpan = LANES * kColumns;
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < K; k++)
-#pragma unroll
-                for (int i = 0; i < V; i++) joined[rl.sub * kSpan + col[k] + i] = s[k][i];
-            __syncthreads();
-            for (int c = threadIdx.x; c < a.width; c += kBlock) {
-                float v = 0.0f;
-                for (int r = 0; r < kBlock / LANES; r++) v += joined[r * kSpan + c];
-                to[c] = v;
-            }
-        }
-    };
-    if constexpr (POST) {
-        join(sw, a.sum_weight);
-        join(ss, a.sum_scale);
-    }
-    if constexpr (NEXT) join(sn, a.sum_next);
+    if (a.y && a.next_weight) block_norm_kernel<T, LANES, true, true, STREAM><<<grid, block, 0, s>>>(a);
+    else if (a.y) block_norm_kernel<T, LANES, true, false, STREAM><<<grid, block, 0, s>>>(a);
+    else block_norm_kernel<T, LANES, false, true, STREAM><<<grid, block, 0, s>>>(a);
 }
+
+template <typename T, int LANES> void launch_lanes(const NormArgs &a, bool stream_past, dim3 grid, dim3 block, hipStream_t s)
+{
+    if (stream_past) launch_as<T, LANES, true>(a, grid, block, s);
+    else launch_as<T, LANES, false>(a, grid, block, s);
+}
+
+template <typename T> void launch_type(const NormArgs &a, bool stream_past, int64_t blocks, hipStream_t s)
+{
+    const int lanes = lanes_for(a.width);
+    const dim3 grid((unsigned)blocks), block(lanes > 64 ? lanes : kNormBlock);
+    if (lanes == 8) launch_lanes<T, 8>(a, stream_past, grid, block, s);
+    else if (lanes == 16) launch_lanes<T, 16>(a, stream_past, grid, block, s);
+    else if (lanes == 32) launch_lanes<T, 32>(a, stream_past, grid, block, s);
+    else if (lanes == 64) launch_lanes<T, 64>(a, stream_past, grid, block, s);
+    else if (lanes <= 512) launch_lanes<T, kWorkgroup>(a, stream_past, grid, block, s);
+    else launch_lanes<T, kLargest>(a, stream_past, grid, block, s);
+}
+
+}  // namespace
+
+void launch_block_norm(const NormArgs &a, int dtype, bool stream_past, int64_t blocks, hipStream_t s)
+{
+    if (dtype == IGX_F32) launch_type<float>(a, stream_past, blocks, s);
+    else if (dtype == IGX_F16) launch_type<_Float16>(a, stream_past, blocks, s);
+    else launch_type<__bf16>(a, stream_past, blocks, s);
+}
+
+namespace {
 
 struct SumArgs {
-    const float *partial;
-    float *to[3];
+    const float *block, *next;    // the partial rows of each sum
+    bool sum_block;               // is the block's wanted (then its workgroups come first)
+    const float *weight, *scale;  // d_weight = scale * the block's sum, d_scale = weight * it
+    float *d_weight, *d_scale, *d_next_weight;
     int64_t blocks;
     int width;
 };
 
-// sums[c] = partial[0][c] + partial[1][c] + ...: 64 columns a workgroup, its 16 waves share the rows and are joined in order
+// sum[c] = partial[0][c] + partial[1][c] + ...: 64 columns a workgroup, its 16 waves share the rows and are joined in order
 __global__ __launch_bounds__(1024) void column_sum_kernel(SumArgs a)
 {
     __shared__ float part[16][64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int c = blockIdx.x * 64 + lane;
-    const float *p = a.partial + (int64_t)blockIdx.y * a.blocks * a.width;
+    const bool next = !a.sum_block || blockIdx.y == 1;
+    const float *p = next ? a.next : a.block;
     float v = 0.0f;
     if (c < a.width) {
 #pragma unroll 4
@@ -487,27 +208,35 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(SumArgs a)
         v = 0.0f;
 #pragma unroll
         for (int w = 0; w < 16; w++) v += part[w][lane];
-        a.to[blockIdx.y][c] = v;
+        if (next) {
+            a.d_next_weight[c] = v;
+        } else {
+            if (a.d_weight) a.d_weight[c] = a.scale ? v * a.scale[c] : v;
+            if (a.d_scale) a.d_scale[c] = v * a.weight[c];
+        }
     }
 }
 
-// lanes of a row: the fewest that hold its columns; above 64 a workgroup of that many
-int lanes_for(int64_t width)
-{
-    int lanes = 8;
-    while (lanes * kColumns < width) lanes *= 2;
-    return lanes;
-}
-
-// workgroups: enough to fill every CU (16 waves each), each with at least one group of rows
+// Workgroups: as many as run at a time, which walk over the rows - more would start when the first are done and leave most
+// of the card idle at the end (backward of 2^20 x 256 bf16: 871 us with the 12 waves a CU holds, 1 046 with 16).  Without a
+// block (waves 0) a lane keeps only the norm's weight, and a workgroup for every group of rows is faster: 2^20 x 256 fp32
+// 338 us, 398 walking.
 int64_t blocks_for(int64_t rows, int64_t width, int64_t waves_per_cu)
 {
     const int lanes = lanes_for(width);
-    const int64_t threads = lanes > 64 ? lanes : kBlock, rows_per_block = lanes > 64 ? 1 : kBlock / lanes;
-    const int64_t most = 256 * waves_per_cu * 64 / threads, need = ceil_div(rows, rows_per_block);
+    const int64_t threads = lanes > 64 ? lanes : kNormBlock, rows_per_block = lanes > 64 ? 1 : kNormBlock / lanes;
+    const int64_t need = ceil_div(rows, rows_per_block);
+    const int64_t most = waves_per_cu ? 256 * waves_per_cu * 64 / threads : (int64_t)1 << 21;
     return need < most ? need : most;
 }
-constexpr int64_t kForwardWaves = 32, kBackwardWaves = 16;
+constexpr int64_t kForwardWaves = 16, kBackwardWaves = 12;
+
+// Does the call move more than the 256 MB that the last level of cache holds?  (2^20 x 256 bf16, forward and backward: 1 388 us
+// past the caches, 1 465 through them; 16 411 x 211 fp32: 56 and 51.)
+bool beyond_cache(const igx_block_norm *b, int64_t arrays)
+{
+    return arrays * b->rows * b->width * element_size(b->dtype) > (int64_t)256 << 20;
+}
 
 int check(const igx_block_norm *b, const char *who)
 {
@@ -564,51 +293,6 @@ void base_args(const igx_block_norm *b, NormArgs &a)
     a.eps = b->eps;
 }
 
-template <typename T, int LANES> void launch_forward(const NormArgs &a, dim3 grid, dim3 block, hipStream_t s)
-{
-    if (a.y && a.next_weight) block_norm_kernel<T, LANES, true, true><<<grid, block, 0, s>>>(a);
-    else if (a.y) block_norm_kernel<T, LANES, true, false><<<grid, block, 0, s>>>(a);
-    else block_norm_kernel<T, LANES, false, true><<<grid, block, 0, s>>>(a);
-}
-
-template <typename T, int LANES, bool CODES> void launch_backward_as(const NormArgs &a, dim3 grid, dim3 block, hipStream_t s)
-{
-    if (a.y && a.next_weight) block_norm_backward_kernel<T, LANES, true, true, CODES><<<grid, block, 0, s>>>(a);
-    else if (a.y) block_norm_backward_kernel<T, LANES, true, false, CODES><<<grid, block, 0, s>>>(a);
-    else block_norm_backward_kernel<T, LANES, false, true, CODES><<<grid, block, 0, s>>>(a);
-}
-
-template <typename T, int LANES> void launch_backward(const NormArgs &a, dim3 grid, dim3 block, hipStream_t s)
-{
-    if (a.y8) launch_backward_as<T, LANES, true>(a, grid, block, s);
-    else launch_backward_as<T, LANES, false>(a, grid, block, s);
-}
-
-template <typename T> void launch_type(const NormArgs &a, bool backward, int64_t blocks, hipStream_t s)
-{
-    const int lanes = lanes_for(a.width);
-    const dim3 grid((unsigned)blocks), block(lanes > 64 ? lanes : kBlock);
-#define IGX_NORM_GO(L)                                        \
-    do {                                                      \
-        if (backward) launch_backward<T, L>(a, grid, block, s); \
-        else launch_forward<T, L>(a, grid, block, s);         \
-    } while (0)
-    if (lanes == 8) IGX_NORM_GO(8);
-    else if (lanes == 16) IGX_NORM_GO(16);
-    else if (lanes == 32) IGX_NORM_GO(32);
-    else if (lanes == 64) IGX_NORM_GO(64);
-    else if (lanes <= 512) IGX_NORM_GO(kWorkgroup);
-    else IGX_NORM_GO(kLargest);
-#undef IGX_NORM_GO
-}
-
-void launch(const NormArgs &a, int dtype, bool backward, int64_t blocks, hipStream_t s)
-{
-    if (dtype == IGX_F32) launch_type<float>(a, backward, blocks, s);
-    else if (dtype == IGX_F16) launch_type<_Float16>(a, backward, blocks, s);
-    else launch_type<__bf16>(a, backward, blocks, s);
-}
-
 }  // namespace
 }  // namespace igx
 
@@ -623,7 +307,9 @@ extern "C" int igx_block_norm_forward(const igx_block_norm *b, igx_stream_t stre
     if (b->next_weight) IGX_REQUIRE_PTR(b->next, "next");
     igx::NormArgs a;
     igx::base_args(b, a);
-    igx::launch(a, b->dtype, false, igx::blocks_for(b->rows, b->width, igx::kForwardWaves), static_cast<hipStream_t>(stream));
+    const int64_t arrays = 1 + (b->y != nullptr) * 2 + (b->gate != nullptr) + (b->next_weight != nullptr);
+    igx::launch_block_norm(a, b->dtype, igx::beyond_cache(b, arrays), igx::blocks_for(b->rows, b->width, b->y ? igx::kForwardWaves : 0),
+                           static_cast<hipStream_t>(stream));
     return igx::launch_status(__func__);
 }
 
@@ -631,7 +317,7 @@ extern "C" int64_t igx_block_norm_workspace(const igx_block_norm *b)
 {
     const int rc = igx::check(b, __func__);
     if (rc) return rc;
-    return 3 * igx::blocks_for(b->rows, b->width, igx::kBackwardWaves) * b->width * (int64_t)sizeof(float);
+    return 2 * igx::blocks_for(b->rows, b->width, igx::kBackwardWaves) * b->width * (int64_t)sizeof(float);
 }
 
 extern "C" int igx_block_norm_backward(const igx_block_norm *b, const igx_block_norm_grad *g, igx_stream_t stream)
@@ -646,9 +332,8 @@ extern "C" int igx_block_norm_backward(const igx_block_norm *b, const igx_block_
     if (!b->next_weight && g->d_next_weight)
         return igx::fail(IGX_E_PARAM, "%s: d_next_weight is wanted, but next_weight is NULL", __func__);
     if (b->rows && !b->gate && g->d_gate) return igx::fail(IGX_E_PARAM, "%s: d_gate is wanted, but gate is NULL", __func__);
-    float *sums[3] = {g->d_weight, g->d_scale, g->d_next_weight};
-    int wanted = 0;
-    for (float *p : sums) wanted += p != nullptr;
+    const bool sum_block = g->d_weight || g->d_scale, sum_next = g->d_next_weight != nullptr;
+    const int wanted = sum_block + sum_next;
     if (wanted == 0 && !g->d_x && !g->d_y && !g->d_gate) return IGX_OK;
     const int64_t blocks = igx::blocks_for(b->rows, b->width, igx::kBackwardWaves);
     if (b->rows > 0) {
@@ -658,7 +343,7 @@ extern "C" int igx_block_norm_backward(const igx_block_norm *b, const igx_block_
         if (wanted) {
             IGX_REQUIRE_PTR(g->workspace, "workspace");
             IGX_REQUIRE_ALIGNED(g->workspace, "workspace");
-            if (g->workspace_bytes < 3 * blocks * b->width * (int64_t)sizeof(float))
+            if (g->workspace_bytes < 2 * blocks * b->width * (int64_t)sizeof(float))
                 return igx::fail(IGX_E_SIZE, "%s: workspace of %lld bytes is smaller than igx_block_norm_workspace()", __func__,
                                  (long long)g->workspace_bytes);
         }
@@ -678,17 +363,18 @@ extern "C" int igx_block_norm_backward(const igx_block_norm *b, const igx_block_
         a.d_y = static_cast<char *>(g->d_y);
         a.d_gate = static_cast<char *>(g->d_gate);
         a.partial = static_cast<float *>(g->workspace);
-        a.sum_weight = g->d_weight != nullptr;
-        a.sum_scale = g->d_scale != nullptr;
-        a.sum_next = g->d_next_weight != nullptr;
-        igx::launch(a, b->dtype, true, blocks, s);
+        a.sum_block = sum_block;
+        a.sum_next = sum_next;
+        const int64_t arrays = (a.d_out != nullptr) + (a.d_next != nullptr) + (a.d_x != nullptr) + (a.d_y != nullptr) +
+                               (a.d_gate != nullptr) + (b->y != nullptr) + (b->gate != nullptr) + (b->next_weight != nullptr);
+        igx::launch_block_norm_backward(a, b->dtype, igx::beyond_cache(b, arrays), blocks, s);
     }
     if (wanted) {  // without rows: zeros
-        igx::SumArgs sum = {static_cast<const float *>(g->workspace), {}, blocks, (int)b->width};
-        int n = 0;
-        for (float *p : sums)
-            if (p) sum.to[n++] = p;
-        igx::column_sum_kernel<<<dim3((unsigned)igx::ceil_div(b->width, 64), n), dim3(1024), 0, s>>>(sum);
+        const float *partial = static_cast<const float *>(g->workspace);
+        const float *second = partial + (sum_block ? blocks * b->width : 0);
+        const igx::SumArgs sum = {partial, second, sum_block, b->weight, b->scale, g->d_weight, g->d_scale,
+                                  g->d_next_weight, blocks, (int)b->width};
+        igx::column_sum_kernel<<<dim3((unsigned)igx::ceil_div(b->width, 64), wanted), dim3(1024), 0, s>>>(sum);
     }
     return igx::launch_status(__func__);
 }

@@ -1,0 +1,504 @@
+// The linear recurrence's kernels (recurrence.hip instantiates the forward, recurrence_backward.hip the backward ones).
+#pragma once
+#include "igx_seq.hpp"
+
+namespace igx {
+
+constexpr int kRecBlock = 256;
+
+// reset flags a lane needs for a step: its channels belong to one environment, to two, or to any number
+enum Flags { kNoFlags = 0, kOneFlag = 1, kTwoFlags = 2, kFlagEach = 3 };
+
+// One call as the kernels see it.  The steps are numbered in the order they are computed (the host turns an array
+// round by pointing at its last step and negating its stride), strides are in bytes.  Forward reads gate and `add` = inp;
+// backward runs the other way, add = d_out, before = out one step further on.
+struct RecArgs {
+    const char *gate, *add, *reset, *before;
+    char *to, *d_gate;          // forward: out; backward: d_inp, d_gate (NULL: not wanted)
+    const float *start;         // forward: state, backward: d_last; NULL: zeros
+    float *end;                 // forward: last, backward: d_state; NULL: not wanted
+    const float *state;         // backward: what stands before the first step; NULL: zeros
+    float *spans;               // [0]: start; [1 + 2 s], [2 + 2 s]: A and B of span s; rows of `vectors` lane vectors
+    int64_t gate_t, gate_n, add_t, add_n, reset_t, reset_n, before_t, before_n, to_t, to_n, d_gate_t, d_gate_n;
+    int64_t T, span;            // steps in all, and in a span
+    uint32_t D;
+    uint32_t run;      // channels that are adjacent in every array: N * D where the environments follow each other, else D
+    uint32_t per_run;  // vectors in a run
+    uint32_t vectors;  // vectors in all
+    int splat;         // one gate for all channels of a run
+};
+
+// Which channels a lane owns: V of them from `col` of run `row`.  The last vector of a run that V does not divide is
+// moved back to end with the run: its first `skip` channels belong to the lane before and are computed but not stored.
+struct Lane {
+    uint32_t row, col;
+    int skip;
+    int64_t channel;  // of state, last and their gradients
+};
+
+template <int V> __device__ __forceinline__ Lane lane_of(const RecArgs &a, uint32_t v)
+{
+    Lane l;
+    l.row = a.per_run == a.vectors ? 0 : v / a.per_run;
+    l.col = (v - l.row * a.per_run) * V;
+    l.skip = 0;
+    if (V > 1 && a.run - l.col < V) {
+        l.skip = (int)(V - (a.run - l.col));
+        l.col = a.run - V;
+    }
+    l.channel = (int64_t)l.row * a.run + l.col;
+    return l;
+}
+
+template <typename T, int V, bool STREAM = false> __device__ __forceinline__ void store_from(char *p, const float (&f)[V], int skip)
+{
+    if (V == 1 || skip == 0) {
+        store_vec<T, V, STREAM>(p, f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i >= skip) reinterpret_cast<T *>(p)[i] = (T)f[i];
+    }
+}
+
+// Reset flags of the lane's channels for one step: one environment's, that of the first and the last (the environment
+// changes at channel `cut`), or each channel's.
+template <int V, int FL> struct LaneFlags {
+    static constexpr int kCount = FL == kFlagEach ? V : FL == kTwoFlags ? 2 : 1;
+    const char *p[kCount];
+    int cut;
+    __device__ __forceinline__ LaneFlags(const RecArgs &a, const Lane &l)
+    {
+        if constexpr (FL == kNoFlags) return;
+        // a run of D channels is one environment; the only run of N * D holds them all
+#pragma unroll
+        for (int i = 0; i < kCount; i++) {
+            const uint32_t env = l.row + (l.col + (FL == kTwoFlags && i ? V - 1 : i)) / a.D;
+            p[i] = a.reset + (int64_t)env * a.reset_n;
+            if (FL == kTwoFlags && i) cut = (int)((env - l.row) * a.D - l.col);
+        }
+    }
+};
+
+// Steps whose loads a lane has in flight, by the groups that share a workgroup's channels (measured, forward + backward):
+// with a lane for all steps 1, since thousands of waves are in flight and fewer rows [N, D] open at a time suit HBM better
+// (32 x 65 536 x 64 bf16: 406 us with 1, 415 with 2, 431 with 4, 475 with 8); with four groups 2 (32 x 4 096 x 64 fp32:
+// 49 us, 51 with 4, 55 with 8); with sixteen, where waves are few, 8 (2 048 x 16 x 1 024 bf16: 172 us, 237 with 4).
+constexpr int steps_of(int seg) { return seg == 1 ? 1 : seg == 4 ? 2 : 8; }
+
+template <int V, int FL> struct StepFlags {
+    using Places = LaneFlags<V, FL>;
+    int64_t f[Places::kCount];
+    int cut;
+    __device__ __forceinline__ void load(const Places &lf, int64_t off)
+    {
+        if constexpr (FL != kNoFlags) {
+#pragma unroll
+            for (int i = 0; i < Places::kCount; i++) f[i] = *reinterpret_cast<const int64_t *>(lf.p[i] + off);
+            if (FL == kTwoFlags) cut = lf.cut;
+        }
+    }
+    __device__ __forceinline__ bool begins(int i) const
+    {
+        if constexpr (FL == kNoFlags) return false;
+        if constexpr (FL == kTwoFlags) return i < cut ? f[0] != 0 : f[1] != 0;
+        return f[FL == kFlagEach ? i : 0] != 0;
+    }
+};
+
+template <typename T, int V, bool STREAM> __device__ __forceinline__ void load_gate(Raw<T, V> &g, const char *p, int splat)
+{
+    if (V == 1 || !splat) {
+        g = load_raw<T, V, STREAM>(p);
+    } else if constexpr (V > 1) {
+        const T one = *reinterpret_cast<const T *>(p);
+#pragma unroll
+        for (int i = 0; i < V; i++) g.v[i] = one;
+    }
+}
+
+// The map of some steps, h -> A h + B.  Behind an episode's start nothing of h is left, not even an inf or NaN times 0:
+// such a map has kDropped for A, a NaN that arithmetic does not produce.  And where nothing is carried in, the result is
+// B whatever A has grown to.
+constexpr uint32_t kDropped = 0x7fc0d209u;
+__device__ __forceinline__ bool dropped(float A) { return __float_as_uint(A) == kDropped; }
+__device__ __forceinline__ float through(float A, float B, float h) { return h == 0.0f || dropped(A) ? B : fmaf(A, h, B); }
+
+// K consecutive steps of a lane's channels in registers.  `count` of them exist, the others repeat the last one and are
+// neutral; whole steps of a full group cost no test (CHECK false).
+template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STREAM> struct Steps {
+    Raw<T, V> g[K], x[K], hb[K];
+    StepFlags<V, FL> f[K];
+    int count;
+
+    __device__ __forceinline__ void load(const RecArgs &a, const LaneFlags<V, FL> &lf, const char *gate, const char *add,
+                                         const char *before, int64_t t0, int64_t t1)
+    {
+        count = CHECK ? (t1 - t0 < K ? (int)(t1 - t0) : K) : K;
+        const int64_t most = t1 - 1;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int64_t t = CHECK && t0 + k > most ? most : t0 + k;
+            load_gate<T, V, STREAM>(g[k], gate + t * a.gate_t, a.splat);
+            f[k].load(lf, t * a.reset_t);
+        }
+        if (!BACKWARD || add) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                const int64_t t = CHECK && t0 + k > most ? most : t0 + k;
+                x[k] = load_raw<T, V, STREAM>(add + t * a.add_t);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; k++) x[k] = {};
+        }
+        if (BACKWARD && before) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {  // before the first step stands `state`, which is not in out
+                const int64_t t = CHECK && t0 + k > most ? most : t0 + k;
+                if (t < a.T - 1) hb[k] = load_raw<T, V, STREAM>(before + t * a.before_t);
+            }
+        }
+    }
+    __device__ __forceinline__ bool there(int k) const { return !CHECK || k < count; }
+
+    // the steps as one map (A, B) after those already in it; `starts`: channels in which an episode began
+    __device__ __forceinline__ void reduce(float (&A)[V], float (&B)[V], bool (&starts)[V]) const
+    {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const bool begins = f[k].begins(i);
+                const float gate = raw_at(g[k], i), x1 = raw_at(x[k], i);
+                const float b = BACKWARD ? (begins ? 0.0f : gate * (B[i] + x1)) : (begins ? x1 : fmaf(gate, B[i], x1));
+                A[i] = there(k) ? gate * A[i] : A[i];
+                B[i] = there(k) ? b : B[i];
+                starts[i] = starts[i] || (there(k) && begins);
+            }
+        }
+    }
+
+    // forward: h = gate h + inp -> out.  backward: d = d_out + h -> d_inp, d * before -> d_gate, h = gate d
+    __device__ __forceinline__ void walk(const RecArgs &a, const Lane &l, bool store, char *to, char *d_gate, int64_t t0,
+                                         float (&h)[V]) const
+    {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            if (CHECK && !there(k)) break;
+            const int64_t t = t0 + k;
+            if constexpr (!BACKWARD) {
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const float x1 = raw_at(x[k], i);
+                    h[i] = f[k].begins(i) ? x1 : fmaf(raw_at(g[k], i), h[i], x1);
+                }
+                if (store) store_from<T, V, true>(to + t * a.to_t, h, l.skip);
+            } else {
+                float d[V], dg[V];
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    d[i] = raw_at(x[k], i) + h[i];
+                    dg[i] = 0.0f;
+                    h[i] = f[k].begins(i) ? 0.0f : raw_at(g[k], i) * d[i];
+                }
+                if (d_gate) {
+                    if (t < a.T - 1) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) dg[i] = f[k].begins(i) ? 0.0f : d[i] * raw_at(hb[k], i);
+                    } else if (a.state) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) dg[i] = f[k].begins(i) ? 0.0f : d[i] * a.state[l.channel + i];
+                    }
+                    if (store) store_from<T, V, true>(d_gate + t * a.d_gate_t, dg, l.skip);
+                }
+                if (to && store) store_from<T, V, true>(to + t * a.to_t, d, l.skip);
+            }
+        }
+    }
+};
+
+template <int V> __device__ __forceinline__ void identity(float (&A)[V], float (&B)[V], bool (&starts)[V])
+{
+#pragma unroll
+    for (int i = 0; i < V; i++) A[i] = 1.0f, B[i] = 0.0f, starts[i] = false;
+}
+
+// A as the maps hold it
+template <int V> __device__ __forceinline__ void mark(float (&A)[V], const bool (&starts)[V])
+{
+#pragma unroll
+    for (int i = 0; i < V; i++) A[i] = __uint_as_float(starts[i] ? kDropped : A[i] != A[i] ? 0x7fc00000u : __float_as_uint(A[i]));
+}
+
+// where a lane's channels lie in the arrays
+template <typename T> struct Places {
+    const char *gate, *add, *before;
+    char *to, *d_gate;
+    __device__ __forceinline__ Places(const RecArgs &a, const Lane &l)
+    {
+        const int64_t at = (int64_t)l.col * sizeof(T);
+        gate = a.gate + l.row * a.gate_n + (a.splat ? 0 : at);
+        add = a.add ? a.add + l.row * a.add_n + at : nullptr;
+        before = a.before ? a.before + l.row * a.before_n + at : nullptr;
+        to = a.to ? a.to + l.row * a.to_n + at : nullptr;
+        d_gate = a.d_gate ? a.d_gate + l.row * a.d_gate_n + at : nullptr;
+    }
+};
+
+// the carried values of a lane's channels, [N, D] fp32
+template <int V> __device__ __forceinline__ void load_start(const float *p, const Lane &l, float (&h)[V])
+{
+    if (p) {
+        widen(load_raw<float, V>(p + l.channel), h);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) h[i] = 0.0f;
+    }
+}
+
+template <int V> __device__ __forceinline__ void store_end(const RecArgs &a, const Lane &l, const float (&h)[V])
+{
+    if (a.end) store_from<float, V>(reinterpret_cast<char *>(a.end + l.channel), h, l.skip);
+}
+
+// enough channels: a lane walks all the steps
+template <typename T, int V, int FL, bool BACKWARD>
+__global__ __launch_bounds__(kRecBlock) void recurrence_kernel(RecArgs a)
+{
+    const uint32_t v = blockIdx.x * kRecBlock + threadIdx.x;
+    if (v >= a.vectors) return;
+    const Lane l = lane_of<V>(a, v);
+    const LaneFlags<V, FL> lf(a, l);
+    const Places<T> p(a, l);
+    float h[V];
+    load_start<V>(a.start, l, h);
+    for (int64_t t = 0; t < a.T; t++) {
+        Steps<T, V, FL, steps_of(1), BACKWARD, false, true> s;
+        s.load(a, lf, p.gate, p.add, p.before, t, t + 1);
+        s.walk(a, l, true, p.to, p.d_gate, t, h);
+    }
+    store_end<V>(a, l, h);
+}
+
+// V floats of each of a workgroup's lanes, as 16-byte columns without bank conflicts
+template <int V, int LANES> struct Exchange {
+    static constexpr int Q = V >= 4 ? V / 4 : 1, W = V >= 4 ? 4 : V;
+    typedef typename Pack<float, W>::type Word __attribute__((aligned(4 * W)));
+    Word w[Q][LANES];
+    __device__ __forceinline__ void put(int lane, const float (&f)[V])
+    {
+        if constexpr (V == 1) {
+            w[0][lane] = f[0];
+        } else {
+#pragma unroll
+            for (int q = 0; q < Q; q++) w[q][lane] = {f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]};
+        }
+    }
+    __device__ __forceinline__ void get(int lane, float (&f)[V]) const
+    {
+        if constexpr (V == 1) {
+            f[0] = w[0][lane];
+        } else {
+#pragma unroll
+            for (int q = 0; q < Q; q++) {
+                const Word x = w[q][lane];
+#pragma unroll
+                for (int i = 0; i < 4; i++) f[4 * q + i] = x[i];
+            }
+        }
+    }
+};
+
+// the map (A, B) behind (A1, B1), into the latter
+template <int V> __device__ __forceinline__ void compose(float (&A1)[V], float (&B1)[V], const float (&A)[V], const float (&B)[V])
+{
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const bool none = dropped(A[i]) || dropped(A1[i]);
+        const float product = A[i] * A1[i];
+        B1[i] = through(A[i], B[i], B1[i]);
+        A1[i] = __uint_as_float(none ? kDropped : product != product ? 0x7fc00000u : __float_as_uint(product));
+    }
+}
+
+template <int V> __device__ __forceinline__ void load_span(const RecArgs &a, int64_t row, uint32_t v, float (&f)[V])
+{
+    const float *p = a.spans + (row * a.vectors + v) * V;
+    if constexpr (V == 1) f[0] = *p;
+    else widen(load_raw<float, V>(p), f);
+}
+
+// Time split: SEG groups of 256 / SEG lanes take steps_of(SEG) steps each of the same channels; blockIdx.y is the span.
+template <typename T, int V, int FL, bool BACKWARD, int SEG>
+__global__ __launch_bounds__(kRecBlock) void recurrence_split_kernel(RecArgs a)
+{
+    constexpr int LANES = kRecBlock / SEG;
+    __shared__ Exchange<V, LANES> maps[2][SEG][2];
+    const int lane = threadIdx.x % LANES, seg = threadIdx.x / LANES;
+    const uint32_t mine = blockIdx.x * LANES + lane, v = mine < a.vectors ? mine : a.vectors - 1;
+    const bool store = mine < a.vectors;  // the other lanes of the last workgroup repeat its last vector
+    const Lane l = lane_of<V>(a, v);
+    const LaneFlags<V, FL> lf(a, l);
+    const Places<T> p(a, l);
+    const int64_t first = (int64_t)blockIdx.y * a.span, t1 = first + a.span < a.T ? first + a.span : a.T;
+    constexpr int kSteps = steps_of(SEG);
+    Steps<T, V, FL, kSteps, BACKWARD, true, false> s;
+    s.load(a, lf, p.gate, p.add, p.before, first + seg * kSteps, t1);  // on its way while the spans are composed
+    float h[V];
+    if (gridDim.y == 1) {
+        load_start<V>(a.start, l, h);
+    } else {  // each group composes its part of the spans before this one, then all go through the parts
+        const int64_t spans = blockIdx.y, part = ceil_div(spans, SEG);
+        float A[V], B[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) A[i] = 1.0f, B[i] = 0.0f;
+        const int64_t end = (seg + 1) * part < spans ? (seg + 1) * part : spans;
+#pragma unroll 2
+        for (int64_t q = seg * part; q < end; q++) {
+            float A2[V], B2[V];
+            load_span<V>(a, 1 + 2 * q, v, A2);
+            load_span<V>(a, 2 + 2 * q, v, B2);
+            compose<V>(A, B, A2, B2);
+        }
+        maps[1][seg][0].put(lane, A);
+        maps[1][seg][1].put(lane, B);
+        load_span<V>(a, 0, v, h);
+        __syncthreads();
+#pragma unroll 2
+        for (int q = 0; q < SEG; q++) {
+            float A2[V], B2[V];
+            maps[1][q][0].get(lane, A2);
+            maps[1][q][1].get(lane, B2);
+#pragma unroll
+            for (int i = 0; i < V; i++) h[i] = through(A2[i], B2[i], h[i]);
+        }
+    }
+    int turn = 0;
+    for (int64_t t0 = first; t0 < t1; t0 += SEG * kSteps, turn ^= 1) {
+        const int64_t ts = t0 + seg * kSteps, next = t0 + SEG * kSteps;
+        float A[V], B[V], from[V] = {};
+        bool starts[V];
+        identity<V>(A, B, starts);
+        s.reduce(A, B, starts);
+        mark<V>(A, starts);
+        maps[turn][seg][0].put(lane, A);
+        maps[turn][seg][1].put(lane, B);
+        __syncthreads();
+#pragma unroll 2
+        for (int q = 0; q < SEG; q++) {
+            float A2[V], B2[V];
+            maps[turn][q][0].get(lane, A2);
+            maps[turn][q][1].get(lane, B2);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                from[i] = q == seg ? h[i] : from[i];
+                h[i] = through(A2[i], B2[i], h[i]);
+            }
+        }
+        s.walk(a, l, store, p.to, p.d_gate, ts, from);
+        if (next < t1) s.load(a, lf, p.gate, p.add, p.before, next + seg * kSteps, t1);
+    }
+    if (store && seg == 0 && blockIdx.y == gridDim.y - 1) store_end<V>(a, l, h);
+}
+
+// The (A, B) of every span: SEG groups of lanes reduce consecutive parts of it, joined through LDS.
+template <typename T, int V, int FL, bool BACKWARD>
+__global__ __launch_bounds__(kRecBlock) void recurrence_spans_kernel(RecArgs a)
+{
+    constexpr int SEG = 16, LANES = kRecBlock / SEG;
+    __shared__ Exchange<V, LANES> maps[SEG][2];
+    const int lane = threadIdx.x % LANES, seg = threadIdx.x / LANES;
+    const uint32_t mine = blockIdx.x * LANES + lane, v = mine < a.vectors ? mine : a.vectors - 1;
+    const Lane l = lane_of<V>(a, v);
+    const LaneFlags<V, FL> lf(a, l);
+    const Places<T> p(a, l);
+    const int64_t first = (int64_t)blockIdx.y * a.span, last = first + a.span < a.T ? first + a.span : a.T;
+    const int64_t part = ceil_div(a.span, SEG);
+    const int64_t from = first + seg * part, to = from + part < last ? from + part : last;
+    float A[V], B[V];
+    bool starts[V];
+    identity<V>(A, B, starts);
+    constexpr int kSteps = steps_of(16);
+    for (int64_t t = from; t < to; t += kSteps) {
+        Steps<T, V, FL, kSteps, BACKWARD, true, false> s;
+        s.load(a, lf, p.gate, p.add, nullptr, t, to);
+        s.reduce(A, B, starts);
+    }
+    mark<V>(A, starts);
+    maps[seg][0].put(lane, A);
+    maps[seg][1].put(lane, B);
+    __syncthreads();
+    if (seg != 0 || mine >= a.vectors) return;
+#pragma unroll 2
+    for (int q = 1; q < SEG; q++) {
+        float A2[V], B2[V];
+        maps[q][0].get(lane, A2);
+        maps[q][1].get(lane, B2);
+        compose<V>(A, B, A2, B2);
+    }
+    const int64_t at = (int64_t)a.vectors * V;
+    float *to_span = a.spans + (int64_t)v * V;
+    store_vec<float, V>(to_span + (1 + 2 * (int64_t)blockIdx.y) * at, A);
+    store_vec<float, V>(to_span + (2 + 2 * (int64_t)blockIdx.y) * at, B);
+    if (blockIdx.y == 0) {  // the second kernel takes the start from here: `end` may be the array it comes from
+        load_start<V>(a.start, l, A);
+        store_vec<float, V>(to_span, A);
+    }
+}
+
+struct Plan {
+    RecArgs a;
+    int vec;    // channels per lane: the type's 16 bytes, or 4, or 1 where a run is shorter than that
+    int flags;
+    int seg;    // groups of lanes that share a workgroup's channels; 1: a lane walks all steps
+    int64_t spans;
+    int64_t workspace() const { return spans > 1 ? (1 + 2 * spans) * a.vectors * vec * (int64_t)sizeof(float) : 0; }
+};
+
+template <typename T, int V, int FL, bool BACKWARD> void launch_as(const Plan &p, hipStream_t s)
+{
+    const dim3 block(kRecBlock);
+    const uint32_t v = p.a.vectors;
+    if (p.spans > 1)
+        recurrence_spans_kernel<T, V, FL, BACKWARD><<<dim3((unsigned)ceil_div(v, kRecBlock / 16), (unsigned)p.spans), block, 0, s>>>(p.a);
+    if (p.seg == 1) {
+        recurrence_kernel<T, V, FL, BACKWARD><<<dim3((unsigned)ceil_div(v, kRecBlock)), block, 0, s>>>(p.a);
+    } else if (p.seg == 4) {
+        recurrence_split_kernel<T, V, FL, BACKWARD, 4><<<dim3((unsigned)ceil_div(v, kRecBlock / 4)), block, 0, s>>>(p.a);
+    } else {
+        const dim3 grid((unsigned)ceil_div(v, kRecBlock / 16), (unsigned)p.spans);
+        recurrence_split_kernel<T, V, FL, BACKWARD, 16><<<grid, block, 0, s>>>(p.a);
+    }
+}
+
+template <int DT, bool BACKWARD> void launch_type(const Plan &p, hipStream_t s)
+{
+    using T = typename Elem<DT>::type;
+    constexpr int V = Elem<DT>::vec;
+    if (p.vec == 4 && V != 4) {
+        if (p.flags == kNoFlags) launch_as<T, 4, kNoFlags, BACKWARD>(p, s);
+        else if (p.flags == kOneFlag) launch_as<T, 4, kOneFlag, BACKWARD>(p, s);
+        else if (p.flags == kTwoFlags) launch_as<T, 4, kTwoFlags, BACKWARD>(p, s);
+        else launch_as<T, 4, kFlagEach, BACKWARD>(p, s);
+    } else if (p.vec == 1) {
+        if (p.flags == kNoFlags) launch_as<T, 1, kNoFlags, BACKWARD>(p, s);
+        else launch_as<T, 1, kOneFlag, BACKWARD>(p, s);
+    } else {
+        if (p.flags == kNoFlags) launch_as<T, V, kNoFlags, BACKWARD>(p, s);
+        else if (p.flags == kOneFlag) launch_as<T, V, kOneFlag, BACKWARD>(p, s);
+        else if (p.flags == kTwoFlags) launch_as<T, V, kTwoFlags, BACKWARD>(p, s);
+        else launch_as<T, V, kFlagEach, BACKWARD>(p, s);
+    }
+}
+
+template <bool BACKWARD> void launch_recurrence(int dtype, const Plan &p, hipStream_t s)
+{
+    if (dtype == IGX_F32) launch_type<IGX_F32, BACKWARD>(p, s);
+    else if (dtype == IGX_F16) launch_type<IGX_F16, BACKWARD>(p, s);
+    else launch_type<IGX_BF16, BACKWARD>(p, s);
+}
+
+extern template void launch_recurrence<true>(int dtype, const Plan &p, hipStream_t s);
+
+}  // namespace igx

@@ -362,6 +362,40 @@ def test_residual_norm_many_rows():
     check_norm(t, do, dn)
 
 
+@pytest.mark.parametrize("dtype,checkpoint", [(F32, False), (BF16, True)])
+def test_norms_larger_than_the_caches(dtype, checkpoint):
+    """A call that moves more than the caches hold gives every row the bits of a small call on it; its column sums are the
+    small calls' sums, added up in another order: (rows + calls) roundings of the magnitudes' sum."""
+    R, D, part = 1 << 18, 200, 1 << 14
+    g = torch.Generator(device=DEV).manual_seed(33)
+    x, y, z, do, dn = (torch.randn(R, D, device=DEV, generator=g).to(dtype) for _ in range(5))
+    w, s, w2 = (torch.randn(D, device=DEV, generator=g) for _ in range(3))
+    for post in (True, False):
+        def run(lo, hi):
+            leaves = [t[lo:hi].detach().requires_grad_(True) for t in ((x, y, z) if post else (x,))]
+            leaves += [t.detach().requires_grad_(True) for t in ((w, s, w2) if post else (w2,))]
+            if post:
+                outs = sequence.residual_norm(leaves[0], leaves[1], leaves[3], gate=leaves[2], scale=leaves[4],
+                                              next_weight=leaves[5], checkpoint=checkpoint)
+                heads = (do[lo:hi], dn[lo:hi])
+            else:
+                outs, heads = (sequence.rms_norm(leaves[0], leaves[1], checkpoint=checkpoint),), (dn[lo:hi],)
+            grads = torch.autograd.grad(outs, leaves, heads)
+            rows = [o.detach() for o in outs] + list(grads[:3 if post else 1])
+            return rows, [t.double() for t in grads[3 if post else 1:]]
+
+        rows, sums = run(0, R)
+        total = [torch.zeros_like(t) for t in sums]
+        for lo in range(0, R, part):
+            some, parts = run(lo, lo + part)
+            for a, b in zip(rows, some):
+                assert torch.equal(a[lo:lo + part], b)
+            total = [a + b for a, b in zip(total, parts)]
+        for a, b in zip(sums, total):
+            # the terms are d * unit-sized values: their magnitudes' sum is below 16 a row
+            assert ((a - b).abs() <= (R + R // part) * S.U * 16 * R ** 0.5).all()
+
+
 def test_residual_norm_leading_dimensions_and_unused_outputs():
     t, do, dn = norm_inputs(24, 40, F32, 26)
     dev = {k: (v.view(2, 3, 4, 40) if v.dim() == 2 else v).to(DEV).requires_grad_(True) for k, v in t.items()}
