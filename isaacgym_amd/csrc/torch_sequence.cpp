@@ -1,0 +1,539 @@
+// The differentiable forms of the sequence operators (isaacgym_amd.sequence): checks, allocation, autograd nodes and the
+// launches through libigx's C ABI.  They are C++ because a small call is bound by its host time, and a node written in Python
+// costs more than the kernels of a rollout of 4 096 environments (forward and backward of the recurrence: 125 us in Python).
+//
+// The library is not linked: isaacgym_amd._lib, its only loader, hands over the addresses of its entry points.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include "../../include/igx.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+// ---- libigx ---------------------------------------------------------------------------------------------------------
+
+struct Library {
+    decltype(&igx_last_error_string) last_error;
+    decltype(&igx_linear_recurrence_workspace) recurrence_workspace;
+    decltype(&igx_linear_recurrence) recurrence;
+    decltype(&igx_linear_recurrence_backward) recurrence_backward;
+    decltype(&igx_block_norm_workspace) norm_workspace;
+    decltype(&igx_block_norm_forward) norm;
+    decltype(&igx_block_norm_backward) norm_backward;
+    decltype(&igx_pack8) pack8;
+    decltype(&igx_unpack8) unpack8;
+} lib;
+
+struct IgxFailure : std::runtime_error {
+    int code;
+    IgxFailure(int code, const std::string &text) : std::runtime_error(text), code(code) {}
+};
+
+void check(int64_t rc)
+{
+    if (rc) throw IgxFailure((int)rc, lib.last_error());
+}
+
+igx_stream_t stream_of(const Tensor &t)
+{
+    return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream();
+}
+
+// ---- checks of arguments -------------------------------------------------------------------------------------------
+
+int element(const Tensor &t, const char *name)
+{
+    const auto type = t.scalar_type();
+    const int e = type == at::kFloat ? IGX_F32 : type == at::kHalf ? IGX_F16 : type == at::kBFloat16 ? IGX_BF16 : -1;
+    TORCH_CHECK_TYPE(e >= 0, name, ": expected float32, float16 or bfloat16, got ", type);
+    TORCH_CHECK_VALUE(t.is_cuda(), "libigx works on device tensors only (", name, " is a ", t.device(), " tensor)");
+    return e;
+}
+
+void same(const Tensor &t, const char *name, at::IntArrayRef shape, at::ScalarType type, const Tensor &like)
+{
+    TORCH_CHECK_VALUE(t.is_cuda(), "libigx works on device tensors only (", name, " is a ", t.device(), " tensor)");
+    TORCH_CHECK_TYPE(t.scalar_type() == type, name, ": expected dtype ", type, ", got ", t.scalar_type());
+    TORCH_CHECK_VALUE(t.get_device() == like.get_device(), name, " is on ", t.device(), ", others on ", like.device());
+    TORCH_CHECK_VALUE(t.sizes() == shape, name, ": expected shape ", shape, ", got ", t.sizes());
+}
+
+// the address of a contiguous tensor (undefined: NULL)
+template <typename T> T *packed(const Tensor &t, const char *name, at::IntArrayRef shape, at::ScalarType type, const Tensor &like)
+{
+    if (!t.defined()) return nullptr;
+    same(t, name, shape, type, like);
+    TORCH_CHECK_VALUE(t.is_contiguous(), name, " must be contiguous");
+    return static_cast<T *>(t.data_ptr());
+}
+
+bool adjacent(const Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
+
+Tensor given(const OptTensor &t) { return t ? *t : Tensor(); }
+OptTensor maybe(const Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+bool differentiated(std::initializer_list<const Tensor *> tensors)
+{
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor *t : tensors)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+// torch adds a captured gradient to a leaf on the stream where the leaf's accumulator was made: an eager graph that still
+// holds one would drag its stream into the capture, which ends the process.  Such a capture is refused.
+void refuse_foreign_accumulators(std::initializer_list<const Tensor *> tensors, const Tensor &like)
+{
+    c10::DeviceGuard guard(like.device());
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const c10::Stream now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(like.get_device()).unwrap();
+    for (const Tensor *t : tensors) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto made = node ? node->stream() : std::nullopt;
+        TORCH_CHECK(!made || *made == now,
+                    "a tensor that requires grad is still part of an eager autograd graph: release that graph's outputs before "
+                    "capturing one with the same tensor");
+    }
+}
+
+void once(const AutogradContext *)
+{
+    TORCH_CHECK(!at::GradMode::is_enabled(), "the sequence operators' gradients cannot be differentiated again (create_graph=True)");
+}
+
+// ---- linear recurrence ---------------------------------------------------------------------------------------------
+
+// (stride over steps, over environments) of a [T, N, D] tensor with adjacent channels; its address
+template <typename P> void rollout(const Tensor &t, const char *name, const Tensor &like, P &address, int64_t (&stride)[2])
+{
+    if (!t.defined()) return;
+    same(t, name, like.sizes(), like.scalar_type(), like);
+    TORCH_CHECK_VALUE(adjacent(t), name, ": the channels (last dimension) must be adjacent, their stride is ", t.stride(2));
+    address = t.data_ptr();
+    stride[0] = t.stride(0);
+    stride[1] = t.stride(1);
+}
+
+// what forward and backward share; `like` gives shape, type and device
+igx_recurrence recurrence_args(const Tensor &gate, const Tensor &like, const Tensor &state, const Tensor &reset, bool reverse)
+{
+    igx_recurrence r = {};
+    TORCH_CHECK_VALUE(like.dim() == 3, "linear_recurrence: rollouts are [steps, environments, channels] tensors");
+    r.dtype = element(like, "inp");
+    r.reverse = reverse;
+    r.steps = like.size(0);
+    r.envs = like.size(1);
+    r.width = like.size(2);
+    same(gate, "gate", like.sizes(), like.scalar_type(), like);
+    const int64_t sd = like.size(2) > 1 ? gate.stride(2) : 1;
+    TORCH_CHECK_VALUE(sd == 0 || sd == 1, "gate: the channels (last dimension) must be adjacent or share one gate, their stride is ", sd);
+    r.gate = gate.data_ptr();
+    r.gate_stride[0] = gate.stride(0);
+    r.gate_stride[1] = gate.stride(1);
+    r.gate_stride[2] = sd;
+    r.state = packed<float>(state, "state", like.sizes().slice(1), at::kFloat, like);
+    if (reset.defined()) {
+        same(reset, "reset", like.sizes().slice(0, 2), at::kLong, like);
+        r.reset = static_cast<const int64_t *>(reset.data_ptr());
+        r.reset_stride[0] = reset.stride(0);
+        r.reset_stride[1] = reset.stride(1);
+    }
+    return r;
+}
+
+// a call's workspace; back to the stream's pool when it goes out of scope, behind the launch
+Tensor recurrence_workspace(igx_recurrence &r, const Tensor &like)
+{
+    const int64_t size = lib.recurrence_workspace(&r);
+    if (size < 0) check(size);
+    Tensor ws;
+    if (size) {
+        ws = at::empty({size}, like.options().dtype(at::kByte));
+        r.workspace = ws.data_ptr();
+        r.workspace_bytes = size;
+    }
+    return ws;
+}
+
+std::pair<Tensor, Tensor> run_recurrence(const Tensor &gate, const Tensor &inp, const Tensor &state, const Tensor &reset, bool reverse)
+{
+    igx_recurrence r = recurrence_args(gate, inp, state, reset, reverse);
+    rollout(inp, "inp", inp, r.inp, r.inp_stride);
+    c10::DeviceGuard guard(inp.device());
+    Tensor out = at::empty_like(inp);  // in inp's layout, so that neighbouring operators see the one they were given
+    if (!adjacent(out) || (!out.is_contiguous() && !out.is_non_overlapping_and_dense())) out = at::empty(inp.sizes(), inp.options());
+    Tensor last = at::empty(inp.sizes().slice(1), inp.options().dtype(at::kFloat));
+    rollout(out, "out", inp, r.out, r.out_stride);
+    r.last = static_cast<float *>(last.data_ptr());
+    const Tensor ws = recurrence_workspace(r, inp);
+    check(lib.recurrence(&r, stream_of(inp)));
+    return {out, last};
+}
+
+struct LinearRecurrence : torch::autograd::Function<LinearRecurrence> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &gate, const Tensor &inp, const OptTensor &state_,
+                                 const OptTensor &reset_, bool reverse)
+    {
+        const Tensor state = given(state_), reset = given(reset_);
+        ctx->set_materialize_grads(false);
+        auto [out, last] = run_recurrence(gate, inp, state, reset, reverse);
+        ctx->save_for_backward({gate, out, state, reset});
+        ctx->saved_data["reverse"] = reverse;
+        return {out, last};
+    }
+
+    static variable_list backward(AutogradContext *ctx, const variable_list &grads)
+    {
+        once(ctx);
+        Tensor d_out = grads[0], d_last = grads[1];
+        variable_list result(5);
+        if (!d_out.defined() && !d_last.defined()) return result;
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &gate = saved[0], &out = saved[1], &state = saved[2], &reset = saved[3];
+        c10::DeviceGuard guard(out.device());
+        if (d_out.defined() && !adjacent(d_out)) d_out = d_out.contiguous();
+        if (d_last.defined()) d_last = d_last.contiguous();
+        igx_recurrence r = recurrence_args(gate, out, state, reset, ctx->saved_data["reverse"].toBool());
+        igx_recurrence_grad g = {};
+        rollout(out, "out", out, r.out, r.out_stride);
+        rollout(d_out, "d_out", out, g.d_out, g.d_out_stride);
+        g.d_last = packed<float>(d_last, "d_last", out.sizes().slice(1), at::kFloat, out);
+        if (ctx->needs_input_grad(0)) rollout(result[0] = at::empty_like(out), "d_gate", out, g.d_gate, g.d_gate_stride);
+        if (ctx->needs_input_grad(1)) rollout(result[1] = at::empty_like(out), "d_inp", out, g.d_inp, g.d_inp_stride);
+        if (state.defined() && ctx->needs_input_grad(2)) {
+            result[2] = at::empty_like(state);
+            g.d_state = static_cast<float *>(result[2].data_ptr());
+        }
+        const Tensor ws = recurrence_workspace(r, out);
+        check(lib.recurrence_backward(&r, &g, stream_of(out)));
+        return result;
+    }
+};
+
+std::pair<Tensor, Tensor> linear_recurrence(const Tensor &gate_, const Tensor &inp, const OptTensor &state_, const OptTensor &reset_,
+                                            bool reverse)
+{
+    const Tensor gate = gate_.sizes() == inp.sizes() ? gate_ : gate_.expand(inp.sizes());
+    const Tensor state = given(state_), reset = given(reset_);
+    if (!differentiated({&gate, &inp, &state})) return run_recurrence(gate, inp, state, reset, reverse);
+    if (inp.is_cuda()) refuse_foreign_accumulators({&gate, &inp, &state}, inp);
+    const variable_list v = LinearRecurrence::apply(gate, inp, maybe(state), maybe(reset), reverse);
+    return {v[0], v[1]};
+}
+
+Tensor linear_recurrence_step(const Tensor &gate_, const Tensor &inp, const Tensor &state, const OptTensor &reset_,
+                              const OptTensor &state_out, const OptTensor &out_)
+{
+    TORCH_CHECK_VALUE(inp.dim() == 2, "linear_recurrence_step: gate and inp are [environments, channels] tensors");
+    const at::NoGradGuard no_grad;
+    const Tensor gate = gate_.sizes() == inp.sizes() ? gate_ : gate_.expand(inp.sizes()), reset = given(reset_);
+    igx_recurrence r = {};
+    r.dtype = element(inp, "inp");
+    r.steps = 1;
+    r.envs = inp.size(0);
+    r.width = inp.size(1);
+    same(gate, "gate", inp.sizes(), inp.scalar_type(), inp);
+    const int64_t sd = r.width > 1 ? gate.stride(1) : 1;
+    TORCH_CHECK_VALUE(sd == 0 || sd == 1, "gate: the channels (last dimension) must be adjacent or share one gate, their stride is ", sd);
+    TORCH_CHECK_VALUE(adjacent(inp), "inp: the channels (last dimension) must be adjacent, their stride is ", inp.stride(1));
+    r.gate = gate.data_ptr();
+    r.gate_stride[1] = gate.stride(0);
+    r.gate_stride[2] = sd;
+    r.inp = inp.data_ptr();
+    r.inp_stride[1] = inp.stride(0);
+    r.state = packed<float>(state, "state", inp.sizes(), at::kFloat, inp);
+    const Tensor to = state_out ? *state_out : state;
+    r.last = packed<float>(to, "state_out", inp.sizes(), at::kFloat, inp);
+    if (reset.defined()) {
+        same(reset, "reset", inp.sizes().slice(0, 1), at::kLong, inp);
+        r.reset = static_cast<const int64_t *>(reset.data_ptr());
+        r.reset_stride[1] = reset.stride(0);
+    }
+    c10::DeviceGuard guard(inp.device());
+    const Tensor out = out_ ? *out_ : at::empty(inp.sizes(), inp.options());
+    packed<char>(out, "out", inp.sizes(), inp.scalar_type(), inp);
+    TORCH_CHECK_VALUE(!out.numel() || (out.data_ptr() != r.gate && out.data_ptr() != r.inp && out.data_ptr() != r.state && out.data_ptr() != r.last),
+                      "out must not overlap an input");
+    r.out = out.data_ptr();
+    r.out_stride[1] = r.width;
+    check(lib.recurrence(&r, stream_of(inp)));
+    return out;
+}
+
+// ---- block norms ---------------------------------------------------------------------------------------------------
+
+// the address of a [..., width] tensor with adjacent columns and evenly spaced rows, and the stride from row to row
+template <typename P> void row_array(const Tensor &t, const char *name, const Tensor &like, P &address, int64_t &stride)
+{
+    if (!t.defined()) return;
+    same(t, name, like.sizes(), like.scalar_type(), like);
+    address = t.data_ptr();
+    stride = like.size(-1);
+    if (t.is_contiguous()) return;
+    TORCH_CHECK_VALUE(adjacent(t), name, ": the columns (last dimension) must be adjacent, their stride is ", t.stride(-1));
+    int64_t reach = 0;  // rows between two entries of the dimension in front; 0 as long as there is one row
+    for (int64_t i = t.dim() - 2; i >= 0; i--) {
+        if (t.size(i) == 1) continue;
+        if (reach == 0) {
+            stride = t.stride(i);
+            reach = t.size(i);
+        } else {
+            TORCH_CHECK_VALUE(t.stride(i) == stride * reach, name, ": its rows (all but the last dimension) must be evenly spaced");
+            reach *= t.size(i);
+        }
+    }
+}
+
+int64_t rows_of(const Tensor &t) { return t.size(-1) ? t.numel() / t.size(-1) : 0; }
+
+std::vector<int64_t> scales_shape(const Tensor &t)
+{
+    std::vector<int64_t> s = t.sizes().vec();
+    s.back() = (s.back() + IGX_PACK8_GROUP - 1) / IGX_PACK8_GROUP;
+    return s;
+}
+
+struct Parameters {
+    Tensor weight, scale, next_weight;
+};
+
+igx_block_norm norm_args(const Tensor &like, const Parameters &p, const Tensor &inv_rms, int64_t activation, double eps)
+{
+    igx_block_norm b = {};
+    b.dtype = element(like, "x");
+    b.activation = (int32_t)activation;
+    b.rows = rows_of(like);
+    b.width = like.size(-1);
+    b.eps = (float)eps;
+    const auto vector = like.sizes().slice(like.dim() - 1);
+    b.weight = packed<float>(p.weight, "weight", vector, at::kFloat, like);
+    b.scale = packed<float>(p.scale, "scale", vector, at::kFloat, like);
+    b.next_weight = packed<float>(p.next_weight, "next_weight", vector, at::kFloat, like);
+    if (inv_rms.defined() && b.rows) {
+        b.y_inv_rms = static_cast<float *>(inv_rms.data_ptr());
+        b.out_inv_rms = b.y_inv_rms + b.rows;
+    }
+    return b;
+}
+
+// (out, next); undefined where the call has none.  inv_rms and the codes are filled in where defined.
+std::pair<Tensor, Tensor> run_norm(const Tensor &x, const Tensor &y, const Tensor &gate, const Parameters &p, int64_t activation,
+                                   double eps, const Tensor &inv_rms, const variable_list &codes)
+{
+    igx_block_norm b = norm_args(x, p, inv_rms, activation, eps);
+    row_array(x, "x", x, b.x, b.x_stride);
+    row_array(y, "y", x, b.y, b.y_stride);
+    row_array(gate, "gate", x, b.gate, b.gate_stride);
+    c10::DeviceGuard guard(x.device());
+    Tensor out, next;
+    if (y.defined()) out = at::empty(x.sizes(), x.options());
+    if (p.next_weight.defined()) next = at::empty(x.sizes(), x.options());
+    if (out.defined()) b.out = out.data_ptr();
+    if (next.defined()) b.next = next.data_ptr();
+    if (codes.size() > 1) {
+        b.y8 = static_cast<int8_t *>(codes[0].data_ptr());
+        b.y8_scale = static_cast<float *>(codes[1].data_ptr());
+    }
+    if (codes.size() > 3) {
+        b.gate8 = static_cast<int8_t *>(codes[2].data_ptr());
+        b.gate8_scale = static_cast<float *>(codes[3].data_ptr());
+    }
+    check(lib.norm(&b, stream_of(x)));
+    return {out, next};
+}
+
+Tensor even_rows(const Tensor &t) { return !t.defined() || t.is_contiguous() ? t : t.contiguous(); }
+
+struct BlockNorm : torch::autograd::Function<BlockNorm> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const OptTensor &y_, const OptTensor &weight_,
+                                 const OptTensor &gate_, const OptTensor &scale_, const OptTensor &next_weight_, int64_t activation,
+                                 double eps, bool checkpoint)
+    {
+        const Tensor y = given(y_), weight = given(weight_), gate = given(gate_), scale = given(scale_), next_weight = given(next_weight_);
+        ctx->set_materialize_grads(false);
+        element(x, "x");
+        c10::DeviceGuard guard(x.device());
+        const Tensor inv_rms = at::empty({2, rows_of(x)}, x.options().dtype(at::kFloat));
+        variable_list codes;
+        if (checkpoint) {
+            for (int i = 0; i < (gate.defined() ? 2 : 1); i++) {
+                codes.push_back(at::empty(x.sizes(), x.options().dtype(at::kChar)));
+                codes.push_back(at::empty(scales_shape(x), x.options().dtype(at::kFloat)));
+            }
+        }
+        auto [out, next] = run_norm(x, y, gate, {weight, scale, next_weight}, activation, eps, inv_rms, codes);
+        const bool keep_x = next_weight.defined() && (y.defined() || !checkpoint);
+        variable_list saved = {keep_x ? x : Tensor(), checkpoint ? Tensor() : y, checkpoint ? Tensor() : gate, weight, scale,
+                               next_weight, inv_rms};
+        saved.insert(saved.end(), codes.begin(), codes.end());
+        ctx->save_for_backward(saved);
+        ctx->saved_data["activation"] = activation;
+        ctx->saved_data["eps"] = eps;
+        variable_list outs;
+        if (out.defined()) outs.push_back(out);
+        if (next.defined()) outs.push_back(next);
+        return outs;
+    }
+
+    static variable_list backward(AutogradContext *ctx, const variable_list &grads)
+    {
+        once(ctx);
+        variable_list result(9);
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &y = saved[1], &gate = saved[2];
+        const Parameters p = {saved[3], saved[4], saved[5]};
+        const bool block = p.weight.defined(), behind = p.next_weight.defined(), codes = saved.size() > 7;
+        const Tensor given_out = block ? grads[0] : Tensor();
+        const Tensor d_out = even_rows(given_out), d_next = even_rows(behind ? grads.back() : Tensor());
+        if (!d_out.defined() && !d_next.defined()) return result;
+        const Tensor &like = d_out.defined() ? d_out : d_next;
+        c10::DeviceGuard guard(like.device());
+        igx_block_norm b = norm_args(like, p, saved[6], ctx->saved_data["activation"].toInt(), ctx->saved_data["eps"].toDouble());
+        row_array(x, "x", like, b.x, b.x_stride);
+        row_array(y, "y", like, b.y, b.y_stride);
+        row_array(gate, "gate", like, b.gate, b.gate_stride);
+        if (codes) {
+            b.y8 = static_cast<int8_t *>(saved[7].data_ptr());
+            b.y8_scale = static_cast<float *>(saved[8].data_ptr());
+            if (block) b.y = b.y8;  // says that there is a block; not read
+            if (saved.size() > 9) {
+                b.gate8 = static_cast<int8_t *>(saved[9].data_ptr());
+                b.gate8_scale = static_cast<float *>(saved[10].data_ptr());
+                b.gate = b.gate8;
+            }
+        }
+        igx_block_norm_grad g = {};
+        row_array(d_out, "d_out", like, g.d_out, g.d_out_stride);
+        row_array(d_next, "d_next", like, g.d_next, g.d_next_stride);
+        // autograd numbers the edges of the inputs that there are
+        const bool there[6] = {true, block, block, b.gate != nullptr, p.scale.defined(), behind};
+        auto wanted = [&](int i) {
+            int edge = 0;
+            for (int j = 0; j < i; j++) edge += there[j];
+            return there[i] && ctx->needs_input_grad(edge);
+        };
+        auto rows = [&](int i, void *&to) {
+            if (!wanted(i)) return;
+            result[i] = at::empty(like.sizes(), like.options());
+            to = result[i].data_ptr();
+        };
+        // without a norm behind, the gradient of x is that of out
+        if (d_next.defined()) rows(0, g.d_x);
+        else if (wanted(0)) result[0] = given_out;
+        rows(1, g.d_y);
+        rows(3, g.d_gate);
+        auto vector = [&](int i, float *&to) {
+            if (!wanted(i)) return;
+            result[i] = at::empty({like.size(-1)}, like.options().dtype(at::kFloat));
+            to = static_cast<float *>(result[i].data_ptr());
+        };
+        vector(2, g.d_weight);
+        vector(4, g.d_scale);
+        vector(5, g.d_next_weight);
+        Tensor ws;
+        if (g.d_weight || g.d_scale || g.d_next_weight) {
+            g.workspace_bytes = lib.norm_workspace(&b);
+            if (g.workspace_bytes < 0) check(g.workspace_bytes);
+            ws = at::empty({g.workspace_bytes}, like.options().dtype(at::kByte));
+            g.workspace = ws.data_ptr();
+        }
+        check(lib.norm_backward(&b, &g, stream_of(like)));
+        return result;
+    }
+};
+
+std::pair<Tensor, Tensor> block_norm(const Tensor &x, const OptTensor &y_, const OptTensor &weight_, const OptTensor &gate_,
+                                     const OptTensor &scale_, const OptTensor &next_weight_, const std::string &activation, double eps,
+                                     bool checkpoint)
+{
+    const int64_t act = activation == "silu" ? IGX_GATE_SILU : activation == "sigmoid" ? IGX_GATE_SIGMOID : activation == "none" ? IGX_GATE_NONE : -1;
+    TORCH_CHECK_VALUE(act >= 0, "activation must be one of 'none', 'sigmoid', 'silu', got '", activation, "'");
+    TORCH_CHECK_VALUE(x.dim() >= 1, "x must be a tensor of at least one dimension");
+    const Tensor y = given(y_), weight = given(weight_), gate = given(gate_), scale = given(scale_), next_weight = given(next_weight_);
+    if (!differentiated({&x, &y, &weight, &gate, &scale, &next_weight}))
+        return run_norm(x, y, gate, {weight, scale, next_weight}, act, eps, {}, {});
+    if (x.is_cuda()) refuse_foreign_accumulators({&x, &y, &weight, &gate, &scale, &next_weight}, x);
+    const variable_list v = BlockNorm::apply(x, maybe(y), maybe(weight), maybe(gate), maybe(scale), maybe(next_weight), act, eps, checkpoint);
+    return {y.defined() ? v[0] : Tensor(), next_weight.defined() ? v.back() : Tensor()};
+}
+
+// ---- 8-bit checkpoints ----------------------------------------------------------------------------------------------
+
+std::pair<Tensor, Tensor> pack8(const Tensor &x)
+{
+    TORCH_CHECK_VALUE(x.dim() >= 1, "x must be a tensor of at least one dimension");
+    const at::NoGradGuard no_grad;
+    const int e = element(x, "x");
+    const void *p = nullptr;
+    int64_t stride = 0;
+    row_array(x, "x", x, p, stride);
+    c10::DeviceGuard guard(x.device());
+    const Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
+    const Tensor scales = at::empty(scales_shape(x), x.options().dtype(at::kFloat));
+    check(lib.pack8(p, e, rows_of(x), x.size(-1), stride, static_cast<int8_t *>(codes.data_ptr()),
+                    static_cast<float *>(scales.data_ptr()), stream_of(x)));
+    return {codes, scales};
+}
+
+Tensor unpack8(const Tensor &codes, const Tensor &scales, const py::object &dtype)
+{
+    TORCH_CHECK_VALUE(codes.dim() >= 1, "codes must be a tensor of at least one dimension");
+    TORCH_CHECK_VALUE(codes.is_cuda(), "libigx works on device tensors only (codes is a ", codes.device(), " tensor)");
+    TORCH_CHECK_TYPE(THPDtype_Check(dtype.ptr()), "dtype must be a torch.dtype");
+    c10::DeviceGuard guard(codes.device());
+    const Tensor out = at::empty(codes.sizes(), codes.options().dtype(reinterpret_cast<THPDtype *>(dtype.ptr())->scalar_type));
+    const int e = element(out, "dtype");
+    const auto *q = packed<int8_t>(codes, "codes", codes.sizes(), at::kChar, codes);
+    const auto *s = packed<float>(scales, "scales", scales_shape(codes), at::kFloat, codes);
+    check(lib.unpack8(q, s, e, rows_of(codes), codes.size(-1), out.data_ptr(), stream_of(codes)));
+    return out;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_sequence, m)
+{
+    m.doc() = "Differentiable forms of the sequence operators; isaacgym_amd.sequence is their documented interface.";
+    m.def("bind", [](const py::dict &addresses, const py::object &error) {
+        auto take = [&](const char *name, auto &fn) {
+            fn = reinterpret_cast<std::decay_t<decltype(fn)>>(addresses[name].cast<uintptr_t>());
+        };
+        take("igx_last_error_string", lib.last_error);
+        take("igx_linear_recurrence_workspace", lib.recurrence_workspace);
+        take("igx_linear_recurrence", lib.recurrence);
+        take("igx_linear_recurrence_backward", lib.recurrence_backward);
+        take("igx_block_norm_workspace", lib.norm_workspace);
+        take("igx_block_norm_forward", lib.norm);
+        take("igx_block_norm_backward", lib.norm_backward);
+        take("igx_pack8", lib.pack8);
+        take("igx_unpack8", lib.unpack8);
+        // isaacgym_amd._lib.IgxError(code, text); never released, so that no order of teardown matters
+        static py::object *error_class = nullptr;
+        if (error_class) return;
+        error_class = new py::object(error);
+        py::register_exception_translator([](std::exception_ptr p) {
+            try {
+                if (p) std::rethrow_exception(p);
+            } catch (const IgxFailure &e) {
+                const py::object value = (*error_class)(e.code, std::string(e.what()));
+                PyErr_SetObject(error_class->ptr(), value.ptr());
+            }
+        });
+    });
+    m.def("linear_recurrence", &linear_recurrence);
+    m.def("linear_recurrence_step", &linear_recurrence_step);
+    m.def("block_norm", &block_norm);
+    m.def("pack8", &pack8);
+    m.def("unpack8", &unpack8);
+}

@@ -1,6 +1,5 @@
 """What the sequence operators refuse, and the plain forms that the GPU tests compare with (no GPU needed)."""
 import ctypes as C
-import gc
 
 import pytest
 import torch
@@ -143,28 +142,6 @@ def test_host_tensors_wrong_types_and_shapes_are_refused():
         sequence.residual_norm(x, x, torch.ones(4), activation="tanh")
     with pytest.raises(RuntimeError):
         sequence.linear_recurrence(torch.zeros(3, 3, 4), x)  # does not broadcast
-
-
-def test_capture_guard_counts_live_eager_nodes(monkeypatch):
-    """The guard's bookkeeping on the CPU, with the kernel calls and the capture query stood in for."""
-    monkeypatch.setattr(ops, "linear_recurrence", lambda gate, inp, out, **kw: out.zero_())
-    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
-    capturing = [False]
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
-    a = torch.zeros(3, 2, 4, requires_grad=True)
-    b = torch.zeros(3, 2, 4)
-    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
-    first = sequence.linear_recurrence(a, b)
-    second = sequence.linear_recurrence(a * 1.0, b)  # not a leaf of the operator
-    capturing[0] = True
-    with pytest.raises(RuntimeError, match="eager autograd graph"):
-        sequence.linear_recurrence(a, b)
-    sequence.linear_recurrence(a.detach(), b)
-    sequence.linear_recurrence(torch.zeros(3, 2, 4, requires_grad=True), b)
-    del first
-    gc.collect()
-    sequence.linear_recurrence(a, b)
-    del second
 
 
 def test_plain_recurrence_is_the_loop_and_its_autograd():
