@@ -1058,7 +1058,8 @@ int igx_extract_positions_from_rigid_body_states(const float *states, int64_t ro
  * [T, N, D] (step, environment, channel).  Element types of the arrays marked
  * "elements"; every sum, state and statistic is kept in fp32.
  * Strides are counted in elements.  Unlike the task buffers these arrays need
- * only their element's own alignment.
+ * only their element's own alignment.  What a call writes must not overlap
+ * what it reads, unless a comment allows it.
  * ---------------------------------------------------------------------- */
 #define IGX_F32 0
 #define IGX_F16 1
@@ -1133,7 +1134,7 @@ typedef struct igx_block_norm {
     int32_t activation;  /* IGX_GATE_* */
     int64_t rows;        /* may be 0 */
     int64_t width;       /* 1 ... IGX_BLOCK_NORM_MAX_WIDTH */
-    float eps;
+    float eps;           /* >= 0 */
     const void *x;       /* elements [rows, width], x_stride elements (>= 0) from row to row; so are y and gate */
     int64_t x_stride;
     const void *y;       /* NULL: no block in front, out = x */

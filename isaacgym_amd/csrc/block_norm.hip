@@ -255,6 +255,7 @@ int check_parts(const igx_block_norm *b, const char *who)
     if (!b->y && !b->next_weight) return fail(IGX_E_NULL, "%s: neither y nor next_weight is given", who);
     if (!b->y && (b->gate || b->scale || b->gate8)) return fail(IGX_E_PARAM, "%s: gate and scale belong to y, which is NULL", who);
     if (b->y && !b->weight) return fail(IGX_E_NULL, "%s: weight is NULL", who);
+    if (!(b->eps >= 0.0f)) return fail(IGX_E_PARAM, "%s: eps %g is negative or NaN", who, (double)b->eps);
     if (b->x_stride < 0 || b->y_stride < 0 || b->gate_stride < 0) return fail(IGX_E_PARAM, "%s: a row stride is negative", who);
     if ((b->y8 != nullptr) != (b->y8_scale != nullptr) || (b->gate8 != nullptr) != (b->gate8_scale != nullptr))
         return fail(IGX_E_NULL, "%s: codes without their scales, or scales without their codes", who);

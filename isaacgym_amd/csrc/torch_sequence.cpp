@@ -11,6 +11,8 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <unordered_set>
+
 #include "../../include/igx.h"
 
 namespace {
@@ -90,20 +92,31 @@ bool differentiated(std::initializer_list<const Tensor *> tensors)
     return false;
 }
 
-// torch adds a captured gradient to a leaf on the stream where the leaf's accumulator was made: an eager graph that still
-// holds one would drag its stream into the capture, which ends the process.  Such a capture is refused.
-void refuse_foreign_accumulators(std::initializer_list<const Tensor *> tensors, const Tensor &like)
+// The nodes of a captured backward pass run on the streams their forward ran on; one that belongs to another stream - a
+// leaf's accumulator that an eager graph still holds, or an eager node further up - would drag that stream into the capture,
+// which ends the process.  Such a capture is refused.
+void refuse_foreign_nodes(std::initializer_list<const Tensor *> tensors, const Tensor &like)
 {
     c10::DeviceGuard guard(like.device());
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
     const c10::Stream now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(like.get_device()).unwrap();
+    std::vector<std::shared_ptr<torch::autograd::Node>> open;
+    std::unordered_set<const torch::autograd::Node *> seen;
+    auto reach = [&](std::shared_ptr<torch::autograd::Node> node) {
+        if (node && seen.insert(node.get()).second) open.push_back(std::move(node));
+    };
     for (const Tensor *t : tensors) {
-        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        const auto made = node ? node->stream() : std::nullopt;
-        TORCH_CHECK(!made || *made == now,
+        if (!t->defined() || !t->requires_grad()) continue;
+        reach(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    }
+    while (!open.empty()) {
+        const auto node = open.back();
+        open.pop_back();
+        const auto made = node->stream();
+        TORCH_CHECK(!made || made->device_index() != now.device_index() || *made == now,
                     "a tensor that requires grad is still part of an eager autograd graph: release that graph's outputs before "
                     "capturing one with the same tensor");
+        for (const auto &edge : node->next_edges()) reach(edge.function);
     }
 }
 
@@ -227,7 +240,7 @@ std::pair<Tensor, Tensor> linear_recurrence(const Tensor &gate_, const Tensor &i
     const Tensor gate = gate_.sizes() == inp.sizes() ? gate_ : gate_.expand(inp.sizes());
     const Tensor state = given(state_), reset = given(reset_);
     if (!differentiated({&gate, &inp, &state})) return run_recurrence(gate, inp, state, reset, reverse);
-    if (inp.is_cuda()) refuse_foreign_accumulators({&gate, &inp, &state}, inp);
+    if (inp.is_cuda()) refuse_foreign_nodes({&gate, &inp, &state}, inp);
     const variable_list v = LinearRecurrence::apply(gate, inp, maybe(state), maybe(reset), reverse);
     return {v[0], v[1]};
 }
@@ -463,7 +476,7 @@ std::pair<Tensor, Tensor> block_norm(const Tensor &x, const OptTensor &y_, const
     const Tensor y = given(y_), weight = given(weight_), gate = given(gate_), scale = given(scale_), next_weight = given(next_weight_);
     if (!differentiated({&x, &y, &weight, &gate, &scale, &next_weight}))
         return run_norm(x, y, gate, {weight, scale, next_weight}, act, eps, {}, {});
-    if (x.is_cuda()) refuse_foreign_accumulators({&x, &y, &weight, &gate, &scale, &next_weight}, x);
+    if (x.is_cuda()) refuse_foreign_nodes({&x, &y, &weight, &gate, &scale, &next_weight}, x);
     const variable_list v = BlockNorm::apply(x, maybe(y), maybe(weight), maybe(gate), maybe(scale), maybe(next_weight), act, eps, checkpoint);
     return {y.defined() ? v[0] : Tensor(), next_weight.defined() ? v.back() : Tensor()};
 }

@@ -742,6 +742,15 @@ def _scratch(size, device):
     return ws, ws.data_ptr(), size
 
 
+def _apart(written, read):
+    """No buffer that a call writes is one that it reads (or writes twice)."""
+    seen = {p for p in read if p}
+    for p in written:
+        if p and p in seen:
+            raise ValueError("a written tensor must not overlap another one of the call")
+        seen.add(p)
+
+
 def _rollout(t, name, shape, like, written=False):
     """(address, (stride over steps, stride over environments)) of a [T, N, D] tensor with adjacent channels, any
     strides otherwise; one that is written must not map two elements to one address."""
@@ -785,15 +794,14 @@ def _recurrence(gate, like, state, reset, reverse):
 def linear_recurrence(gate, inp, out, state=None, reset=None, last=None, reverse=False):
     """out[t] = gate[t] * (out before it) + inp[t] over [T, N, D] (igx_linear_recurrence).  gate, inp and out share a type
     and need adjacent channels (gate also one value for all channels of an environment); state and last are fp32 [N, D]
-    (last may be state), reset int64 [T, N].  out must not overlap an input."""
+    (last may be state), reset int64 [T, N].  What is written must not overlap the rest."""
     r, shape = _recurrence(gate, inp, state, reset, reverse)
     r.inp, r.inp_stride = _rollout(inp, "inp", shape, inp)
     if out is None:
         raise TypeError("out: expected a torch.Tensor, got None")
     r.out, r.out_stride = _rollout(out, "out", shape, inp, written=True)
-    if r.out is not None and r.out in (r.gate, r.inp) and out.numel():
-        raise ValueError("out must not overlap an input")
     r.last = _packed(last, "last", shape[1:], torch.float32, inp)
+    _apart((r.out, None if last is state else r.last), (r.gate, r.inp, r.state, r.reset))
     L = _lib.lib()
     ws, r.workspace, r.workspace_bytes = _scratch(L.igx_linear_recurrence_workspace(C.byref(r)), inp.device)
     _lib.check(_lib._launch(L.igx_linear_recurrence, inp.device, C.byref(r)))
@@ -812,6 +820,7 @@ def linear_recurrence_backward(gate, out, d_out=None, d_last=None, d_gate=None, 
     g.d_inp, g.d_inp_stride = _rollout(d_inp, "d_inp", shape, out, written=True)
     g.d_last = _packed(d_last, "d_last", shape[1:], torch.float32, out)
     g.d_state = _packed(d_state, "d_state", shape[1:], torch.float32, out)
+    _apart((g.d_gate, g.d_inp, g.d_state), (r.gate, r.out, r.state, r.reset, g.d_out, g.d_last))
     L = _lib.lib()
     ws, r.workspace, r.workspace_bytes = _scratch(L.igx_linear_recurrence_workspace(C.byref(r)), out.device)
     _lib.check(_lib._launch(L.igx_linear_recurrence_backward, out.device, C.byref(r), C.byref(g)))
@@ -879,6 +888,8 @@ def block_norm(x, y=None, weight=None, gate=None, scale=None, next_weight=None, 
     b.gate, b.gate_stride = _row_array(gate, "gate", shape, x)
     b.out = _packed(out, "out", shape, x.dtype, x)
     b.next = _packed(next, "next", shape, x.dtype, x)
+    _apart((b.out, b.next, b.y_inv_rms, b.y8, b.y8_scale, b.gate8, b.gate8_scale),
+           (b.x, b.y, b.gate, b.weight, b.scale, b.next_weight))
     _lib.check(_lib._launch(_lib.lib().igx_block_norm_forward, x.device, C.byref(b)))
 
 
@@ -905,6 +916,8 @@ def block_norm_backward(like, x=None, y=None, weight=None, gate=None, scale=None
     g.d_weight = _packed(d_weight, "d_weight", vector, f, like)
     g.d_scale = _packed(d_scale, "d_scale", vector, f, like)
     g.d_next_weight = _packed(d_next_weight, "d_next_weight", vector, f, like)
+    _apart((g.d_x, g.d_y, g.d_gate, g.d_weight, g.d_scale, g.d_next_weight),
+           (b.x, b.y, b.gate, b.weight, b.scale, b.next_weight, b.y_inv_rms, b.y8_scale, b.gate8_scale, g.d_out, g.d_next))
     L = _lib.lib()
     if d_weight is not None or d_scale is not None or d_next_weight is not None:
         ws, g.workspace, g.workspace_bytes = _scratch(L.igx_block_norm_workspace(C.byref(b)), like.device)

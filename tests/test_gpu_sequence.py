@@ -670,6 +670,133 @@ def test_capture_with_a_live_eager_graph_of_the_same_leaf_is_refused():
     S.close(out.view(16, 16), *S.block_norm(x.detach().view(16, 16), next_weight=w)["next"], "next")
 
 
+def test_capture_above_an_eager_graph_is_refused():
+    """The same where the leaf is not the operator's own input: an eager graph further up, or one that is alive beside it."""
+    x = torch.randn(8, 2, 16, device=DEV, requires_grad=True)
+    w = torch.ones(16, device=DEV)
+    alive = x * 2
+    for make in (lambda: alive, lambda: x * 3):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager autograd graph"):
+            with torch.cuda.graph(graph):
+                torch.zeros(1, device=DEV).add_(1)
+                sequence.rms_norm(make(), w)
+        del graph
+    with torch.no_grad():  # nothing to differentiate: captured
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = sequence.rms_norm(alive, w)
+    graph.replay()
+    assert torch.equal(out, sequence.rms_norm(alive.detach(), w))
+
+
+def test_captured_backward_accumulates_into_leaves():
+    """backward() inside the capture writes the leaves' grad at every replay."""
+    x, p, state, reset, heads = block_inputs(20, 3, 24, seed=90)
+    leaves = [t.requires_grad_(True) for t in [x, state] + list(p.values())]
+
+    def step():
+        for t in leaves:
+            t.grad = None
+        out, nxt, _ = block(x, p, state, reset)
+        torch.autograd.backward((out, nxt), heads)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for turn in range(3):
+        fresh = block_inputs(20, 3, 24, seed=91 + turn)
+        with torch.no_grad():
+            x.copy_(fresh[0])
+            state.copy_(fresh[2])
+            reset.copy_(fresh[3])
+            for k in p:
+                p[k].copy_(fresh[1][k])
+            for h, f in zip(heads, fresh[4]):
+                h.copy_(f)
+        graph.replay()
+        want = block_pass(*fresh)[3:]
+        for t, w in zip(leaves, want):
+            assert torch.equal(t.grad, w)
+
+
+def test_gradients_are_not_differentiated_again():
+    x = torch.randn(4, 16, device=DEV, requires_grad=True)
+    out = sequence.rms_norm(x, torch.ones(16, device=DEV))
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(out.sum(), x, create_graph=True)
+    r = torch.randn(4, 2, 16, device=DEV, requires_grad=True)
+    out, _ = sequence.linear_recurrence(r, r)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(out.sum(), r, create_graph=True)
+
+
+def test_inputs_changed_between_forward_and_backward_are_noticed():
+    r = torch.randn(4, 2, 16, device=DEV, requires_grad=True)
+    g = torch.rand(4, 2, 16, device=DEV)
+    out, _ = sequence.linear_recurrence(g, r)
+    g.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+# ---- the calls on the caller's buffers ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_calls_on_own_buffers_equal_the_differentiable_ones(checkpoint):
+    T, N, D = 200, 2, 70
+    gate, inp, state, reset, d_out, d_last = (t.to(DEV) for t in rollout(T, N, D, BF16, 95, resets=0.05))
+    leaves = [t.requires_grad_(True) for t in (gate, inp, state)]
+    out, last = sequence.linear_recurrence(*leaves[:2], state=state, reset=reset)
+    grads = torch.autograd.grad((out, last), leaves, (d_out, d_last))
+    mine, end = torch.empty_like(out), torch.empty_like(last)
+    own = [torch.empty_like(t) for t in leaves]
+    with torch.no_grad():
+        ops.linear_recurrence(gate, inp, mine, state=state, reset=reset, last=end)
+        ops.linear_recurrence_backward(gate, mine, d_out=d_out, d_last=d_last, d_gate=own[0], d_inp=own[1], d_state=own[2],
+                                       state=state, reset=reset)
+    for a, b in zip([out, last, *grads], [mine, end, *own]):
+        assert torch.equal(a, b)
+
+    t, do, dn = norm_inputs(60, 130, F32, 96)
+    dev = {k: v.to(DEV).requires_grad_(True) for k, v in t.items()}
+    outs = sequence.residual_norm(**dev, activation="sigmoid", checkpoint=checkpoint)
+    want = list(outs) + list(torch.autograd.grad(outs, list(dev.values()), (do.to(DEV), dn.to(DEV))))
+    rows = [torch.empty(60, 130, device=DEV) for _ in range(2)]
+    inv = torch.empty(2, 60, device=DEV)
+    codes = None
+    if checkpoint:
+        codes = tuple(torch.empty(*s, dtype=d, device=DEV) for _ in range(2) for s, d in (((60, 130), torch.int8), ((60, 3), F32)))
+    p = {k: dev[k].detach() for k in ("weight", "scale", "next_weight")}
+    args = dict(activation="sigmoid", inv_rms=inv, codes=codes, **p)
+    x, y, z = (dev[k].detach() for k in ("x", "y", "gate"))
+    ops.block_norm(x, y=y, gate=z, out=rows[0], next=rows[1], **args)
+    got = {k: torch.empty_like(v) for k, v in dev.items()}
+    ops.block_norm_backward(x, x=x, y=None if checkpoint else y, gate=None if checkpoint else z, d_out=do.to(DEV),
+                            d_next=dn.to(DEV), **{"d_" + k: v for k, v in got.items()}, **args)
+    for a, b in zip(want, rows + list(got.values())):
+        assert torch.equal(a, b)
+    if checkpoint:
+        for i, v in ((0, y), (2, z)):
+            q, s = sequence.pack8(v)
+            assert torch.equal(q, codes[i]) and torch.equal(s, codes[i + 1])
+            mine = [torch.empty_like(q), torch.empty_like(s), torch.empty_like(v)]
+            ops.pack8(v, mine[0], mine[1])
+            ops.unpack8(mine[0], mine[1], mine[2])
+            assert torch.equal(mine[0], q) and torch.equal(mine[1], s) and torch.equal(mine[2], sequence.unpack8(q, s))
+    with pytest.raises(ValueError, match="overlap"):
+        ops.block_norm(x, y=y, out=x, next=rows[1], **args)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.linear_recurrence_backward(gate.detach(), out.detach(), d_out=d_out, d_inp=d_out)
+
+
 # ---- as they are used: a policy on an environment's rollout ------------------------------------------------------------
 
 def test_policy_block_on_a_task_rollout():

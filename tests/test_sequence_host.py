@@ -51,7 +51,7 @@ def test_recurrence_null_structs_and_nothing_to_do():
     (dict(dtype=9), _abi.IGX_E_PARAM), (dict(rows=-1), _abi.IGX_E_SIZE), (dict(width=0), _abi.IGX_E_SIZE),
     (dict(width=8193), _abi.IGX_E_SIZE), (dict(activation=3), _abi.IGX_E_PARAM), (dict(y=None, next_weight=None), _abi.IGX_E_NULL),
     (dict(y=None, weight=None, gate=FAKE), _abi.IGX_E_PARAM), (dict(weight=None), _abi.IGX_E_NULL),
-    (dict(x_stride=-8), _abi.IGX_E_PARAM), (dict(y8=FAKE), _abi.IGX_E_NULL), (dict(x=None), _abi.IGX_E_NULL),
+    (dict(x_stride=-8), _abi.IGX_E_PARAM), (dict(eps=-1e-5), _abi.IGX_E_PARAM), (dict(eps=float("nan")), _abi.IGX_E_PARAM), (dict(y8=FAKE), _abi.IGX_E_NULL), (dict(x=None), _abi.IGX_E_NULL),
     (dict(gate=FAKE, gate_stride=8, y8=FAKE, y8_scale=FAKE), _abi.IGX_E_PARAM)])
 def test_block_norm_refusals(change, code):
     L = _lib.lib()
