@@ -53,7 +53,7 @@ __device__ __forceinline__ void checkpoint_row(const float (&f)[K][V], const int
 template <typename T, int LANES, bool POST, bool NEXT, bool STREAM>
 __global__ __launch_bounds__(block_of(LANES)) void block_norm_kernel(NormArgs a)
 {
-    using Row = RowLanes<T, LANES>;
+    using Row = RowLanes<T, LANES, !POST>;
     constexpr int V = Row::V, K = Row::K;
     __shared__ float slots[32];
     const Row rl;
@@ -159,7 +159,7 @@ template <typename T, int LANES> void launch_lanes(const NormArgs &a, bool strea
 
 template <typename T> void launch_type(const NormArgs &a, bool stream_past, int64_t blocks, hipStream_t s)
 {
-    const int lanes = lanes_for(a.width);
+    const int lanes = lanes_for(a.width, sizeof(T) == 4 ? IGX_F32 : IGX_F16, !a.y);
     const dim3 grid((unsigned)blocks), block(lanes > 64 ? lanes : kNormBlock);
     if (lanes == 8) launch_lanes<T, 8>(a, stream_past, grid, block, s);
     else if (lanes == 16) launch_lanes<T, 16>(a, stream_past, grid, block, s);
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(SumArgs a)
     const float *p = next ? a.next : a.block;
     float v = 0.0f;
     if (c < a.width) {
-#pragma unroll 4
+#pragma unroll 16
         for (int64_t b = wave; b < a.blocks; b += 16) v += p[b * a.width + c];
     }
     part[wave][lane] = v;
@@ -221,9 +221,9 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(SumArgs a)
 // of the card idle at the end (backward of 2^20 x 256 bf16: 871 us with the 12 waves a CU holds, 1 046 with 16).  Without a
 // block (waves 0) a lane keeps only the norm's weight, and a workgroup for every group of rows is faster: 2^20 x 256 fp32
 // 338 us, 398 walking.
-int64_t blocks_for(int64_t rows, int64_t width, int64_t waves_per_cu)
+int64_t blocks_for(int64_t rows, int64_t width, int dtype, int64_t waves_per_cu)
 {
-    const int lanes = lanes_for(width);
+    const int lanes = lanes_for(width, dtype, waves_per_cu == 0);
     const int64_t threads = lanes > 64 ? lanes : kNormBlock, rows_per_block = lanes > 64 ? 1 : kNormBlock / lanes;
     const int64_t need = ceil_div(rows, rows_per_block);
     const int64_t most = waves_per_cu ? 256 * waves_per_cu * 64 / threads : (int64_t)1 << 21;
@@ -309,7 +309,7 @@ extern "C" int igx_block_norm_forward(const igx_block_norm *b, igx_stream_t stre
     igx::NormArgs a;
     igx::base_args(b, a);
     const int64_t arrays = 1 + (b->y != nullptr) * 2 + (b->gate != nullptr) + (b->next_weight != nullptr);
-    igx::launch_block_norm(a, b->dtype, igx::beyond_cache(b, arrays), igx::blocks_for(b->rows, b->width, b->y ? igx::kForwardWaves : 0),
+    igx::launch_block_norm(a, b->dtype, igx::beyond_cache(b, arrays), igx::blocks_for(b->rows, b->width, b->dtype, b->y ? igx::kForwardWaves : 0),
                            static_cast<hipStream_t>(stream));
     return igx::launch_status(__func__);
 }
@@ -318,7 +318,7 @@ extern "C" int64_t igx_block_norm_workspace(const igx_block_norm *b)
 {
     const int rc = igx::check(b, __func__);
     if (rc) return rc;
-    return 2 * igx::blocks_for(b->rows, b->width, igx::kBackwardWaves) * b->width * (int64_t)sizeof(float);
+    return 2 * igx::blocks_for(b->rows, b->width, b->dtype, igx::kBackwardWaves) * b->width * (int64_t)sizeof(float);
 }
 
 extern "C" int igx_block_norm_backward(const igx_block_norm *b, const igx_block_norm_grad *g, igx_stream_t stream)
@@ -336,7 +336,7 @@ extern "C" int igx_block_norm_backward(const igx_block_norm *b, const igx_block_
     const bool sum_block = g->d_weight || g->d_scale, sum_next = g->d_next_weight != nullptr;
     const int wanted = sum_block + sum_next;
     if (wanted == 0 && !g->d_x && !g->d_y && !g->d_gate) return IGX_OK;
-    const int64_t blocks = igx::blocks_for(b->rows, b->width, igx::kBackwardWaves);
+    const int64_t blocks = igx::blocks_for(b->rows, b->width, b->dtype, igx::kBackwardWaves);
     if (b->rows > 0) {
         if (b->next_weight && (b->y || !b->y8)) IGX_REQUIRE_PTR(b->x, "x");
         if (b->y) IGX_REQUIRE_PTR(b->y_inv_rms, "y_inv_rms");

@@ -43,10 +43,10 @@ template <typename T, int V, bool STREAM> struct Saved<T, V, true, STREAM> {
 template <typename T, int LANES, bool POST, bool NEXT, bool CODES, bool STREAM>
 __global__ __launch_bounds__(block_of(LANES)) void block_norm_backward_kernel(NormArgs a)
 {
-    using Row = RowLanes<T, LANES>;
+    using Row = RowLanes<T, LANES, false>;
     constexpr int V = Row::V, K = Row::K;
     __shared__ float slots[32];
-    __shared__ float joined[LANES > 0 ? kNormBlock * kColumns : 1];
+    __shared__ float joined[LANES > 0 ? kNormBlock * Row::V : 1];
     const Row rl;
     int turn = 0;
     int col[K], left[K];
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(block_of(LANES)) void block_norm_backward_kernel(No
                 for (int i = 0; i < V; i++)
                     if (i < left[k]) to[col[k] + i] = s[k][i];
         } else {
-            constexpr int kSpan = LANES * kColumns;
+            constexpr int kSpan = LANES * V;
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < K; k++)
@@ -237,7 +237,7 @@ template <typename T, int LANES> void launch_lanes(const NormArgs &a, bool strea
 
 template <typename T> void launch_type(const NormArgs &a, bool stream_past, int64_t blocks, hipStream_t s)
 {
-    const int lanes = lanes_for(a.width);
+    const int lanes = lanes_for(a.width, sizeof(T) == 4 ? IGX_F32 : IGX_F16, false);
     const dim3 grid((unsigned)blocks), block(lanes > 64 ? lanes : kNormBlock);
     if (lanes == 8) launch_lanes<T, 8>(a, stream_past, grid, block, s);
     else if (lanes == 16) launch_lanes<T, 16>(a, stream_past, grid, block, s);

@@ -7,7 +7,11 @@
 namespace igx {
 
 constexpr int kNormBlock = 256;   // of the kernels whose row fits one wave
-constexpr int kColumns = 8;   // of a lane
+
+// 16-byte vectors of a row in a lane.  One, which leaves registers for enough waves (16 411 x 211 fp32 forward and backward: 38 us,
+// 41 with two) - but two where the forward kernel has a single array to read and its norm's weight to hold (2^20 x 64 fp32: 84 us,
+// 94 with one), and where 1024 lanes need them for the widest rows.
+constexpr int vectors_of(bool alone, bool largest, int vec) { return alone || (largest && vec == 4) ? 2 : 1; }
 
 struct NormArgs {
     const char *x, *y, *gate, *d_out, *d_next;
@@ -61,9 +65,9 @@ __device__ __forceinline__ void activate_slope(float z, int act, float &f, float
 constexpr int kWorkgroup = 0, kLargest = -1;
 constexpr int block_of(int lanes) { return lanes > 0 ? kNormBlock : lanes == kWorkgroup ? 512 : 1024; }
 
-template <typename T, int LANES> struct RowLanes {
-    static constexpr int V = Elem<std::is_same<T, float>::value ? IGX_F32 : std::is_same<T, _Float16>::value ? IGX_F16 : IGX_BF16>::vec;
-    static constexpr int K = kColumns / V;
+template <typename T, int LANES, bool ALONE> struct RowLanes {
+    static constexpr int V = 16 / sizeof(T);
+    static constexpr int K = vectors_of(ALONE, LANES == kLargest, V);
     static constexpr bool kWide = LANES <= 0;
     int lane, lanes, rows_per_block, sub;
     __device__ __forceinline__ RowLanes()
@@ -153,10 +157,11 @@ void launch_block_norm(const NormArgs &a, int dtype, bool stream_past, int64_t b
 void launch_block_norm_backward(const NormArgs &a, int dtype, bool stream_past, int64_t blocks, hipStream_t s);
 
 // Lanes of a row: the fewest that hold its columns; above 64 a workgroup of that many.
-inline int lanes_for(int64_t width)
+inline int lanes_for(int64_t width, int dtype, bool alone)
 {
+    const int vec = 16 / element_size(dtype);
     int lanes = 8;
-    while (lanes * kColumns < width) lanes *= 2;
+    while (lanes < 1024 && lanes * vec * vectors_of(alone, false, vec) < width) lanes *= 2;
     return lanes;
 }
 

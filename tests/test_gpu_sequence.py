@@ -355,6 +355,25 @@ def test_residual_norm_strided_rows(dtype):
         check_norm(t, do, dn, place=place)
 
 
+def test_residual_norm_broadcast_rows_and_one_row():
+    """One gate row for all rows (stride 0): torch adds its full-size gradients up; a single row without other dimensions."""
+    t, do, dn = norm_inputs(40, 36, F32, 35)
+    row = t["gate"][:1].clone()
+    t["gate"] = row.expand(40, 36)
+    dev = {k: v.to(DEV).requires_grad_(True) for k, v in t.items() if k != "gate"}
+    leaf = row.to(DEV).requires_grad_(True)
+    outs = sequence.residual_norm(gate=leaf.expand(40, 36), **dev)
+    ref = S.block_norm(**t, d_out=do, d_next=dn)
+    S.close(outs[0], *ref["out"], "out")
+    grads = torch.autograd.grad(outs, [leaf] + list(dev.values()), (do.to(DEV), dn.to(DEV)))
+    value, bound = ref["d_gate"]
+    S.close(grads[0], value.sum(0, keepdim=True), (bound + 40 * S.U * value.abs()).sum(0, keepdim=True), "summed d_gate")
+    for k, got in zip(dev, grads[1:]):
+        S.close(got, *ref["d_" + k], "d_" + k)
+    one = sequence.rms_norm(dev["x"].detach()[3], dev["weight"].detach())
+    assert one.shape == (36,) and torch.equal(one, sequence.rms_norm(dev["x"].detach(), dev["weight"].detach())[3])
+
+
 def test_residual_norm_many_rows():
     """More rows than there are lane groups on the card: the groups walk, the column sums are joined."""
     t, do, dn = norm_inputs(40001, 24, F32, 24, spread=False)
