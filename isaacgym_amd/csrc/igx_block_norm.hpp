@@ -30,15 +30,15 @@ struct NormArgs {
 };
 
 // 1 / (1 + exp(-z)) from the hardware's exponential and reciprocal (1 ulp each); `rest` carries what the product z log2(e)
-// loses, so that the error does not grow with |z|
+// loses, so that the error does not grow with |z|.  Where the exponential leaves fp32 the result is 0 or 1 without it.
 __device__ __forceinline__ float sigmoid(float z)
 {
     const float log2e = 1.44269504f, ln2 = 0.693147181f, log2e_rest = 1.92596303e-8f;
     const float t = -z * log2e;
-    float rest = fmaf(-z, log2e, -t) - z * log2e_rest;
-    rest = fabsf(t) < 160.0f ? rest * ln2 : 0.0f;  // not inf - inf
-    const float e = __builtin_amdgcn_exp2f(t);
-    return __builtin_amdgcn_rcpf(1.0f + fmaf(e, rest, e));
+    const float rest = (fmaf(-z, log2e, -t) - z * log2e_rest) * ln2;
+    float e = __builtin_amdgcn_exp2f(t);
+    e = fabsf(t) < 126.0f ? fmaf(e, rest, e) : e;  // not inf - inf
+    return __builtin_amdgcn_rcpf(1.0f + e);
 }
 
 __device__ __forceinline__ float activate(float z, int act)

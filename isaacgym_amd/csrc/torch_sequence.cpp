@@ -281,6 +281,9 @@ Tensor linear_recurrence_step(const Tensor &gate_, const Tensor &inp, const Tens
     r.out = out.data_ptr();
     r.out_stride[1] = r.width;
     check(lib.recurrence(&r, stream_of(inp)));
+    // a graph that saved what was overwritten has to notice
+    torch::autograd::impl::bump_version(to);
+    if (out_) torch::autograd::impl::bump_version(out);
     return out;
 }
 
@@ -430,7 +433,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         row_array(d_out, "d_out", like, g.d_out, g.d_out_stride);
         row_array(d_next, "d_next", like, g.d_next, g.d_next_stride);
         // autograd numbers the edges of the inputs that there are
-        const bool there[6] = {true, block, block, b.gate != nullptr, p.scale.defined(), behind};
+        const bool there[6] = {true, block, block, codes ? saved.size() > 9 : gate.defined(), p.scale.defined(), behind};
         auto wanted = [&](int i) {
             int edge = 0;
             for (int j = 0; j < i; j++) edge += there[j];

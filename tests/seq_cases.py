@@ -103,7 +103,8 @@ def block_norm(x, y=None, weight=None, gate=None, scale=None, next_weight=None, 
     Roundings, as counts c of u relative to the magnitudes' sums: a row's sum of squares takes at most 7 serial additions
     in a lane, 6 over a wave's lanes and 16 over the waves, which the inverse root halves: with its own rounding, the
     quotient and the gate's exponential (about 4) no factor of a term is off by more than 32 u.  A second sum over the row
-    (the gradient's) adds as many again: 64 u.  Column sums add at most `rows` further terms one after the other."""
+    (the gradient's) adds as many again: 64 u.  Column sums add at most `rows` further terms one after the other.
+    The sigmoid is a hardware reciprocal, 0 in place of a subnormal result: off by less than 2^-126, and z times that."""
     dt = x.dtype
     c1, c2 = 32 * U, 96 * U
 
@@ -125,6 +126,9 @@ def block_norm(x, y=None, weight=None, gate=None, scale=None, next_weight=None, 
     def inv(v):
         return 1 / (v.square().mean(1, keepdim=True) + eps).sqrt()
 
+    def flushed(z):
+        return 0.0 if z is None or activation == "none" else 2.0 ** -126 * (1 + z.abs())
+
     r = {}
     out, bound = X, torch.zeros_like(X)
     if Y is not None:
@@ -132,7 +136,7 @@ def block_norm(x, y=None, weight=None, gate=None, scale=None, next_weight=None, 
         f, _ = act(Z)
         branch = S * f * Y * iy * W
         out = X + branch
-        bound = c1 * branch.abs() + U * out.abs()
+        bound = c1 * branch.abs() + (S * Y * iy * W).abs() * flushed(Z) + U * out.abs()
         r["out"] = (out, bound + stored(out, dt))
     if W2 is not None:
         io = inv(out)
@@ -157,7 +161,7 @@ def block_norm(x, y=None, weight=None, gate=None, scale=None, next_weight=None, 
         unit = Y * iy
         branch = S * f * unit * W
         out = X + branch
-        bound = c1 * branch.abs() + U * out.abs()
+        bound = c1 * branch.abs() + (S * unit * W).abs() * flushed(Z) + U * out.abs()
     e_d = torch.zeros_like(X)
     d = GO
     if W2 is not None:
@@ -177,11 +181,13 @@ def block_norm(x, y=None, weight=None, gate=None, scale=None, next_weight=None, 
     dg = d * S * normed * slope
     # the slope is p + z p (1 - p): 1 - p is off by u, not by u of itself
     e_slope = (4 * U * (1 + (Z.abs() if Z is not None else 0.0))) if gate is not None and activation != "none" else 0.0
+    e_slope = e_slope + flushed(Z)
     e_dg = (S * normed).abs() * (slope.abs() * e_d + d.abs() * e_slope) + c1 * dg.abs()
     r["d_gate"] = (dg, e_dg + stored(dg, dt))
-    r["d_scale"] = _column(d * f * normed, (f * normed).abs() * e_d + c1 * (d * f * normed).abs(), rows)
+    r["d_scale"] = _column(d * f * normed, (f * normed).abs() * e_d + c1 * (d * f * normed).abs() +
+                           (d * normed).abs() * flushed(Z), rows)
     top = d * S * f
-    e_top = (S * f).abs() * e_d + c1 * top.abs()
+    e_top = (S * f).abs() * e_d + c1 * top.abs() + (d * S).abs() * flushed(Z)
     r["d_weight"] = _column(top * unit, unit.abs() * e_top + c1 * (top * unit).abs(), rows)
     t, e_t = top * W, e_top * W.abs()
     dot = (t * unit).mean(1, keepdim=True)

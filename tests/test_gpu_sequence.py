@@ -277,6 +277,26 @@ def test_recurrence_gradient_against_differences():
         assert abs(float((g * v).sum()) - diff) <= 1e-5 * float((g.abs() * v.abs()).sum() + v.abs().sum())
 
 
+@pytest.mark.parametrize("D", [0, 1, 3])
+@pytest.mark.parametrize("dones", [torch.int64, torch.float32, torch.bool])
+def test_discount_values(D, dones):
+    """The agent's loop in 64 bits: two roundings of the difference, two of the gate, one of the sum, every step."""
+    from isaacgym_amd.utils.rlgames_utils import discount_values
+    T, N = 33, 70
+    g = gen(15)
+    shape = (T, N, D) if D else (T, N)
+    rew, val, nxt = (torch.randn(*shape, generator=g) for _ in range(3))
+    done = (torch.rand(T, N, generator=g) < 0.1)
+    adv = discount_values(done.to(dones).to(DEV), val.to(DEV), rew.to(DEV), nxt.to(DEV), 0.99, 0.95)
+    assert adv.shape == shape and not adv.requires_grad
+    a, m = torch.zeros(shape[1:], dtype=torch.float64), torch.zeros(shape[1:], dtype=torch.float64)
+    for t in range(T - 1, -1, -1):
+        live = 0.99 * 0.95 * (~done[t]).double().view(N, *([1] if D else []))
+        a = rew[t].double() + 0.99 * nxt[t].double() - val[t].double() + live * a
+        m = rew[t].double().abs() + nxt[t].double().abs() + val[t].double().abs() + live * m
+        assert ((adv[t].double().cpu() - a).abs() <= 5 * (T - t) * S.U * m).all()
+
+
 # ---- norms ----------------------------------------------------------------------------------------------------------
 
 def norm_inputs(R, D, dtype, seed, gate=True, scale=True, next=True, spread=True):
@@ -353,6 +373,24 @@ def test_residual_norm_strided_rows(dtype):
     for R, D in ((20, 60), (11, 211), (4, 1030)):
         t, do, dn = norm_inputs(R, D, dtype, 23)
         check_norm(t, do, dn, place=place)
+
+
+@pytest.mark.parametrize("activation", ["silu", "sigmoid", "none"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_residual_norm_extreme_gates(dtype, activation):
+    """Gates up to the type's ends: where exp(-z) leaves fp32 the gate is shut or open, not NaN."""
+    z = [0.0, -0.0, 1e-30, 8.0, 17.0, 40.0, 87.0, 88.5, 89.0, 100.0, 104.0, 110.0, 111.5, 128.0, 200.0, 1e4, torch.finfo(dtype).max]
+    z = torch.tensor(z + [-v for v in z])
+    t, do, dn = norm_inputs(3, z.numel(), dtype, 36, spread=False)
+    if activation == "none":
+        z = z.clamp(-100, 100)  # the gate is then a factor of out, whose square has to stay in fp32
+    t["gate"] = z.expand(3, -1).to(dtype).contiguous()
+    if activation == "silu":
+        big = t["gate"] > 1e3
+        t["gate"][big] = 1e3
+    outs, grads = check_norm(t, do, dn, activation=activation)
+    for v in list(outs) + list(grads.values()):
+        assert torch.isfinite(v).all()
 
 
 def test_residual_norm_broadcast_rows_and_one_row():
@@ -445,8 +483,16 @@ def test_norms_empty():
         gx, gw = torch.autograd.grad(out, (x, w), torch.empty_like(out))
         assert gx.shape == x.shape and (gw == 0).all()
         out, nxt = sequence.residual_norm(x, x, w, gate=x, scale=w, next_weight=w)
-        gw, = torch.autograd.grad((out, nxt), w, (torch.empty_like(out), torch.empty_like(nxt)))
-        assert (gw == 0).all()
+        gx, gw = torch.autograd.grad((out, nxt), (x, w), (torch.empty_like(out), torch.empty_like(nxt)))
+        assert gx.shape == x.shape and (gw == 0).all()
+        for checkpoint in (False, True):  # each input alone: none takes another one's place
+            for i in range(6):
+                leaves = [torch.empty(R, 30, device=DEV) for _ in range(3)] + [torch.ones(30, device=DEV) for _ in range(3)]
+                leaves[i].requires_grad_(True)
+                outs = sequence.residual_norm(leaves[0], leaves[1], leaves[3], gate=leaves[2], scale=leaves[4],
+                                              next_weight=leaves[5], checkpoint=checkpoint)
+                got, = torch.autograd.grad(outs, leaves[i], [torch.empty_like(o) for o in outs])
+                assert got.shape == leaves[i].shape and (got == 0).all()
 
 
 def test_norms_a_row_does_not_touch_its_neighbours():
@@ -762,6 +808,15 @@ def test_inputs_changed_between_forward_and_backward_are_noticed():
     g = torch.rand(4, 2, 16, device=DEV)
     out, _ = sequence.linear_recurrence(g, r)
     g.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_a_step_in_place_is_noticed_by_graphs_that_saved_the_state():
+    r = torch.randn(4, 2, 16, device=DEV, requires_grad=True)
+    state = torch.randn(2, 16, device=DEV)
+    out, _ = sequence.linear_recurrence(torch.sigmoid(r), r, state=state)
+    sequence.linear_recurrence_step(r.detach()[0], r.detach()[1], state)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
 
