@@ -83,8 +83,9 @@ template <int V, int FL> struct LaneFlags {
 // Steps whose loads a lane has in flight, by the groups that share a workgroup's channels (measured, forward + backward):
 // with a lane for all steps 1, since thousands of waves are in flight and fewer rows [N, D] open at a time suit HBM better
 // (32 x 65 536 x 64 bf16: 406 us with 1, 415 with 2, 431 with 4, 475 with 8); with four groups 2 (32 x 4 096 x 64 fp32:
-// 49 us, 51 with 4, 55 with 8); with sixteen, where waves are few, 8 (2 048 x 16 x 1 024 bf16: 172 us, 237 with 4).
-constexpr int steps_of(int seg) { return seg == 1 ? 1 : seg == 4 ? 2 : 8; }
+// 49 us, 51 with 4, 55 with 8); with sixteen, where waves are few, 8 (2 048 x 16 x 1 024 bf16: 172 us, 237 with 4); with
+// sixty-four, whose 16 waves leave 128 registers each, 4.
+constexpr int steps_of(int seg) { return seg == 1 ? 1 : seg == 4 ? 2 : seg == 16 ? 8 : 4; }
 
 template <int V, int FL> struct StepFlags {
     using Places = LaneFlags<V, FL>;
@@ -119,10 +120,14 @@ template <typename T, int V, bool STREAM> __device__ __forceinline__ void load_g
 
 // The map of some steps, h -> A h + B.  Behind an episode's start nothing of h is left, not even an inf or NaN times 0:
 // such a map has kDropped for A, a NaN that arithmetic does not produce.  And where nothing is carried in, the result is
-// B whatever A has grown to.
+// B, also where A has left fp32's range.
 constexpr uint32_t kDropped = 0x7fc0d209u;
 __device__ __forceinline__ bool dropped(float A) { return __float_as_uint(A) == kDropped; }
 __device__ __forceinline__ float through(float A, float B, float h) { return h == 0.0f || dropped(A) ? B : fmaf(A, h, B); }
+__device__ __forceinline__ float as_factor(float A, bool none)
+{
+    return __uint_as_float(none ? kDropped : A != A ? 0x7fc00000u : __float_as_uint(A));
+}
 
 // K consecutive steps of a lane's channels in registers.  `count` of them exist, the others repeat the last one and are
 // neutral; whole steps of a full group cost no test (CHECK false).
@@ -131,35 +136,43 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STRE
     StepFlags<V, FL> f[K];
     int count;
 
+    // The addresses run along by a stride: a product of 64 bits for every load would cost more than the recurrence.  Steps
+    // that do not exist repeat the last one.
     __device__ __forceinline__ void load(const RecArgs &a, const LaneFlags<V, FL> &lf, const char *gate, const char *add,
                                          const char *before, int64_t t0, int64_t t1)
     {
         count = CHECK ? (t1 - t0 < K ? (int)(t1 - t0) : K) : K;
-        const int64_t most = t1 - 1;
+        const int64_t t = CHECK && t0 >= t1 ? t1 - 1 : t0;
+        gate += t * a.gate_t;
+        int64_t flag = t * a.reset_t;
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const int64_t t = CHECK && t0 + k > most ? most : t0 + k;
-            load_gate<T, V, STREAM>(g[k], gate + t * a.gate_t, a.splat);
-            f[k].load(lf, t * a.reset_t);
+            load_gate<T, V, STREAM>(g[k], gate, a.splat);
+            f[k].load(lf, flag);
+            gate += on(k) ? a.gate_t : 0;
+            flag += on(k) ? a.reset_t : 0;
         }
         if (!BACKWARD || add) {
+            add += t * a.add_t;
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                const int64_t t = CHECK && t0 + k > most ? most : t0 + k;
-                x[k] = load_raw<T, V, STREAM>(add + t * a.add_t);
+                x[k] = load_raw<T, V, STREAM>(add);
+                add += on(k) ? a.add_t : 0;
             }
         } else {
 #pragma unroll
             for (int k = 0; k < K; k++) x[k] = {};
         }
         if (BACKWARD && before) {
+            before += t * a.before_t;
 #pragma unroll
             for (int k = 0; k < K; k++) {  // before the first step stands `state`, which is not in out
-                const int64_t t = CHECK && t0 + k > most ? most : t0 + k;
-                if (t < a.T - 1) hb[k] = load_raw<T, V, STREAM>(before + t * a.before_t);
+                if (t + k < a.T - 1) hb[k] = load_raw<T, V, STREAM>(before);
+                before += on(k) ? a.before_t : 0;
             }
         }
     }
+    __device__ __forceinline__ bool on(int k) const { return !CHECK || k + 1 < count; }  // is there a step behind step k?
     __device__ __forceinline__ bool there(int k) const { return !CHECK || k < count; }
 
     // the steps as one map (A, B) after those already in it; `starts`: channels in which an episode began
@@ -183,17 +196,18 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STRE
     __device__ __forceinline__ void walk(const RecArgs &a, const Lane &l, bool store, char *to, char *d_gate, int64_t t0,
                                          float (&h)[V]) const
     {
+        if (to) to += t0 * a.to_t;
+        if (BACKWARD && d_gate) d_gate += t0 * a.d_gate_t;
 #pragma unroll
         for (int k = 0; k < K; k++) {
             if (CHECK && !there(k)) break;
-            const int64_t t = t0 + k;
             if constexpr (!BACKWARD) {
 #pragma unroll
                 for (int i = 0; i < V; i++) {
                     const float x1 = raw_at(x[k], i);
                     h[i] = f[k].begins(i) ? x1 : fmaf(raw_at(g[k], i), h[i], x1);
                 }
-                if (store) store_from<T, V, true>(to + t * a.to_t, h, l.skip);
+                if (store) store_from<T, V, true>(to, h, l.skip);
             } else {
                 float d[V], dg[V];
 #pragma unroll
@@ -203,17 +217,19 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STRE
                     h[i] = f[k].begins(i) ? 0.0f : raw_at(g[k], i) * d[i];
                 }
                 if (d_gate) {
-                    if (t < a.T - 1) {
+                    if (t0 + k < a.T - 1) {
 #pragma unroll
                         for (int i = 0; i < V; i++) dg[i] = f[k].begins(i) ? 0.0f : d[i] * raw_at(hb[k], i);
                     } else if (a.state) {
 #pragma unroll
                         for (int i = 0; i < V; i++) dg[i] = f[k].begins(i) ? 0.0f : d[i] * a.state[l.channel + i];
                     }
-                    if (store) store_from<T, V, true>(d_gate + t * a.d_gate_t, dg, l.skip);
+                    if (store) store_from<T, V, true>(d_gate, dg, l.skip);
+                    d_gate += a.d_gate_t;
                 }
-                if (to && store) store_from<T, V, true>(to + t * a.to_t, d, l.skip);
+                if (to && store) store_from<T, V, true>(to, d, l.skip);
             }
+            if (to) to += a.to_t;
         }
     }
 };
@@ -228,7 +244,7 @@ template <int V> __device__ __forceinline__ void identity(float (&A)[V], float (
 template <int V> __device__ __forceinline__ void mark(float (&A)[V], const bool (&starts)[V])
 {
 #pragma unroll
-    for (int i = 0; i < V; i++) A[i] = __uint_as_float(starts[i] ? kDropped : A[i] != A[i] ? 0x7fc00000u : __float_as_uint(A[i]));
+    for (int i = 0; i < V; i++) A[i] = as_factor(A[i], starts[i]);
 }
 
 // where a lane's channels lie in the arrays
@@ -315,10 +331,8 @@ template <int V> __device__ __forceinline__ void compose(float (&A1)[V], float (
 {
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const bool none = dropped(A[i]) || dropped(A1[i]);
-        const float product = A[i] * A1[i];
         B1[i] = through(A[i], B[i], B1[i]);
-        A1[i] = __uint_as_float(none ? kDropped : product != product ? 0x7fc00000u : __float_as_uint(product));
+        A1[i] = as_factor(A[i] * A1[i], dropped(A[i]) || dropped(A1[i]));
     }
 }
 
@@ -329,30 +343,101 @@ template <int V> __device__ __forceinline__ void load_span(const RecArgs &a, int
     else widen(load_raw<float, V>(p), f);
 }
 
-// Time split: SEG groups of 256 / SEG lanes take steps_of(SEG) steps each of the same channels; blockIdx.y is the span.
+// SEG groups of LANES lanes with the maps of consecutive parts of the time: groups of one wave scan theirs by exchanging
+// registers, the waves' totals go through LDS.
+template <int V, int LANES, int SEG> struct Chain {
+    static constexpr int kInWave = 64 / LANES, kWaves = LANES * SEG / 64;
+    Exchange<V, LANES> (*maps)[kWaves][2];  // [2]: two halves used in turn, so that one barrier a call is enough
+    int lane, in_wave, wave, turn;
+    __device__ __forceinline__ Chain(Exchange<V, LANES> (*lds)[kWaves][2])
+        : maps(lds), lane(threadIdx.x % LANES), in_wave(threadIdx.x % 64 / LANES), wave(threadIdx.x / 64), turn(0)
+    {
+    }
+    // (A, B) becomes the map of this group's part behind those of the groups in front of it in the wave
+    __device__ __forceinline__ void scan_wave(float (&A)[V], float (&B)[V]) const
+    {
+#pragma unroll
+        for (int d = 1; d < kInWave; d *= 2) {
+            float A1[V], B1[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                A1[i] = __shfl_up(A[i], d * LANES);
+                B1[i] = __shfl_up(B[i], d * LANES);
+            }
+            if (in_wave >= d) {
+                compose<V>(A1, B1, A, B);
+#pragma unroll
+                for (int i = 0; i < V; i++) A[i] = A1[i], B[i] = B1[i];
+            }
+        }
+    }
+    __device__ __forceinline__ void publish(const float (&A)[V], const float (&B)[V])
+    {
+        if (in_wave == kInWave - 1) {
+            maps[turn][wave][0].put(lane, A);
+            maps[turn][wave][1].put(lane, B);
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void total(int w, float (&A)[V], float (&B)[V]) const
+    {
+        maps[turn][w][0].get(lane, A);
+        maps[turn][w][1].get(lane, B);
+    }
+    // h goes through all parts; `from` is what reaches this group's
+    __device__ __forceinline__ void run(float (&A)[V], float (&B)[V], float (&h)[V], float (&from)[V])
+    {
+        scan_wave(A, B);
+        publish(A, B);
+#pragma unroll
+        for (int i = 0; i < V; i++) from[i] = 0.0f;
+#pragma unroll 2
+        for (int w = 0; w < kWaves; w++) {
+            float A2[V], B2[V];
+            total(w, A2, B2);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                from[i] = w == wave ? h[i] : from[i];
+                h[i] = through(A2[i], B2[i], h[i]);
+            }
+        }
+        if constexpr (kInWave > 1) {
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const float A1 = __shfl_up(A[i], LANES), B1 = __shfl_up(B[i], LANES);
+                from[i] = in_wave ? through(A1, B1, from[i]) : from[i];
+            }
+        }
+        turn ^= 1;
+    }
+};
+
+// Time split: SEG groups of lanes take steps_of(SEG) steps each of the same channels; blockIdx.y is the span.
+constexpr int lanes_of(int seg) { return seg == 4 ? 64 : 16; }
+
 template <typename T, int V, int FL, bool BACKWARD, int SEG>
-__global__ __launch_bounds__(kRecBlock) void recurrence_split_kernel(RecArgs a)
+__global__ __launch_bounds__(lanes_of(SEG) * SEG) void recurrence_split_kernel(RecArgs a)
 {
-    constexpr int LANES = kRecBlock / SEG;
-    __shared__ Exchange<V, LANES> maps[2][SEG][2];
-    const int lane = threadIdx.x % LANES, seg = threadIdx.x / LANES;
-    const uint32_t mine = blockIdx.x * LANES + lane, v = mine < a.vectors ? mine : a.vectors - 1;
+    constexpr int LANES = lanes_of(SEG), kSteps = steps_of(SEG);
+    using Links = Chain<V, LANES, SEG>;
+    __shared__ Exchange<V, LANES> maps[2][Links::kWaves][2];
+    Links chain(maps);
+    const int seg = threadIdx.x / LANES;
+    const uint32_t mine = blockIdx.x * LANES + chain.lane, v = mine < a.vectors ? mine : a.vectors - 1;
     const bool store = mine < a.vectors;  // the other lanes of the last workgroup repeat its last vector
     const Lane l = lane_of<V>(a, v);
     const LaneFlags<V, FL> lf(a, l);
     const Places<T> p(a, l);
     const int64_t first = (int64_t)blockIdx.y * a.span, t1 = first + a.span < a.T ? first + a.span : a.T;
-    constexpr int kSteps = steps_of(SEG);
     Steps<T, V, FL, kSteps, BACKWARD, true, false> s;
     s.load(a, lf, p.gate, p.add, p.before, first + seg * kSteps, t1);  // on its way while the spans are composed
-    float h[V];
+    float h[V], A[V], B[V], from[V];
+    bool starts[V];
     if (gridDim.y == 1) {
         load_start<V>(a.start, l, h);
     } else {  // each group composes its part of the spans before this one, then all go through the parts
         const int64_t spans = blockIdx.y, part = ceil_div(spans, SEG);
-        float A[V], B[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) A[i] = 1.0f, B[i] = 0.0f;
+        identity<V>(A, B, starts);
         const int64_t end = (seg + 1) * part < spans ? (seg + 1) * part : spans;
 #pragma unroll 2
         for (int64_t q = seg * part; q < end; q++) {
@@ -361,55 +446,31 @@ __global__ __launch_bounds__(kRecBlock) void recurrence_split_kernel(RecArgs a)
             load_span<V>(a, 2 + 2 * q, v, B2);
             compose<V>(A, B, A2, B2);
         }
-        maps[1][seg][0].put(lane, A);
-        maps[1][seg][1].put(lane, B);
         load_span<V>(a, 0, v, h);
-        __syncthreads();
-#pragma unroll 2
-        for (int q = 0; q < SEG; q++) {
-            float A2[V], B2[V];
-            maps[1][q][0].get(lane, A2);
-            maps[1][q][1].get(lane, B2);
-#pragma unroll
-            for (int i = 0; i < V; i++) h[i] = through(A2[i], B2[i], h[i]);
-        }
+        chain.run(A, B, h, from);
     }
-    int turn = 0;
-    for (int64_t t0 = first; t0 < t1; t0 += SEG * kSteps, turn ^= 1) {
+    for (int64_t t0 = first; t0 < t1; t0 += SEG * kSteps) {
         const int64_t ts = t0 + seg * kSteps, next = t0 + SEG * kSteps;
-        float A[V], B[V], from[V] = {};
-        bool starts[V];
         identity<V>(A, B, starts);
         s.reduce(A, B, starts);
         mark<V>(A, starts);
-        maps[turn][seg][0].put(lane, A);
-        maps[turn][seg][1].put(lane, B);
-        __syncthreads();
-#pragma unroll 2
-        for (int q = 0; q < SEG; q++) {
-            float A2[V], B2[V];
-            maps[turn][q][0].get(lane, A2);
-            maps[turn][q][1].get(lane, B2);
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                from[i] = q == seg ? h[i] : from[i];
-                h[i] = through(A2[i], B2[i], h[i]);
-            }
-        }
+        chain.run(A, B, h, from);
         s.walk(a, l, store, p.to, p.d_gate, ts, from);
         if (next < t1) s.load(a, lf, p.gate, p.add, p.before, next + seg * kSteps, t1);
     }
     if (store && seg == 0 && blockIdx.y == gridDim.y - 1) store_end<V>(a, l, h);
 }
 
-// The (A, B) of every span: SEG groups of lanes reduce consecutive parts of it, joined through LDS.
+// The (A, B) of every span: SEG groups of lanes reduce consecutive parts of it.
 template <typename T, int V, int FL, bool BACKWARD>
 __global__ __launch_bounds__(kRecBlock) void recurrence_spans_kernel(RecArgs a)
 {
-    constexpr int SEG = 16, LANES = kRecBlock / SEG;
-    __shared__ Exchange<V, LANES> maps[SEG][2];
-    const int lane = threadIdx.x % LANES, seg = threadIdx.x / LANES;
-    const uint32_t mine = blockIdx.x * LANES + lane, v = mine < a.vectors ? mine : a.vectors - 1;
+    constexpr int SEG = 16, LANES = kRecBlock / SEG, kSteps = 8;
+    using Links = Chain<V, LANES, SEG>;
+    __shared__ Exchange<V, LANES> maps[2][Links::kWaves][2];
+    Links chain(maps);
+    const int seg = threadIdx.x / LANES;
+    const uint32_t mine = blockIdx.x * LANES + chain.lane, v = mine < a.vectors ? mine : a.vectors - 1;
     const Lane l = lane_of<V>(a, v);
     const LaneFlags<V, FL> lf(a, l);
     const Places<T> p(a, l);
@@ -419,22 +480,20 @@ __global__ __launch_bounds__(kRecBlock) void recurrence_spans_kernel(RecArgs a)
     float A[V], B[V];
     bool starts[V];
     identity<V>(A, B, starts);
-    constexpr int kSteps = steps_of(16);
     for (int64_t t = from; t < to; t += kSteps) {
         Steps<T, V, FL, kSteps, BACKWARD, true, false> s;
         s.load(a, lf, p.gate, p.add, nullptr, t, to);
         s.reduce(A, B, starts);
     }
     mark<V>(A, starts);
-    maps[seg][0].put(lane, A);
-    maps[seg][1].put(lane, B);
-    __syncthreads();
+    chain.scan_wave(A, B);
+    chain.publish(A, B);
     if (seg != 0 || mine >= a.vectors) return;
-#pragma unroll 2
-    for (int q = 1; q < SEG; q++) {
+    chain.total(0, A, B);
+#pragma unroll
+    for (int w = 1; w < Links::kWaves; w++) {
         float A2[V], B2[V];
-        maps[q][0].get(lane, A2);
-        maps[q][1].get(lane, B2);
+        chain.total(w, A2, B2);
         compose<V>(A, B, A2, B2);
     }
     const int64_t at = (int64_t)a.vectors * V;
@@ -451,7 +510,7 @@ struct Plan {
     RecArgs a;
     int vec;    // channels per lane: the type's 16 bytes, or 4, or 1 where a run is shorter than that
     int flags;
-    int seg;    // groups of lanes that share a workgroup's channels; 1: a lane walks all steps
+    int seg;    // groups of lanes that share a workgroup's channels: 4, 16 or 64; 1: a lane walks all steps
     int64_t spans;
     int64_t workspace() const { return spans > 1 ? (1 + 2 * spans) * a.vectors * vec * (int64_t)sizeof(float) : 0; }
 };
@@ -465,9 +524,12 @@ template <typename T, int V, int FL, bool BACKWARD> void launch_as(const Plan &p
     if (p.seg == 1) {
         recurrence_kernel<T, V, FL, BACKWARD><<<dim3((unsigned)ceil_div(v, kRecBlock)), block, 0, s>>>(p.a);
     } else if (p.seg == 4) {
-        recurrence_split_kernel<T, V, FL, BACKWARD, 4><<<dim3((unsigned)ceil_div(v, kRecBlock / 4)), block, 0, s>>>(p.a);
+        recurrence_split_kernel<T, V, FL, BACKWARD, 4><<<dim3((unsigned)ceil_div(v, lanes_of(4))), block, 0, s>>>(p.a);
     } else {
-        const dim3 grid((unsigned)ceil_div(v, kRecBlock / 16), (unsigned)p.spans);
+        const dim3 grid((unsigned)ceil_div(v, lanes_of(16)), (unsigned)p.spans);
+        if constexpr (FL <= kOneFlag) {
+            if (p.seg == 64) return recurrence_split_kernel<T, V, FL, BACKWARD, 64><<<grid, dim3(lanes_of(64) * 64), 0, s>>>(p.a);
+        }
         recurrence_split_kernel<T, V, FL, BACKWARD, 16><<<grid, block, 0, s>>>(p.a);
     }
 }

@@ -9,12 +9,12 @@
 //
 // With fewer channels the time is split, for the recurrence is a composition of maps h -> A h + B that is associative:
 //   - within a workgroup SEG groups of lanes take a few consecutive steps each of the same channels, reduce them to
-//     (A, B) in registers, exchange those through LDS, and then walk their steps from the value that reaches them, so
-//     every element is still read and written once;
+//     (A, B) in registers, exchange those - between the groups of a wave in registers, between waves through LDS - and then
+//     walk their steps from the value that reaches them, so every element is still read and written once;
 //   - across workgroups a first kernel reduces every span of the time to its (A, B) in a workspace, and each workgroup of
 //     the second composes the spans before its own, while its first steps are on their way.  That reads gate and inp twice
 //     (the second time mostly from the caches), so it is done only where the channels alone leave CUs without work: 8 192
-//     steps of 512 channels in bf16 take 23 us forward and 23 us backward, bound by the latency of two launches and the
+//     steps of 512 channels in bf16 take 17 us forward and 20 us backward, bound by the latency of two launches and the
 //     exchange (a lane for every 8 channels needs 7 565 us).
 #include "igx_recurrence.hpp"
 
@@ -50,7 +50,9 @@ bool follows(const igx_recurrence *r, int64_t stride_n) { return r->envs == 1 ||
 // 64 fp32: 364 us, 452 in four groups).  With fewer, four groups share a workgroup's steps (32 x 4 096 x 64 fp32, 65 536
 // lanes: 49 us, 82 alone), below 16 384 lanes sixteen.  A sequence goes to several workgroups in spans only where the
 // channels fill fewer than 256 of them, one for each CU (1 024 x 64 x 256 fp32 fills 256: 118 us in one span, 153 in two,
-// for gate and inp are then read twice); 512 workgroups in all are enough.
+// for gate and inp are then read twice); 512 workgroups in all are enough.  Where they fill 256 and the sequence is long,
+// sixty-four groups keep a CU's waves busy (2 048 x 16 x 1 024 bf16: 137 us, 164 in sixteen; 1 024 x 64 x 256 fp32: 105, 139),
+// unless a lane needs more than one flag a step, which takes the registers (1 000 x 200 x 105 bf16: 234, 166 in sixteen).
 void split(Plan &p)
 {
     const int64_t vectors = p.a.vectors, T = p.a.T;
@@ -58,8 +60,12 @@ void split(Plan &p)
     p.a.span = T;
     p.seg = T <= steps_of(16) || vectors >= 131072 ? 1 : vectors >= 16384 ? 4 : 16;
     if (p.seg != 16) return;
-    const int64_t strips = ceil_div(vectors, kRecBlock / 16), tile = 16 * steps_of(16);
-    if (strips >= 256 || T <= tile) return;
+    const int64_t strips = ceil_div(vectors, lanes_of(16)), tile = 16 * steps_of(16);
+    if (strips >= 256) {
+        if (T >= 512 && p.flags <= kOneFlag) p.seg = 64;
+        return;
+    }
+    if (T <= tile) return;
     const int64_t want = ceil_div(512, strips), most = ceil_div(T, tile);
     const int64_t spans = want < most ? want : most;
     p.a.span = ceil_div(ceil_div(T, spans), tile) * tile;
@@ -90,6 +96,7 @@ void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, Plan &p)
         p.vec = a.run >= (uint32_t)vec ? vec : 1;
         a.per_run = (uint32_t)ceil_div(a.run, p.vec);
         a.vectors = (uint32_t)(flat ? 1 : N) * a.per_run;
+        p.flags = !r->reset ? kNoFlags : (p.vec == 1 || !flat || D % p.vec == 0 || N == 1) ? kOneFlag : D >= p.vec ? kTwoFlags : kFlagEach;
         split(p);
     };
     lanes(r->dtype == IGX_F32 ? 4 : 8);
@@ -97,7 +104,6 @@ void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, Plan &p)
         lanes(4);
         if (p.seg == 1) p.seg = 4;
     }
-    p.flags = !r->reset ? kNoFlags : (p.vec == 1 || !flat || D % p.vec == 0 || N == 1) ? kOneFlag : D >= p.vec ? kTwoFlags : kFlagEach;
 
     // forward order: as stored, or turned round for reverse; the backward pass goes the other way through the same order
     const bool down = (r->reverse != 0) != (g != nullptr);

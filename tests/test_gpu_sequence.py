@@ -81,7 +81,8 @@ def test_recurrence_shapes(shape, dtype):
     check_recurrence(*rollout(T, N, D, dtype, 1, resets=min(0.3, 4.0 / T)))
 
 
-MANY = [(13, 1100, 64), (11, 700, 105), (12, 25000, 3), (11, 5000, 105), (10, 9001, 64), (9, 180000, 3)]
+MANY = [(13, 1100, 64), (11, 700, 105), (12, 25000, 3), (11, 5000, 105), (10, 9001, 64), (9, 180000, 3),
+        (600, 17, 1000), (517, 330, 50)]  # ... or many groups share a long sequence, with one flag a lane or two
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -182,12 +183,15 @@ def test_recurrence_every_step_reset_and_zero_state():
 
 
 def test_recurrence_growing_gates_from_a_zero_state():
-    """Gates of 2 over 300 steps: their product overflows fp32, the state stays 0 until the last step."""
-    for T in (300, 3000):
-        inp = torch.zeros(T, 1, 8)
+    """Gates of 2 over 300 steps: their product overflows fp32, the state stays 0 until the last step.  A state that is not
+    0 overflows with it: inf, never a finite value."""
+    for T, N in ((300, 1), (3000, 1), (700, 2100)):
+        inp = torch.zeros(T, N, 8)
         inp[-1] = 1.0
-        out, last = sequence.linear_recurrence(torch.full((T, 1, 8), 2.0, device=DEV), inp.to(DEV))
+        gate = torch.full((T, N, 8), 2.0, device=DEV)
+        out, last = sequence.linear_recurrence(gate, inp.to(DEV))
         assert torch.equal(out.cpu(), inp) and (last == 1).all()
+        assert torch.isinf(sequence.linear_recurrence(gate, inp.to(DEV), state=torch.full((N, 8), 2.0 ** -40, device=DEV))[1]).all()
 
 
 @pytest.mark.parametrize("T,N,D", [(0, 3, 4), (5, 0, 4), (5, 3, 0), (0, 0, 0)])
