@@ -687,6 +687,35 @@ def test_side_stream():
         assert torch.equal(a, b)
 
 
+def test_host_threads_on_their_own_streams():
+    """Four host threads, each on its own stream and inputs, give what the serial calls give."""
+    import threading
+    shapes = [(600, 1, 40), (40, 6, 130), (300, 5, 100), (33, 300, 64)]
+    args = [block_inputs(*s, seed=100 + i) for i, s in enumerate(shapes)]
+    want = [block_pass(*a) for a in args]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i] = block_pass(*args[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # the assertion below reports it
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, b in zip(want, got):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
 def test_two_captured_graphs_replayed_with_eager_work_between():
     """Forward and backward of a block in two graphs, on new inputs every replay, against the eager pass."""
     graphs = []
