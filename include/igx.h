@@ -4,7 +4,8 @@
  *
  * Every entry point replaces a group of module-level @torch.jit.script
  * functions plus the in-place bookkeeping of one task class of the reference
- * (IsaacGymEnvs fork, paths relative to IsaacGymEnvs/isaacgymenvs/).  The
+ * (IsaacGymEnvs fork, paths relative to IsaacGymEnvs/isaacgymenvs/); the
+ * sequence operators at the end have no counterpart there.  The
  * reference has no FFI for this path (it is Python calling ATen); the
  * signatures below are what a ctypes binding on the reference side binds.
  *
