@@ -276,8 +276,9 @@ Tensor linear_recurrence_step(const Tensor &gate_, const Tensor &inp, const Tens
     c10::DeviceGuard guard(inp.device());
     const Tensor out = out_ ? *out_ : at::empty(inp.sizes(), inp.options());
     packed<char>(out, "out", inp.sizes(), inp.scalar_type(), inp);
-    TORCH_CHECK_VALUE(!out.numel() || (out.data_ptr() != r.gate && out.data_ptr() != r.inp && out.data_ptr() != r.state && out.data_ptr() != r.last),
-                      "out must not overlap an input");
+    auto apart = [&](const void *p) { return p != r.gate && p != r.inp; };
+    TORCH_CHECK_VALUE(!out.numel() || (apart(out.data_ptr()) && apart(r.last) && out.data_ptr() != r.state && out.data_ptr() != r.last),
+                      "a written tensor must not overlap another one of the call (state_out may be state)");
     r.out = out.data_ptr();
     r.out_stride[1] = r.width;
     check(lib.recurrence(&r, stream_of(inp)));

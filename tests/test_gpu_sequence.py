@@ -634,6 +634,15 @@ def test_layouts_that_are_refused():
         ops.linear_recurrence(r, r, r)
     with pytest.raises(ValueError, match="share one address"):
         ops.linear_recurrence(r, r, torch.zeros(4, 6, device=DEV).expand(3, 4, 6))
+    step = torch.zeros(4, 6, device=DEV)
+    with pytest.raises(ValueError, match="overlap"):
+        sequence.linear_recurrence_step(r[0], step, torch.zeros(4, 6, device=DEV), state_out=step)
+    with pytest.raises(ValueError, match="overlap"):
+        sequence.linear_recurrence_step(r[0], r[1], step, out=step)
+    with pytest.raises(ValueError, match="expected shape"):
+        sequence.linear_recurrence_step(r[0], r[1], step[:2])
+    with pytest.raises(TypeError, match="expected dtype"):
+        sequence.linear_recurrence_step(r[0], r[1], step.half())
     with pytest.raises(IgxError, match="8192"):
         sequence.rms_norm(torch.zeros(2, 8193, device=DEV), torch.ones(8193, device=DEV))
 
