@@ -29,14 +29,14 @@ struct NormArgs {
     bool sum_block, sum_next;
 };
 
-// 1 / (1 + exp(-z)) from the hardware's exponential and reciprocal (1 ulp each); `rest` carries what the product z log2(e)
-// loses, so that the error does not grow with |z|.  Where the exponential leaves fp32 the result is 0 or 1 without it.
-__device__ __forceinline__ float sigmoid(float z)
+// e = exp(-z) and 1 / (1 + e) from the hardware's exponential and reciprocal (1 ulp each); `rest` carries what the product
+// z log2(e) loses, so that the error does not grow with |z|.  Where e leaves fp32 the result is 0 or 1 without it.
+__device__ __forceinline__ float sigmoid(float z, float &e)
 {
     const float log2e = 1.44269504f, ln2 = 0.693147181f, log2e_rest = 1.92596303e-8f;
     const float t = -z * log2e;
     const float rest = (fmaf(-z, log2e, -t) - z * log2e_rest) * ln2;
-    float e = __builtin_amdgcn_exp2f(t);
+    e = __builtin_amdgcn_exp2f(t);
     e = fabsf(t) < 126.0f ? fmaf(e, rest, e) : e;  // not inf - inf
     return __builtin_amdgcn_rcpf(1.0f + e);
 }
@@ -44,7 +44,8 @@ __device__ __forceinline__ float sigmoid(float z)
 __device__ __forceinline__ float activate(float z, int act)
 {
     if (act == IGX_GATE_NONE) return z;
-    const float p = sigmoid(z);
+    float e;
+    const float p = sigmoid(z, e);
     return act == IGX_GATE_SIGMOID ? p : z * p;
 }
 
@@ -55,7 +56,8 @@ __device__ __forceinline__ void activate_slope(float z, int act, float &f, float
         slope = 1.0f;
         return;
     }
-    const float p = sigmoid(z), q = p * (1.0f - p);
+    float e;
+    const float p = sigmoid(z, e), q = fminf(e, 3.0e38f) * p * p;  // p (1 - p) without the difference of near values
     f = act == IGX_GATE_SIGMOID ? p : z * p;
     slope = act == IGX_GATE_SIGMOID ? q : fmaf(z, q, p);
 }
