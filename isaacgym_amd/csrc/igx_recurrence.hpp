@@ -26,6 +26,7 @@ struct RecArgs {
     uint32_t per_run;  // vectors in a run
     uint32_t vectors;  // vectors in all
     int splat;         // one gate for all channels of a run
+    int past;          // what is written goes past the caches' replacement
 };
 
 // Which channels a lane owns: V of them from `col` of run `row`.  The last vector of a run that V does not divide is
@@ -59,6 +60,12 @@ template <typename T, int V, bool STREAM = false> __device__ __forceinline__ voi
         for (int i = 0; i < V; i++)
             if (i >= skip) reinterpret_cast<T *>(p)[i] = (T)f[i];
     }
+}
+
+template <typename T, int V> __device__ __forceinline__ void store_step(const RecArgs &a, char *p, const float (&f)[V], int skip)
+{
+    if (a.past) store_from<T, V, true>(p, f, skip);
+    else store_from<T, V>(p, f, skip);
 }
 
 // Reset flags of the lane's channels for one step: one environment's, that of the first and the last (the environment
@@ -207,7 +214,7 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STRE
                     const float x1 = raw_at(x[k], i);
                     h[i] = f[k].begins(i) ? x1 : fmaf(raw_at(g[k], i), h[i], x1);
                 }
-                if (store) store_from<T, V, true>(to, h, l.skip);
+                if (store) store_step<T, V>(a, to, h, l.skip);
             } else {
                 float d[V], dg[V];
 #pragma unroll
@@ -224,10 +231,10 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STRE
 #pragma unroll
                         for (int i = 0; i < V; i++) dg[i] = f[k].begins(i) ? 0.0f : d[i] * a.state[l.channel + i];
                     }
-                    if (store) store_from<T, V, true>(d_gate, dg, l.skip);
+                    if (store) store_step<T, V>(a, d_gate, dg, l.skip);
                     d_gate += a.d_gate_t;
                 }
-                if (to && store) store_from<T, V, true>(to, d, l.skip);
+                if (to && store) store_step<T, V>(a, to, d, l.skip);
             }
             if (to) to += a.to_t;
         }
@@ -512,6 +519,7 @@ struct Plan {
     int flags;
     int seg;    // groups of lanes that share a workgroup's channels: 4, 16 or 64; 1: a lane walks all steps
     int64_t spans;
+    bool apart;  // an environment's steps are adjacent in memory rather than a step's environments
     int64_t workspace() const { return spans > 1 ? (1 + 2 * spans) * a.vectors * vec * (int64_t)sizeof(float) : 0; }
 };
 

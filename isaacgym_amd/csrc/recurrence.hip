@@ -53,12 +53,15 @@ bool follows(const igx_recurrence *r, int64_t stride_n) { return r->envs == 1 ||
 // for gate and inp are then read twice); 512 workgroups in all are enough.  Where they fill 256 and the sequence is long,
 // sixty-four groups keep a CU's waves busy (2 048 x 16 x 1 024 bf16: 137 us, 164 in sixteen; 1 024 x 64 x 256 fp32: 105, 139),
 // unless a lane needs more than one flag a step, which takes the registers (1 000 x 200 x 105 bf16: 234, 166 in sixteen).
+// Rollouts kept environment by environment have their next steps next to each other: four groups, however many lanes there
+// are, and the caches, which complete the lines that narrow rows share (32 x 20 000 x 60 fp32: 288 us, 474 with lanes that walk
+// alone past the caches).
 void split(Plan &p)
 {
     const int64_t vectors = p.a.vectors, T = p.a.T;
     p.spans = 1;
     p.a.span = T;
-    p.seg = T <= steps_of(16) || vectors >= 131072 ? 1 : vectors >= 16384 ? 4 : 16;
+    p.seg = T <= steps_of(16) || (vectors >= 131072 && !p.apart) ? 1 : vectors >= 16384 ? 4 : 16;
     if (p.seg != 16) return;
     const int64_t strips = ceil_div(vectors, lanes_of(16)), tile = 16 * steps_of(16);
     if (strips >= 256) {
@@ -85,6 +88,8 @@ void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, Plan &p)
         flat = (!g->d_out || follows(r, g->d_out_stride[1])) && (!g->d_inp || follows(r, g->d_inp_stride[1])) &&
                (!g->d_gate || (follows(r, g->d_gate_stride[1]) && follows(r, r->out_stride[1])));
     }
+    p.apart = !flat;
+    a.past = flat;
     // one gate for everything (all strides 0 beyond time) keeps the environments in one run
     const bool one_gate = (r->gate_stride[1] == 0 || N == 1) && (r->gate_stride[2] == 0 || D == 1);
     flat = flat && (one_gate || (!shared && follows(r, r->gate_stride[1])));

@@ -96,7 +96,7 @@ def test_recurrence_many_channels(shape, dtype):
 @pytest.mark.parametrize("layout", ["env", "slice"])
 def test_recurrence_many_short_rows(layout):
     """Environments that do not follow each other, narrower than a lane's vector or not divided by it."""
-    for T, N, D in ((11, 20000, 3), (10, 4000, 21)):
+    for T, N, D in ((11, 20000, 3), (10, 4000, 21), (9, 27000, 20)):
         check_recurrence(*rollout(T, N, D, F32, 14, resets=0.1), layout=layout, grad_layout="time")
 
 
