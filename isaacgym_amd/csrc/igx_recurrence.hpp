@@ -463,9 +463,9 @@ __global__ __launch_bounds__(lanes_of(SEG) * SEG) void recurrence_split_kernel(R
         mark<V>(A, starts);
         chain.run(A, B, h, from);
         s.walk(a, l, store, p.to, p.d_gate, ts, from);
+        if (store && ts < a.T && ts + kSteps >= a.T) store_end<V>(a, l, from);  // what the last step left: `out` is its rounding
         if (next < t1) s.load(a, lf, p.gate, p.add, p.before, next + seg * kSteps, t1);
     }
-    if (store && seg == 0 && blockIdx.y == gridDim.y - 1) store_end<V>(a, l, h);
 }
 
 // The (A, B) of every span: SEG groups of lanes reduce consecutive parts of it.

@@ -54,6 +54,7 @@ def linear_recurrence(gate, inp, state=None, reset=None, reverse=False):
     step (None: zeros); reset [T, N] int64: where it is not 0 an episode begins and the value before is dropped.
     reverse=True runs from the last step to the first.  Differentiable (once) in gate, inp and state; where gate is
     broadcast its full-size gradient is summed by torch afterwards.
+    Steps behind the end of a shorter rollout are padded with gate 1 and input 0: they hand the value through.
 
     The carried value is float32 whatever the type; `out` is its rounding, and the gradient of gate is computed from
     `out` as stored.  Products of consecutive gates have to stay within float32's range (gates in [-1, 1] always do)."""

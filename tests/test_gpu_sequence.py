@@ -236,6 +236,44 @@ def test_recurrence_step_in_place_where_lanes_share_channels():
             assert torch.equal(h, to)
 
 
+@pytest.mark.parametrize("T,N,D", [(60, 7, 20), (2000, 1, 24)])
+def test_recurrence_in_two_calls(T, N, D):
+    """A rollout cut in two, `last` handed on as `state`: outputs and gradients are those of the whole."""
+    gate, inp, state, reset, d_out, d_last = rollout(T, N, D, F32, 16, resets=0.02)
+    ref = S.recurrence(gate, inp, state, reset, False, d_out, d_last)
+    a, b, h = (t.to(DEV).requires_grad_(True) for t in (gate, inp, state))
+    f, cut = reset.to(DEV), T // 3
+    one, mid = sequence.linear_recurrence(a[:cut], b[:cut], state=h, reset=f[:cut])
+    two, end = sequence.linear_recurrence(a[cut:], b[cut:], state=mid, reset=f[cut:])
+    out = torch.cat((one, two))
+    S.close(out, *ref["out"], "out")
+    S.close(end, *ref["last"], "last")
+    for name, got in zip(("d_gate", "d_inp", "d_state"), torch.autograd.grad((out, end), (a, b, h), (d_out.to(DEV), d_last.to(DEV)))):
+        S.close(got, *ref[name], name)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("shape", [(7, 5, 12), (40, 6, 12), (3000, 1, 8), (700, 2100, 8), (20, 9000, 8), (10, 70000, 8)])
+def test_recurrence_last_is_what_the_last_step_left(shape, reverse):
+    """In every split of the time `last` is the fp32 value whose rounding is out's last step, and steps with gate 1 and input
+    0 behind an environment's last one hand its state through."""
+    T, N, D = shape
+    g = torch.Generator(device=DEV).manual_seed(17)
+    gate, inp = torch.rand(T, N, D, device=DEV, generator=g), torch.randn(T, N, D, device=DEV, generator=g)
+    length = torch.randint(1, T, (N,), device=DEV, generator=g)
+    pad = torch.arange(T, device=DEV)[:, None] >= length
+    gate[pad], inp[pad] = 1.0, 0.0
+    if reverse:
+        gate, inp = gate.flip(0), inp.flip(0)
+    for dtype in (F32, BF16):
+        out, last = sequence.linear_recurrence(gate.to(dtype), inp.to(dtype), reverse=reverse)
+        assert torch.equal(out[0 if reverse else -1], last.to(dtype))
+    out, last = sequence.linear_recurrence(gate, inp, reverse=reverse)
+    end = out.flip(0)[length - 1, torch.arange(N, device=DEV)] if reverse else out[length - 1, torch.arange(N, device=DEV)]
+    # |out| < 1 + the magnitudes' sum of a recurrence with gates below 1 and inputs below 7; 3 u of it a step, T steps
+    assert float((end - last).abs().max()) <= 3 * S.U * T * 7 * min(T, 20)
+
+
 def test_recurrence_writes_only_its_elements():
     gate, inp, state, reset, _, _ = rollout(70, 3, 13, F16, 9, resets=0.1)
     big = torch.full((140, 3, 20), 7.0, dtype=F16, device=DEV)
