@@ -3,9 +3,9 @@
 // Channels are independent and adjacent in memory, so a lane owns a vector of channels (16 bytes) and walks the steps with
 // the carried value in fp32 registers.  A call moves 3 elements per (t, n, d) forward and 5 backward and does 2 - 3
 // operations on each: HBM bounds it where there are enough channels to fill the card (32 x 65 536 x 64 bf16 forward and
-// backward: 2.15 GB in 406 us, 5.3 TB/s; one step of 262 144 x 64 with its fp32 state: 235 MB in 38 us, 6.2 TB/s).  Arrays
-// that nothing reads again soon go past the caches' replacement (non-temporal; loads too where a lane walks alone: 406 us
-// against 444).
+// backward: 2.25 GB in 400 us, 5.6 TB/s; one step of 262 144 x 64 with its fp32 state: 235 MB in 38 us, 6.2 TB/s).  Arrays
+// that nothing reads again soon go past the caches' replacement (non-temporal; loads too where a lane walks alone: 400 us
+// against 427).
 //
 // With fewer channels the time is split, for the recurrence is a composition of maps h -> A h + B that is associative:
 //   - within a workgroup SEG groups of lanes take a few consecutive steps each of the same channels, reduce them to
