@@ -1124,7 +1124,8 @@ int igx_linear_recurrence_backward(const igx_recurrence *r, const igx_recurrence
  * with out = x where y is NULL (a norm in front of the first block), scale and gate 1 where NULL.  Statistics and the
  * whole row's arithmetic are fp32, `next` is computed from the unrounded out, every result is rounded once.
  * Checkpoints (optional outputs of the forward call): the 8-bit codes of y and gate - of x where y is NULL - in the
- * form of igx_pack8, for a backward call that has the codes in place of those arrays. */
+ * form of igx_pack8, for a backward call that has the codes in place of those arrays.  A gate is limited before it
+ * is coded: to >= -16 for the SiLU, to within +-16 for the sigmoid. */
 #define IGX_GATE_NONE 0     /* act(z) = z */
 #define IGX_GATE_SIGMOID 1  /* act(z) = 1 / (1 + exp(-z)) */
 #define IGX_GATE_SILU 2     /* act(z) = z / (1 + exp(-z)) */

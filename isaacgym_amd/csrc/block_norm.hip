@@ -13,6 +13,24 @@
 namespace igx {
 namespace {
 
+// Gates as their codes hold them: no further out than +-16, so that one that is shut by a very low value does not take the
+// other 63 of its group their scale.  Beyond it the activations are off by less than 16 exp(-16) < 2^-19, where a code of
+// such a group has steps of 16 / 127.  NaN stays.  One instruction an element, with a branch for the sigmoid's upper end (the
+// whole kernel on 131 072 x 512 bf16: 156 us, 154 without limits, 161 with two instructions or selects).
+template <int V, int K> __device__ __forceinline__ void limit_gates(const float (&z)[K][V], int act, float (&g)[K][V])
+{
+    const float most = 16.0f, lowest = act == IGX_GATE_NONE ? -__builtin_inff() : -most;
+#pragma unroll
+    for (int k = 0; k < K; k++)
+#pragma unroll
+        for (int i = 0; i < V; i++) g[k][i] = __builtin_elementwise_maximum(z[k][i], lowest);
+    if (act != IGX_GATE_SIGMOID) return;
+#pragma unroll
+    for (int k = 0; k < K; k++)
+#pragma unroll
+        for (int i = 0; i < V; i++) g[k][i] = __builtin_elementwise_minimum(g[k][i], most);
+}
+
 // the row's 8-bit codes: a group's lanes sit next to each other (with 8 lanes of 4 columns, in both of their vectors)
 template <int V, int K, int LANES>
 __device__ __forceinline__ void checkpoint_row(const float (&f)[K][V], const int (&left)[K], const int (&col)[K], int8_t *codes,
@@ -113,7 +131,11 @@ __global__ __launch_bounds__(block_of(LANES)) void block_norm_kernel(NormArgs a)
                 for (int k = 0; k < K; k++) widen_row<T, V>(in.gate[k], have[k], z[k]);
             }
             if (a.y8) checkpoint_row<V, K, LANES>(y, have, col, a.y8 + at_row, a.y8_scale + row * a.groups);
-            if (a.gate && a.gate8) checkpoint_row<V, K, LANES>(z, have, col, a.gate8 + at_row, a.gate8_scale + row * a.groups);
+            if (a.gate && a.gate8) {
+                float g[K][V];
+                limit_gates(z, a.act, g);
+                checkpoint_row<V, K, LANES>(g, have, col, a.gate8 + at_row, a.gate8_scale + row * a.groups);
+            }
 #pragma unroll
             for (int k = 0; k < K; k++) {
 #pragma unroll

@@ -621,6 +621,30 @@ def test_pack8_shapes_and_empty():
     assert sequence.unpack8(codes, scales).shape == (0, 70)
 
 
+@pytest.mark.parametrize("activation", ["silu", "sigmoid"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", [(40, 60), (9, 130), (3, 1100)])
+def test_checkpointed_gates_shut_by_very_low_values(shape, dtype, activation):
+    """A shut gate takes the others of its group no precision; the gradients are those at the limited gates' codes."""
+    t, do, dn = norm_inputs(*shape, dtype, 46)
+    shut = torch.rand(shape, generator=gen(47)) < 0.1
+    shut[1] = True  # a row without any open one
+    t["gate"] = torch.where(shut, torch.full_like(t["gate"], torch.finfo(dtype).min), t["gate"])
+    if activation == "sigmoid":
+        t["gate"][0, 3], t["gate"][2, 5] = float("inf"), float("-inf")
+    dev = {k: v.to(DEV).requires_grad_(True) for k, v in t.items()}
+    outs = sequence.residual_norm(**dev, activation=activation, checkpoint=True)
+    grads = torch.autograd.grad(outs, list(dev.values()), (do.to(DEV), dn.to(DEV)))
+    limited = t["gate"].clamp(min=-16, max=16 if activation == "sigmoid" else None)
+    # Results and the rows' inverse roots come from the gates themselves, whose activations are off from the limited ones' by
+    # less than 16 exp(-16) < 2^-19.  That moves a row's inverse root by less than 2^-18 of it, and no result holds more than
+    # its third power: 2^-16 of the terms' magnitudes, of which twice the largest result is taken as the bound.
+    ref = S.block_norm(**dict(t, gate=limited), activation=activation, d_out=do, d_next=dn, checkpoint=True)
+    for name, got in list(zip(("out", "next"), outs)) + [("d_" + k, g) for k, g in zip(dev, grads)]:
+        value, bound = ref[name]
+        S.close(got, value, bound + 2.0 ** -15 * value.abs().max(), name)
+
+
 def test_checkpoint_frees_what_it_replaces():
     """With checkpoint=True the graph holds codes, not the block's output and gate."""
     R, D = 8192, 512
