@@ -62,7 +62,7 @@ __device__ __forceinline__ void checkpoint_row(const float (&f)[K][V], const int
         } else {
 #pragma unroll
             for (int i = 0; i < V; i++)
-                if (i < left[k]) codes[col[k] + i] = (int8_t)code_of(f[k][i], s.inverse);
+                if (i < left[k]) codes[col[k] + i] = code_of(f[k][i], s.inverse);
         }
         if (left[k] > 0 && col[k] % IGX_PACK8_GROUP == 0) scales[col[k] / IGX_PACK8_GROUP] = s.scale;
     }

@@ -79,9 +79,16 @@ __device__ __forceinline__ GroupScale group_scale(uint32_t top_bits)
     return s;
 }
 
-__device__ __forceinline__ int code_of(float x, float inverse)
+// The code in the low byte.  |x| <= top, so the product lies within +-127 and the sum's last place is 1: the addition rounds
+// to the nearest integer, ties to even, and its mantissa ends in the integer's two's complement.
+__device__ __forceinline__ uint32_t code_bits(float x, float inverse)
 {
-    return inverse == 0.0f ? 0 : (int)rintf(x * inverse);  // |x| <= top: within +-127
+    return __float_as_uint(x * inverse + 12582912.0f);  // 3 * 2^22
+}
+
+__device__ __forceinline__ int8_t code_of(float x, float inverse)
+{
+    return inverse == 0.0f ? 0 : (int8_t)code_bits(x, inverse);
 }
 
 template <int V> __device__ __forceinline__ void store_codes(int8_t *p, const float (&x)[V], float inverse)
@@ -89,9 +96,11 @@ template <int V> __device__ __forceinline__ void store_codes(int8_t *p, const fl
     uint32_t w[V / 4];
 #pragma unroll
     for (int j = 0; j < V / 4; j++) {
-        w[j] = 0;
+        uint32_t c[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[j] |= (uint32_t)(code_of(x[4 * j + i], inverse) & 255) << (8 * i);
+        for (int i = 0; i < 4; i++) c[i] = code_bits(x[4 * j + i], inverse);
+        const uint32_t low = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400), high = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400);
+        w[j] = inverse == 0.0f ? 0 : __builtin_amdgcn_perm(high, low, 0x05040100);  // 0: the products may be NaN
     }
     __builtin_memcpy(p, w, V);
 }

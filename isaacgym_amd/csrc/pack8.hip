@@ -63,7 +63,7 @@ __global__ __launch_bounds__(kBlock) void pack8_kernel(const char *x, int64_t st
     } else {
 #pragma unroll
         for (int i = 0; i < V; i++)
-            if (i < p.left) codes[p.at + i] = (int8_t)code_of(f[i], s.inverse);
+            if (i < p.left) codes[p.at + i] = code_of(f[i], s.inverse);
     }
     if (threadIdx.x % LPG == 0 && p.left > 0) scales[p.row * groups + p.group] = s.scale;
 }
