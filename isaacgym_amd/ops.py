@@ -880,7 +880,7 @@ def block_norm(x, y=None, weight=None, gate=None, scale=None, next_weight=None, 
     without y: out = x).  x, y, gate are [..., width] with adjacent columns and evenly spaced rows, out and next
     contiguous, parameters fp32 [width].  Filled in where given: inv_rms fp32 [2, rows], the rows' 1 / rms of y and of out
     (what block_norm_backward needs); codes: the 8-bit checkpoint, (codes, scales) of y - of x without y - and then of
-    gate if there is one."""
+    gate if there is one, as >= -16 with "silu" and within +-16 with "sigmoid"."""
     b = _block_norm(x, weight, gate, scale, next_weight, inv_rms, codes, activation, eps)
     shape = x.shape
     b.x, b.x_stride = _row_array(x, "x", shape, x)
