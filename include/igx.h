@@ -47,9 +47,10 @@ extern "C" {
 typedef void *igx_stream_t; /* hipStream_t */
 
 /* Library identification and error text (no reference counterpart).
- * igx_version() = 100 * major + 10 * minor, 130 for this header: a binding that needs igx_motion_fetch_amp_obs,
+ * igx_version() = 100 * major + 10 * minor, 140 for this header: a binding that needs igx_motion_fetch_amp_obs,
  * igx_motion_amp_obs_history or igx_extract_positions_from_rigid_body_states checks for >= 120, one that needs the
- * sequence operators (igx_linear_recurrence*, igx_block_norm*, igx_pack8, igx_unpack8) for >= 130. */
+ * sequence operators (igx_linear_recurrence*, igx_block_norm*, igx_pack8, igx_unpack8) for >= 130, and one that needs
+ * their forms _with_rest for >= 140. */
 int igx_version(void);
 const char *igx_last_error_string(void);
 
@@ -1102,7 +1103,7 @@ int igx_linear_recurrence(const igx_recurrence *r, igx_stream_t stream);
 /* Gradients: r holds the forward call's arguments (out as the forward wrote it; inp and last are not read).
  *     d[t] = d_out[t] + gate of the following step * d of the following step (d_last behind the last one)
  *     d_inp = d,  d_gate = d * before (0 where an episode begins),  d_state = what leaves the first step.
- * `before` is read from `out`, at the precision it was stored in.  A gate that several channels or environments share
+ * `before` is read from `out`, at the precision it was stored in (but see igx_recurrence_rest).  A gate that several channels or environments share
  * (a stride of 0) gets its [T, N, D] gradients unsummed. */
 typedef struct igx_recurrence_grad {
     const void *d_out;        /* elements [T, N, D] at d_out_stride, channels adjacent; NULL = zeros */
@@ -1116,6 +1117,19 @@ typedef struct igx_recurrence_grad {
 } igx_recurrence_grad;
 
 int igx_linear_recurrence_backward(const igx_recurrence *r, const igx_recurrence_grad *g, igx_stream_t stream);
+
+/* The same with what out's rounding to 16 bits took from the carried value, so that d_gate is computed from that value:
+ * 8 bits more of it, within 2^-7 of out's own half step (fp16 below its smallest normal number: less is gained), nothing
+ * where out is inf or NaN.  The forward call writes codes, the backward call reads them beside out where d_gate is wanted.
+ * IGX_F16 and IGX_BF16 only: an fp32 out is the value.  rest NULL: the calls above. */
+typedef struct igx_recurrence_rest {
+    int8_t *codes;            /* [T, N, D] at stride, channels adjacent */
+    int64_t stride[2];
+} igx_recurrence_rest;
+
+int igx_linear_recurrence_with_rest(const igx_recurrence *r, const igx_recurrence_rest *rest, igx_stream_t stream);
+int igx_linear_recurrence_backward_with_rest(const igx_recurrence *r, const igx_recurrence_grad *g,
+                                             const igx_recurrence_rest *rest, igx_stream_t stream);
 
 /* The norms before and after a block of a residual network, with the branch's gate and residual scale, row by row
  * (rms(v) = v / sqrt(mean(v^2) + eps) over the row's `width` elements):

@@ -425,6 +425,10 @@ class RecurrenceGrad(_Struct):
                 ("d_inp", ptr), ("d_inp_stride", i64 * 2), ("d_state", ptr)]
 
 
+class RecurrenceRest(_Struct):
+    _fields_ = [("codes", ptr), ("stride", i64 * 2)]
+
+
 class BlockNorm(_Struct):
     _fields_ = [("dtype", i32), ("activation", i32), ("rows", i64), ("width", i64), ("eps", f32),
                 ("x", ptr), ("x_stride", i64), ("y", ptr), ("y_stride", i64), ("gate", ptr), ("gate_stride", i64),

@@ -114,6 +114,8 @@ SYMBOLS.update({
     "igx_linear_recurrence_workspace": (_I64, [_P]),
     "igx_linear_recurrence": (C.c_int, [_P, _P]),
     "igx_linear_recurrence_backward": (C.c_int, [_P, _P, _P]),
+    "igx_linear_recurrence_with_rest": (C.c_int, [_P, _P, _P]),
+    "igx_linear_recurrence_backward_with_rest": (C.c_int, [_P, _P, _P, _P]),
     "igx_block_norm_workspace": (_I64, [_P]),
     "igx_block_norm_forward": (C.c_int, [_P, _P]),
     "igx_block_norm_backward": (C.c_int, [_P, _P, _P]),

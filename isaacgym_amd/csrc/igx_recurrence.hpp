@@ -1,5 +1,7 @@
 // The linear recurrence's kernels (recurrence.hip instantiates the forward, recurrence_backward.hip the backward ones).
 #pragma once
+#include <type_traits>
+
 #include "igx_seq.hpp"
 
 namespace igx {
@@ -14,12 +16,13 @@ enum Flags { kNoFlags = 0, kOneFlag = 1, kTwoFlags = 2, kFlagEach = 3 };
 // backward runs the other way, add = d_out, before = out one step further on.
 struct RecArgs {
     const char *gate, *add, *reset, *before;
+    char *rest;                 // what out's rounding took: forward writes it, backward reads it beside `before`; NULL: not kept
     char *to, *d_gate;          // forward: out; backward: d_inp, d_gate (NULL: not wanted)
     const float *start;         // forward: state, backward: d_last; NULL: zeros
     float *end;                 // forward: last, backward: d_state; NULL: not wanted
     const float *state;         // backward: what stands before the first step; NULL: zeros
     float *spans;               // [0]: start; [1 + 2 s], [2 + 2 s]: A and B of span s; rows of `vectors` lane vectors
-    int64_t gate_t, gate_n, add_t, add_n, reset_t, reset_n, before_t, before_n, to_t, to_n, d_gate_t, d_gate_n;
+    int64_t gate_t, gate_n, add_t, add_n, reset_t, reset_n, before_t, before_n, rest_t, rest_n, to_t, to_n, d_gate_t, d_gate_n;
     int64_t T, span;            // steps in all, and in a span
     uint32_t D;
     uint32_t run;      // channels that are adjacent in every array: N * D where the environments follow each other, else D
@@ -66,6 +69,64 @@ template <typename T, int V> __device__ __forceinline__ void store_step(const Re
 {
     if (a.past) store_from<T, V, true>(p, f, skip);
     else store_from<T, V>(p, f, skip);
+}
+
+// What the rounding to a 16-bit type took from a value, as 8 more bits: numbers of one sign order like their fp32 bit patterns,
+// so it is the difference of the value's and the rounded value's patterns, counted in 1/256 of the type's step (2^16 patterns
+// in bf16, 2^13 in fp16) and rounded to that: value and sum differ by at most 2^-7 of the half step that out is off by, and not
+// at all where out is the value.  fp16's subnormals, whose steps are wider, gain less.  Beside inf and NaN it is 0.  8 bits, not
+// the 16 that would be fp32: what is computed from the sum is itself rounded to T, a step 2^8 times as wide.  They take half
+// of an array's bytes each way and go through the caches even where the arrays go past them (32 x 65 536 x 64 bf16, forward and
+// backward: 427 us, 469 past the caches, 398 without codes).
+template <typename T> constexpr int kRestShift = sizeof(T) == 4 ? 0 : std::is_same<T, __bf16>::value ? 8 : 5;
+
+template <typename T> __device__ __forceinline__ int rest_code(float h)
+{
+    constexpr int S = kRestShift<T>;
+    const uint32_t o = __float_as_uint((float)(T)h);
+    const int d = (int)(__float_as_uint(h) - o);
+    const int code = min(max((d + (1 << S >> 1)) >> S, -128), 127);
+    return (o & 0x7f800000u) == 0x7f800000u ? 0 : code;
+}
+
+template <int V> struct RestWords {
+    static constexpr int kCount = V >= 4 ? V / 4 : 1;
+    uint32_t w[kCount];
+    __device__ __forceinline__ int at(int i) const { return (int8_t)(w[i / 4] >> (8 * (i % 4))); }
+};
+
+template <int V> __device__ __forceinline__ RestWords<V> load_rest(const char *p)
+{
+    RestWords<V> r;
+    if constexpr (V == 1) {
+        r.w[0] = *reinterpret_cast<const uint8_t *>(p);
+    } else {
+        typedef uint32_t Word __attribute__((aligned(1)));
+#pragma unroll
+        for (int j = 0; j < V / 4; j++) {
+            r.w[j] = reinterpret_cast<const Word *>(p)[j];
+        }
+    }
+    return r;
+}
+
+template <typename T, int V> __device__ __forceinline__ void store_rest(char *p, const float (&h)[V], int skip)
+{
+    if (V == 1 || skip) {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i >= skip) p[i] = (char)rest_code<T>(h[i]);
+    } else if constexpr (V > 1) {
+        typedef uint32_t Word __attribute__((aligned(1)));
+#pragma unroll
+        for (int j = 0; j < V / 4; j++) {
+            uint32_t c[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) c[i] = (uint32_t)rest_code<T>(h[4 * j + i]);
+            const uint32_t low = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400), high = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400);
+            reinterpret_cast<Word *>(p)[j] = __builtin_amdgcn_perm(high, low, 0x05040100);
+        }
+    }
 }
 
 // Reset flags of the lane's channels for one step: one environment's, that of the first and the last (the environment
@@ -137,16 +198,17 @@ __device__ __forceinline__ float as_factor(float A, bool none)
 }
 
 // K consecutive steps of a lane's channels in registers.  `count` of them exist, the others repeat the last one and are
-// neutral; whole steps of a full group cost no test (CHECK false).
-template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STREAM> struct Steps {
+// neutral; whole steps of a full group cost no test (CHECK false).  REST: there may be codes of out's rounding.
+template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STREAM, bool REST> struct Steps {
     Raw<T, V> g[K], x[K], hb[K];
+    RestWords<V> rb[K];  // REST
     StepFlags<V, FL> f[K];
     int count;
 
     // The addresses run along by a stride: a product of 64 bits for every load would cost more than the recurrence.  Steps
     // that do not exist repeat the last one.
     __device__ __forceinline__ void load(const RecArgs &a, const LaneFlags<V, FL> &lf, const char *gate, const char *add,
-                                         const char *before, int64_t t0, int64_t t1)
+                                         const char *before, const char *rest, int64_t t0, int64_t t1)
     {
         count = CHECK ? (t1 - t0 < K ? (int)(t1 - t0) : K) : K;
         const int64_t t = CHECK && t0 >= t1 ? t1 - 1 : t0;
@@ -177,7 +239,27 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STRE
                 if (t + k < a.T - 1) hb[k] = load_raw<T, V, STREAM>(before);
                 before += on(k) ? a.before_t : 0;
             }
+            if constexpr (REST) {
+#pragma unroll
+                for (int k = 0; k < K; k++) rb[k] = {};
+                if (rest) {
+                    rest += t * a.rest_t;
+#pragma unroll
+                    for (int k = 0; k < K; k++) {
+                        if (t + k < a.T - 1) rb[k] = load_rest<V>(rest);
+                        rest += on(k) ? a.rest_t : 0;
+                    }
+                }
+            }
         }
+    }
+    // the value before step k, from out (and what its rounding took)
+    __device__ __forceinline__ float value_before(int k, int i) const
+    {
+        if constexpr (REST)
+            return __uint_as_float(__float_as_uint(raw_at(hb[k], i)) + (uint32_t)(rb[k].at(i) << kRestShift<T>));
+        else
+            return raw_at(hb[k], i);
     }
     __device__ __forceinline__ bool on(int k) const { return !CHECK || k + 1 < count; }  // is there a step behind step k?
     __device__ __forceinline__ bool there(int k) const { return !CHECK || k < count; }
@@ -199,11 +281,12 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STRE
         }
     }
 
-    // forward: h = gate h + inp -> out.  backward: d = d_out + h -> d_inp, d * before -> d_gate, h = gate d
-    __device__ __forceinline__ void walk(const RecArgs &a, const Lane &l, bool store, char *to, char *d_gate, int64_t t0,
-                                         float (&h)[V]) const
+    // forward: h = gate h + inp -> out, rest.  backward: d = d_out + h -> d_inp, d * before -> d_gate, h = gate d
+    __device__ __forceinline__ void walk(const RecArgs &a, const Lane &l, bool store, char *to, char *d_gate, char *rest,
+                                         int64_t t0, float (&h)[V]) const
     {
         if (to) to += t0 * a.to_t;
+        if (!BACKWARD && rest) rest += t0 * a.rest_t;
         if (BACKWARD && d_gate) d_gate += t0 * a.d_gate_t;
 #pragma unroll
         for (int k = 0; k < K; k++) {
@@ -215,6 +298,12 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STRE
                     h[i] = f[k].begins(i) ? x1 : fmaf(raw_at(g[k], i), h[i], x1);
                 }
                 if (store) store_step<T, V>(a, to, h, l.skip);
+                if constexpr (REST) {
+                    if (rest) {
+                        if (store) store_rest<T, V>(rest, h, l.skip);
+                        rest += a.rest_t;
+                    }
+                }
             } else {
                 float d[V], dg[V];
 #pragma unroll
@@ -226,7 +315,7 @@ template <typename T, int V, int FL, int K, bool BACKWARD, bool CHECK, bool STRE
                 if (d_gate) {
                     if (t0 + k < a.T - 1) {
 #pragma unroll
-                        for (int i = 0; i < V; i++) dg[i] = f[k].begins(i) ? 0.0f : d[i] * raw_at(hb[k], i);
+                        for (int i = 0; i < V; i++) dg[i] = f[k].begins(i) ? 0.0f : d[i] * value_before(k, i);
                     } else if (a.state) {
 #pragma unroll
                         for (int i = 0; i < V; i++) dg[i] = f[k].begins(i) ? 0.0f : d[i] * a.state[l.channel + i];
@@ -257,13 +346,14 @@ template <int V> __device__ __forceinline__ void mark(float (&A)[V], const bool 
 // where a lane's channels lie in the arrays
 template <typename T> struct Places {
     const char *gate, *add, *before;
-    char *to, *d_gate;
+    char *rest, *to, *d_gate;
     __device__ __forceinline__ Places(const RecArgs &a, const Lane &l)
     {
         const int64_t at = (int64_t)l.col * sizeof(T);
         gate = a.gate + l.row * a.gate_n + (a.splat ? 0 : at);
         add = a.add ? a.add + l.row * a.add_n + at : nullptr;
         before = a.before ? a.before + l.row * a.before_n + at : nullptr;
+        rest = a.rest ? a.rest + l.row * a.rest_n + l.col : nullptr;
         to = a.to ? a.to + l.row * a.to_n + at : nullptr;
         d_gate = a.d_gate ? a.d_gate + l.row * a.d_gate_n + at : nullptr;
     }
@@ -285,8 +375,9 @@ template <int V> __device__ __forceinline__ void store_end(const RecArgs &a, con
     if (a.end) store_from<float, V>(reinterpret_cast<char *>(a.end + l.channel), h, l.skip);
 }
 
-// enough channels: a lane walks all the steps
-template <typename T, int V, int FL, bool BACKWARD>
+// enough channels: a lane walks all the steps.  REST is an argument of the template here, for a branch around its loads costs
+// calls without it 2 % (32 x 65 536 x 64 bf16, forward and backward: 399 us, 408 with the branch).
+template <typename T, int V, int FL, bool BACKWARD, bool REST>
 __global__ __launch_bounds__(kRecBlock) void recurrence_kernel(RecArgs a)
 {
     const uint32_t v = blockIdx.x * kRecBlock + threadIdx.x;
@@ -297,9 +388,9 @@ __global__ __launch_bounds__(kRecBlock) void recurrence_kernel(RecArgs a)
     float h[V];
     load_start<V>(a.start, l, h);
     for (int64_t t = 0; t < a.T; t++) {
-        Steps<T, V, FL, steps_of(1), BACKWARD, false, true> s;
-        s.load(a, lf, p.gate, p.add, p.before, t, t + 1);
-        s.walk(a, l, true, p.to, p.d_gate, t, h);
+        Steps<T, V, FL, steps_of(1), BACKWARD, false, true, REST> s;
+        s.load(a, lf, p.gate, p.add, p.before, p.rest, t, t + 1);
+        s.walk(a, l, true, p.to, p.d_gate, p.rest, t, h);
     }
     store_end<V>(a, l, h);
 }
@@ -436,8 +527,8 @@ __global__ __launch_bounds__(lanes_of(SEG) * SEG) void recurrence_split_kernel(R
     const LaneFlags<V, FL> lf(a, l);
     const Places<T> p(a, l);
     const int64_t first = (int64_t)blockIdx.y * a.span, t1 = first + a.span < a.T ? first + a.span : a.T;
-    Steps<T, V, FL, kSteps, BACKWARD, true, false> s;
-    s.load(a, lf, p.gate, p.add, p.before, first + seg * kSteps, t1);  // on its way while the spans are composed
+    Steps<T, V, FL, kSteps, BACKWARD, true, false, sizeof(T) == 2> s;
+    s.load(a, lf, p.gate, p.add, p.before, p.rest, first + seg * kSteps, t1);  // on its way while the spans are composed
     float h[V], A[V], B[V], from[V];
     bool starts[V];
     if (gridDim.y == 1) {
@@ -462,9 +553,9 @@ __global__ __launch_bounds__(lanes_of(SEG) * SEG) void recurrence_split_kernel(R
         s.reduce(A, B, starts);
         mark<V>(A, starts);
         chain.run(A, B, h, from);
-        s.walk(a, l, store, p.to, p.d_gate, ts, from);
+        s.walk(a, l, store, p.to, p.d_gate, p.rest, ts, from);
         if (store && ts < a.T && ts + kSteps >= a.T) store_end<V>(a, l, from);  // what the last step left: `out` is its rounding
-        if (next < t1) s.load(a, lf, p.gate, p.add, p.before, next + seg * kSteps, t1);
+        if (next < t1) s.load(a, lf, p.gate, p.add, p.before, p.rest, next + seg * kSteps, t1);
     }
 }
 
@@ -488,8 +579,8 @@ __global__ __launch_bounds__(kRecBlock) void recurrence_spans_kernel(RecArgs a)
     bool starts[V];
     identity<V>(A, B, starts);
     for (int64_t t = from; t < to; t += kSteps) {
-        Steps<T, V, FL, kSteps, BACKWARD, true, false> s;
-        s.load(a, lf, p.gate, p.add, nullptr, t, to);
+        Steps<T, V, FL, kSteps, BACKWARD, true, false, false> s;
+        s.load(a, lf, p.gate, p.add, nullptr, nullptr, t, to);
         s.reduce(A, B, starts);
     }
     mark<V>(A, starts);
@@ -530,7 +621,11 @@ template <typename T, int V, int FL, bool BACKWARD> void launch_as(const Plan &p
     if (p.spans > 1)
         recurrence_spans_kernel<T, V, FL, BACKWARD><<<dim3((unsigned)ceil_div(v, kRecBlock / 16), (unsigned)p.spans), block, 0, s>>>(p.a);
     if (p.seg == 1) {
-        recurrence_kernel<T, V, FL, BACKWARD><<<dim3((unsigned)ceil_div(v, kRecBlock)), block, 0, s>>>(p.a);
+        const dim3 grid((unsigned)ceil_div(v, kRecBlock));
+        if constexpr (sizeof(T) == 2) {
+            if (p.a.rest) return recurrence_kernel<T, V, FL, BACKWARD, true><<<grid, block, 0, s>>>(p.a);
+        }
+        recurrence_kernel<T, V, FL, BACKWARD, false><<<grid, block, 0, s>>>(p.a);
     } else if (p.seg == 4) {
         recurrence_split_kernel<T, V, FL, BACKWARD, 4><<<dim3((unsigned)ceil_div(v, lanes_of(4))), block, 0, s>>>(p.a);
     } else {

@@ -75,7 +75,7 @@ void split(Plan &p)
     p.spans = ceil_div(T, p.a.span);
 }
 
-void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, Plan &p)
+void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, const igx_recurrence_rest *rest, Plan &p)
 {
     RecArgs &a = p.a;
     a = RecArgs();
@@ -88,6 +88,8 @@ void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, Plan &p)
         flat = (!g->d_out || follows(r, g->d_out_stride[1])) && (!g->d_inp || follows(r, g->d_inp_stride[1])) &&
                (!g->d_gate || (follows(r, g->d_gate_stride[1]) && follows(r, r->out_stride[1])));
     }
+    if (g && !g->d_gate) rest = nullptr;  // not read
+    if (rest) flat = flat && follows(r, rest->stride[1]);
     p.apart = !flat;
     a.past = flat;
     // one gate for everything (all strides 0 beyond time) keeps the environments in one run
@@ -123,6 +125,7 @@ void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, Plan &p)
     if (!g) {
         a.add = turn(r->inp, r->inp_stride[0], r->inp_stride[1], e, a.add_t, a.add_n);
         a.to = const_cast<char *>(turn(r->out, r->out_stride[0], r->out_stride[1], e, a.to_t, a.to_n));
+        if (rest) a.rest = const_cast<char *>(turn(rest->codes, rest->stride[0], rest->stride[1], 1, a.rest_t, a.rest_n));
         a.start = r->state;
         a.end = r->last;
     } else {
@@ -132,6 +135,10 @@ void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, Plan &p)
         if (a.d_gate) {  // the value before a step is one step further on in out, counted backwards
             a.before = turn(r->out, r->out_stride[0], r->out_stride[1], e, a.before_t, a.before_n);
             a.before += a.before_t;
+            if (rest) {
+                a.rest = const_cast<char *>(turn(rest->codes, rest->stride[0], rest->stride[1], 1, a.rest_t, a.rest_n));
+                a.rest += a.rest_t;
+            }
             a.state = r->state;
         }
         a.start = g->d_last;
@@ -176,40 +183,79 @@ extern "C" int64_t igx_linear_recurrence_workspace(const igx_recurrence *r)
     for (int apart = 0; apart < 2; apart++) {
         q.inp_stride[1] = q.out_stride[1] = r->width + apart;
         igx::Plan p;
-        igx::make_plan(&q, nullptr, p);
+        igx::make_plan(&q, nullptr, nullptr, p);
         if (p.workspace() > most) most = p.workspace();
     }
     return most;
 }
 
-extern "C" int igx_linear_recurrence(const igx_recurrence *r, igx_stream_t stream)
+namespace igx {
+namespace {
+
+int check_rest(const igx_recurrence *r, const igx_recurrence_rest *rest, const char *who)
 {
-    int rc = igx::check(r, __func__);
+    if (!rest) return IGX_OK;
+    if (r->dtype == IGX_F32) return fail(IGX_E_PARAM, "%s: float32 results are not rounded, there is no rest", who);
+    return IGX_OK;
+}
+
+int forward(const igx_recurrence *r, const igx_recurrence_rest *rest, igx_stream_t stream, const char *who)
+{
+    int rc = check(r, who);
+    if (!rc) rc = check_rest(r, rest, who);
     if (rc) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t channels = r->envs * r->width;
     if (channels == 0) return IGX_OK;
-    if (r->steps == 0) return igx::carry_through(r->state, r->last, channels, s, __func__);
-    IGX_REQUIRE_PTR(r->gate, "gate");
-    IGX_REQUIRE_PTR(r->inp, "inp");
-    IGX_REQUIRE_PTR(r->out, "out");
-    igx::Plan p;
-    igx::make_plan(r, nullptr, p);
-    return igx::launch<false>(r, p, s, __func__);
+    if (r->steps == 0) return carry_through(r->state, r->last, channels, s, who);
+    if (!r->gate) return fail(IGX_E_NULL, "%s: gate is NULL", who);
+    if (!r->inp) return fail(IGX_E_NULL, "%s: inp is NULL", who);
+    if (!r->out) return fail(IGX_E_NULL, "%s: out is NULL", who);
+    if (rest && !rest->codes) return fail(IGX_E_NULL, "%s: codes is NULL", who);
+    Plan p;
+    make_plan(r, nullptr, rest, p);
+    return launch<false>(r, p, s, who);
+}
+
+int backward(const igx_recurrence *r, const igx_recurrence_grad *g, const igx_recurrence_rest *rest, igx_stream_t stream,
+             const char *who)
+{
+    int rc = check(r, who);
+    if (!rc) rc = check_rest(r, rest, who);
+    if (rc) return rc;
+    if (!g) return fail(IGX_E_NULL, "%s: g is NULL", who);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t channels = r->envs * r->width;
+    if (channels == 0 || (!g->d_gate && !g->d_inp && !g->d_state)) return IGX_OK;
+    if (r->steps == 0) return carry_through(g->d_last, g->d_state, channels, s, who);
+    if (!r->gate) return fail(IGX_E_NULL, "%s: gate is NULL", who);
+    if (g->d_gate && !r->out) return fail(IGX_E_NULL, "%s: out is NULL", who);
+    if (g->d_gate && rest && !rest->codes) return fail(IGX_E_NULL, "%s: codes is NULL", who);
+    Plan p;
+    make_plan(r, g, rest, p);
+    return launch<true>(r, p, s, who);
+}
+
+}  // namespace
+}  // namespace igx
+
+extern "C" int igx_linear_recurrence(const igx_recurrence *r, igx_stream_t stream)
+{
+    return igx::forward(r, nullptr, stream, __func__);
 }
 
 extern "C" int igx_linear_recurrence_backward(const igx_recurrence *r, const igx_recurrence_grad *g, igx_stream_t stream)
 {
-    int rc = igx::check(r, __func__);
-    if (rc) return rc;
-    IGX_REQUIRE_PTR(g, "g");
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    const int64_t channels = r->envs * r->width;
-    if (channels == 0 || (!g->d_gate && !g->d_inp && !g->d_state)) return IGX_OK;
-    if (r->steps == 0) return igx::carry_through(g->d_last, g->d_state, channels, s, __func__);
-    IGX_REQUIRE_PTR(r->gate, "gate");
-    if (g->d_gate) IGX_REQUIRE_PTR(r->out, "out");
-    igx::Plan p;
-    igx::make_plan(r, g, p);
-    return igx::launch<true>(r, p, s, __func__);
+    return igx::backward(r, g, nullptr, stream, __func__);
+}
+
+extern "C" int igx_linear_recurrence_with_rest(const igx_recurrence *r, const igx_recurrence_rest *rest, igx_stream_t stream)
+{
+    return igx::forward(r, rest, stream, __func__);
+}
+
+extern "C" int igx_linear_recurrence_backward_with_rest(const igx_recurrence *r, const igx_recurrence_grad *g,
+                                                        const igx_recurrence_rest *rest, igx_stream_t stream)
+{
+    return igx::backward(r, g, rest, stream, __func__);
 }

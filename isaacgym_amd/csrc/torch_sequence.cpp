@@ -27,8 +27,8 @@ using OptTensor = std::optional<Tensor>;
 struct Library {
     decltype(&igx_last_error_string) last_error;
     decltype(&igx_linear_recurrence_workspace) recurrence_workspace;
-    decltype(&igx_linear_recurrence) recurrence;
-    decltype(&igx_linear_recurrence_backward) recurrence_backward;
+    decltype(&igx_linear_recurrence_with_rest) recurrence;
+    decltype(&igx_linear_recurrence_backward_with_rest) recurrence_backward;
     decltype(&igx_block_norm_workspace) norm_workspace;
     decltype(&igx_block_norm_forward) norm;
     decltype(&igx_block_norm_backward) norm_backward;
@@ -179,7 +179,14 @@ Tensor recurrence_workspace(igx_recurrence &r, const Tensor &like)
     return ws;
 }
 
-std::pair<Tensor, Tensor> run_recurrence(const Tensor &gate, const Tensor &inp, const Tensor &state, const Tensor &reset, bool reverse)
+igx_recurrence_rest rest_args(const Tensor &rest)
+{
+    return {static_cast<int8_t *>(rest.data_ptr()), {rest.stride(0), rest.stride(1)}};
+}
+
+// (out, last); rest (16-bit types): filled in, in out's layout
+std::pair<Tensor, Tensor> run_recurrence(const Tensor &gate, const Tensor &inp, const Tensor &state, const Tensor &reset, bool reverse,
+                                         Tensor *rest = nullptr)
 {
     igx_recurrence r = recurrence_args(gate, inp, state, reset, reverse);
     rollout(inp, "inp", inp, r.inp, r.inp_stride);
@@ -190,18 +197,22 @@ std::pair<Tensor, Tensor> run_recurrence(const Tensor &gate, const Tensor &inp, 
     rollout(out, "out", inp, r.out, r.out_stride);
     r.last = static_cast<float *>(last.data_ptr());
     const Tensor ws = recurrence_workspace(r, inp);
-    check(lib.recurrence(&r, stream_of(inp)));
+    igx_recurrence_rest kept = {};
+    if (rest) kept = rest_args(*rest = at::empty_like(out, out.options().dtype(at::kChar)));
+    check(lib.recurrence(&r, rest ? &kept : nullptr, stream_of(inp)));
     return {out, last};
 }
 
 struct LinearRecurrence : torch::autograd::Function<LinearRecurrence> {
     static variable_list forward(AutogradContext *ctx, const Tensor &gate, const Tensor &inp, const OptTensor &state_,
-                                 const OptTensor &reset_, bool reverse)
+                                 const OptTensor &reset_, bool reverse, bool unrounded)
     {
         const Tensor state = given(state_), reset = given(reset_);
+        Tensor rest;
+        const bool keep = unrounded && gate.requires_grad() && inp.scalar_type() != at::kFloat;
         ctx->set_materialize_grads(false);
-        auto [out, last] = run_recurrence(gate, inp, state, reset, reverse);
-        ctx->save_for_backward({gate, out, state, reset});
+        auto [out, last] = run_recurrence(gate, inp, state, reset, reverse, keep ? &rest : nullptr);
+        ctx->save_for_backward({gate, out, state, reset, rest});
         ctx->saved_data["reverse"] = reverse;
         return {out, last};
     }
@@ -210,10 +221,10 @@ struct LinearRecurrence : torch::autograd::Function<LinearRecurrence> {
     {
         once(ctx);
         Tensor d_out = grads[0], d_last = grads[1];
-        variable_list result(5);
+        variable_list result(6);
         if (!d_out.defined() && !d_last.defined()) return result;
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &gate = saved[0], &out = saved[1], &state = saved[2], &reset = saved[3];
+        const Tensor &gate = saved[0], &out = saved[1], &state = saved[2], &reset = saved[3], &rest = saved[4];
         c10::DeviceGuard guard(out.device());
         if (d_out.defined() && !adjacent(d_out)) d_out = d_out.contiguous();
         if (d_last.defined()) d_last = d_last.contiguous();
@@ -229,19 +240,21 @@ struct LinearRecurrence : torch::autograd::Function<LinearRecurrence> {
             g.d_state = static_cast<float *>(result[2].data_ptr());
         }
         const Tensor ws = recurrence_workspace(r, out);
-        check(lib.recurrence_backward(&r, &g, stream_of(out)));
+        igx_recurrence_rest kept = {};
+        if (rest.defined()) kept = rest_args(rest);
+        check(lib.recurrence_backward(&r, &g, rest.defined() ? &kept : nullptr, stream_of(out)));
         return result;
     }
 };
 
 std::pair<Tensor, Tensor> linear_recurrence(const Tensor &gate_, const Tensor &inp, const OptTensor &state_, const OptTensor &reset_,
-                                            bool reverse)
+                                            bool reverse, bool unrounded)
 {
     const Tensor gate = gate_.sizes() == inp.sizes() ? gate_ : gate_.expand(inp.sizes());
     const Tensor state = given(state_), reset = given(reset_);
     if (!differentiated({&gate, &inp, &state})) return run_recurrence(gate, inp, state, reset, reverse);
     if (inp.is_cuda()) refuse_foreign_nodes({&gate, &inp, &state}, inp);
-    const variable_list v = LinearRecurrence::apply(gate, inp, maybe(state), maybe(reset), reverse);
+    const variable_list v = LinearRecurrence::apply(gate, inp, maybe(state), maybe(reset), reverse, unrounded);
     return {v[0], v[1]};
 }
 
@@ -281,7 +294,7 @@ Tensor linear_recurrence_step(const Tensor &gate_, const Tensor &inp, const Tens
                       "a written tensor must not overlap another one of the call (state_out may be state)");
     r.out = out.data_ptr();
     r.out_stride[1] = r.width;
-    check(lib.recurrence(&r, stream_of(inp)));
+    check(lib.recurrence(&r, nullptr, stream_of(inp)));
     // a graph that saved what was overwritten has to notice
     torch::autograd::impl::bump_version(to);
     if (out_) torch::autograd::impl::bump_version(out);
@@ -528,8 +541,8 @@ PYBIND11_MODULE(_sequence, m)
         };
         take("igx_last_error_string", lib.last_error);
         take("igx_linear_recurrence_workspace", lib.recurrence_workspace);
-        take("igx_linear_recurrence", lib.recurrence);
-        take("igx_linear_recurrence_backward", lib.recurrence_backward);
+        take("igx_linear_recurrence_with_rest", lib.recurrence);
+        take("igx_linear_recurrence_backward_with_rest", lib.recurrence_backward);
         take("igx_block_norm_workspace", lib.norm_workspace);
         take("igx_block_norm_forward", lib.norm);
         take("igx_block_norm_backward", lib.norm_backward);

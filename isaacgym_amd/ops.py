@@ -757,6 +757,10 @@ def _rollout(t, name, shape, like, written=False):
     if t is None:
         return None, (0, 0)
     _same(t, name, shape, like.dtype, like)
+    return _strided(t, name, shape, written)
+
+
+def _strided(t, name, shape, written=False):
     st, sn, sd = t.stride()
     if sd != 1 and shape[2] > 1:
         raise ValueError("%s: the channels (last dimension) must be adjacent, their stride is %d" % (name, sd))
@@ -791,27 +795,40 @@ def _recurrence(gate, like, state, reset, reverse):
     return r, shape
 
 
-def linear_recurrence(gate, inp, out, state=None, reset=None, last=None, reverse=False):
+def _rest(rest, shape, like):
+    """igx_recurrence_rest of an int8 [T, N, D] tensor with adjacent channels (None: NULL)."""
+    if rest is None:
+        return None
+    _same(rest, "rest", shape, torch.int8, like)
+    q = _abi.RecurrenceRest()
+    q.codes, q.stride = _strided(rest, "rest", shape, written=True)
+    return q
+
+
+def linear_recurrence(gate, inp, out, state=None, reset=None, last=None, reverse=False, rest=None):
     """out[t] = gate[t] * (out before it) + inp[t] over [T, N, D] (igx_linear_recurrence).  gate, inp and out share a type
     and need adjacent channels (gate also one value for all channels of an environment); state and last are fp32 [N, D]
-    (last may be state), reset int64 [T, N].  What is written must not overlap the rest."""
+    (last may be state), reset int64 [T, N].  rest int8 [T, N, D], 16-bit types only: filled with what out's rounding took,
+    for linear_recurrence_backward (igx_linear_recurrence_with_rest).  What is written must not overlap anything else."""
     r, shape = _recurrence(gate, inp, state, reset, reverse)
     r.inp, r.inp_stride = _rollout(inp, "inp", shape, inp)
     if out is None:
         raise TypeError("out: expected a torch.Tensor, got None")
     r.out, r.out_stride = _rollout(out, "out", shape, inp, written=True)
     r.last = _packed(last, "last", shape[1:], torch.float32, inp)
-    _apart((r.out, None if last is state else r.last), (r.gate, r.inp, r.state, r.reset))
+    q = _rest(rest, shape, inp)
+    _apart((r.out, None if last is state else r.last, q and q.codes), (r.gate, r.inp, r.state, r.reset))
     L = _lib.lib()
     ws, r.workspace, r.workspace_bytes = _scratch(L.igx_linear_recurrence_workspace(C.byref(r)), inp.device)
-    _lib.check(_lib._launch(L.igx_linear_recurrence, inp.device, C.byref(r)))
+    _lib.check(_lib._launch(L.igx_linear_recurrence_with_rest, inp.device, C.byref(r), q and C.byref(q)))
     return out
 
 
 def linear_recurrence_backward(gate, out, d_out=None, d_last=None, d_gate=None, d_inp=None, d_state=None, state=None,
-                               reset=None, reverse=False):
+                               reset=None, reverse=False, rest=None):
     """The gradients of linear_recurrence (igx_linear_recurrence_backward): those of d_gate, d_inp [T, N, D] and d_state
-    [N, D] that are given are filled in; d_out and d_last None stand for zeros."""
+    [N, D] that are given are filled in; d_out and d_last None stand for zeros.  rest as linear_recurrence filled it: d_gate
+    from the carried values rather than from out, their rounding."""
     r, shape = _recurrence(gate, out, state, reset, reverse)
     r.out, r.out_stride = _rollout(out, "out", shape, out)
     g = _abi.RecurrenceGrad()
@@ -820,10 +837,11 @@ def linear_recurrence_backward(gate, out, d_out=None, d_last=None, d_gate=None, 
     g.d_inp, g.d_inp_stride = _rollout(d_inp, "d_inp", shape, out, written=True)
     g.d_last = _packed(d_last, "d_last", shape[1:], torch.float32, out)
     g.d_state = _packed(d_state, "d_state", shape[1:], torch.float32, out)
-    _apart((g.d_gate, g.d_inp, g.d_state), (r.gate, r.out, r.state, r.reset, g.d_out, g.d_last))
+    q = _rest(rest, shape, out)
+    _apart((g.d_gate, g.d_inp, g.d_state), (r.gate, r.out, r.state, r.reset, g.d_out, g.d_last, q and q.codes))
     L = _lib.lib()
     ws, r.workspace, r.workspace_bytes = _scratch(L.igx_linear_recurrence_workspace(C.byref(r)), out.device)
-    _lib.check(_lib._launch(L.igx_linear_recurrence_backward, out.device, C.byref(r), C.byref(g)))
+    _lib.check(_lib._launch(L.igx_linear_recurrence_backward_with_rest, out.device, C.byref(r), C.byref(g), q and C.byref(q)))
 
 
 def _row_array(t, name, shape, like):

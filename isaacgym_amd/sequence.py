@@ -25,9 +25,9 @@ import torch
 
 from . import _lib
 
-_BOUND = ("igx_last_error_string", "igx_linear_recurrence_workspace", "igx_linear_recurrence",
-          "igx_linear_recurrence_backward", "igx_block_norm_workspace", "igx_block_norm_forward", "igx_block_norm_backward",
-          "igx_pack8", "igx_unpack8")
+_BOUND = ("igx_last_error_string", "igx_linear_recurrence_workspace", "igx_linear_recurrence_with_rest",
+          "igx_linear_recurrence_backward_with_rest", "igx_block_norm_workspace", "igx_block_norm_forward",
+          "igx_block_norm_backward", "igx_pack8", "igx_unpack8")
 _loaded = None
 
 
@@ -46,7 +46,7 @@ def _native():
     return _loaded
 
 
-def linear_recurrence(gate, inp, state=None, reset=None, reverse=False):
+def linear_recurrence(gate, inp, state=None, reset=None, reverse=False, unrounded=False):
     """out[t] = gate[t] * out[t - 1] + inp[t] over a rollout; returns (out [T, N, D], last [N, D] float32).
 
     gate broadcasts against inp [T, N, D] (same type); both need adjacent channels, any strides otherwise, so a rollout
@@ -56,9 +56,11 @@ def linear_recurrence(gate, inp, state=None, reset=None, reverse=False):
     broadcast its full-size gradient is summed by torch afterwards.
     Steps behind the end of a shorter rollout are padded with gate 1 and input 0: they hand the value through.
 
-    The carried value is float32 whatever the type; `out` is its rounding, and the gradient of gate is computed from
-    `out` as stored.  Products of consecutive gates have to stay within float32's range (gates in [-1, 1] always do)."""
-    return _native().linear_recurrence(gate, inp, state, reset, bool(reverse))
+    The carried value is float32 whatever the type; `out` is its rounding.  The gradient of a 16-bit gate is computed from
+    `out` as stored, which makes its error 1.4 times what its own rounding gives.  unrounded=True: from the carried value,
+    of which 8 bits more are kept beside `out` for the backward pass (a byte an element, written and read once; float32
+    needs none).  Products of consecutive gates have to stay within float32's range (gates in [-1, 1] always do)."""
+    return _native().linear_recurrence(gate, inp, state, reset, bool(reverse), bool(unrounded))
 
 
 def linear_recurrence_step(gate, inp, state, reset=None, state_out=None, out=None):
