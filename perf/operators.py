@@ -204,7 +204,7 @@ def _run_own(s):
         return [out, s["state_out"]]
     if op == "recurrence":
         out, last = sequence.linear_recurrence(s["gate"], s["inp"], state=s["state"], reset=s["reset"],
-                                               reverse=case["reverse"])
+                                               reverse=case["reverse"], unrounded=case["train"])
         if not case["train"]:
             return [out, last]
         grads = torch.autograd.grad((out, last), (s["gate"], s["inp"], s["state"]), (s["d_out"], s["d_last"]))
