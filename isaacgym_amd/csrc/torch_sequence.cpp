@@ -9,6 +9,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <unordered_set>
@@ -83,6 +84,22 @@ bool adjacent(const Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
 
 Tensor given(const OptTensor &t) { return t ? *t : Tensor(); }
 OptTensor maybe(const Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+// What would give a value with nothing to show that its derivative or its computation is missing: the tangent of a
+// forward-mode dual tensor, which does not require grad, and the kernels' part of a traced function, of which only the
+// allocations would be recorded.
+void refuse_traces()
+{
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "the sequence operators cannot be recorded by torch.jit.trace");
+}
+
+void refuse_tangents(std::initializer_list<const Tensor *> tensors)
+{
+    refuse_traces();
+    for (const Tensor *t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
+                                    "the sequence operators have no forward-mode derivatives (a dual tensor was given)");
+}
 
 bool differentiated(std::initializer_list<const Tensor *> tensors)
 {
@@ -252,6 +269,7 @@ std::pair<Tensor, Tensor> linear_recurrence(const Tensor &gate_, const Tensor &i
 {
     const Tensor gate = gate_.sizes() == inp.sizes() ? gate_ : gate_.expand(inp.sizes());
     const Tensor state = given(state_), reset = given(reset_);
+    refuse_tangents({&gate, &inp, &state});
     if (!differentiated({&gate, &inp, &state})) return run_recurrence(gate, inp, state, reset, reverse);
     if (inp.is_cuda()) refuse_foreign_nodes({&gate, &inp, &state}, inp);
     const variable_list v = LinearRecurrence::apply(gate, inp, maybe(state), maybe(reset), reverse, unrounded);
@@ -261,6 +279,7 @@ std::pair<Tensor, Tensor> linear_recurrence(const Tensor &gate_, const Tensor &i
 Tensor linear_recurrence_step(const Tensor &gate_, const Tensor &inp, const Tensor &state, const OptTensor &reset_,
                               const OptTensor &state_out, const OptTensor &out_)
 {
+    refuse_traces();
     TORCH_CHECK_VALUE(inp.dim() == 2, "linear_recurrence_step: gate and inp are [environments, channels] tensors");
     const at::NoGradGuard no_grad;
     const Tensor gate = gate_.sizes() == inp.sizes() ? gate_ : gate_.expand(inp.sizes()), reset = given(reset_);
@@ -491,6 +510,7 @@ std::pair<Tensor, Tensor> block_norm(const Tensor &x, const OptTensor &y_, const
     TORCH_CHECK_VALUE(act >= 0, "activation must be one of 'none', 'sigmoid', 'silu', got '", activation, "'");
     TORCH_CHECK_VALUE(x.dim() >= 1, "x must be a tensor of at least one dimension");
     const Tensor y = given(y_), weight = given(weight_), gate = given(gate_), scale = given(scale_), next_weight = given(next_weight_);
+    refuse_tangents({&x, &y, &weight, &gate, &scale, &next_weight});
     if (!differentiated({&x, &y, &weight, &gate, &scale, &next_weight}))
         return run_norm(x, y, gate, {weight, scale, next_weight}, act, eps, {}, {});
     if (x.is_cuda()) refuse_foreign_nodes({&x, &y, &weight, &gate, &scale, &next_weight}, x);
@@ -502,6 +522,7 @@ std::pair<Tensor, Tensor> block_norm(const Tensor &x, const OptTensor &y_, const
 
 std::pair<Tensor, Tensor> pack8(const Tensor &x)
 {
+    refuse_traces();
     TORCH_CHECK_VALUE(x.dim() >= 1, "x must be a tensor of at least one dimension");
     const at::NoGradGuard no_grad;
     const int e = element(x, "x");
@@ -518,6 +539,7 @@ std::pair<Tensor, Tensor> pack8(const Tensor &x)
 
 Tensor unpack8(const Tensor &codes, const Tensor &scales, const py::object &dtype)
 {
+    refuse_traces();
     TORCH_CHECK_VALUE(codes.dim() >= 1, "codes must be a tensor of at least one dimension");
     TORCH_CHECK_VALUE(codes.is_cuda(), "libigx works on device tensors only (codes is a ", codes.device(), " tensor)");
     TORCH_CHECK_TYPE(THPDtype_Check(dtype.ptr()), "dtype must be a torch.dtype");

@@ -13,10 +13,11 @@ flag, so the operators take `reset_buf` (int64) as it is:
   what their backward pass needs of their inputs in that form.
 
 Element types are float32, float16 and bfloat16; states, statistics, sums and parameters are float32.  There is no CPU
-fallback.  Calls only enqueue work on the current stream and can be captured into a HIP graph, forward and backward
-together; a capture while an eager graph of one of the same leaf tensors is alive is refused, because torch would add
-the captured gradient to the leaf on the eager stream.  `ops.linear_recurrence`, `ops.block_norm`, `ops.pack8` and their
-`_backward` are the same calls on buffers that the caller owns.
+fallback; forward-mode derivatives and torch.jit.trace are refused.  Calls only enqueue work on the current stream and
+can be captured into a HIP graph, forward and backward together; a capture while an eager graph of one of the same leaf
+tensors is alive is refused, because torch would add the captured gradient to the leaf on the eager stream.
+`ops.linear_recurrence`, `ops.block_norm`, `ops.pack8` and their `_backward` are the same calls on buffers that the
+caller owns.
 """
 import ctypes as C
 import importlib

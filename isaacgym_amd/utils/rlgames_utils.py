@@ -119,7 +119,7 @@ def discount_values(fdones, values, rewards, next_values, gamma, tau):
     fdones [T, N]: the reset flags the steps returned (int64; the agents' floats are taken too), the others
     [T, N] or [T, N, D] float32 (one episode end for all D values).  Returns the advantages without gradients."""
     with torch.no_grad():
-        delta = torch.add(rewards, next_values, alpha=float(gamma)).sub_(values)
+        delta = torch.add(rewards, next_values, alpha=float(gamma)).sub_(values).detach()  # of forward-mode tangents, too
         rows = delta if delta.dim() == 3 else delta.unsqueeze(-1)
         gate = torch.full((1, 1, 1), float(gamma) * float(tau), dtype=rows.dtype, device=rows.device)
         done = fdones if fdones.dtype == torch.int64 else (fdones != 0).to(torch.int64)

@@ -1,0 +1,69 @@
+"""The sequence operators under autograd's other modes: what they do not have raises, what they share with torch works."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+from isaacgym_amd import sequence
+from isaacgym_amd.utils.rlgames_utils import discount_values
+from tests.test_gpu_sequence import BF16, DEV, F32, block_inputs, block_pass, rollout
+
+pytestmark = pytest.mark.gpu
+
+
+def test_forward_mode_raises_in_place_of_a_lost_tangent():
+    x, w = torch.randn(6, 2, 24, device=DEV), torch.ones(24, device=DEV)
+    with fwAD.dual_level():
+        d = fwAD.make_dual(x, torch.ones_like(x))
+        for call in (lambda: x + sequence.rms_norm(d, w), lambda: sequence.residual_norm(d, x, w),
+                     lambda: sequence.linear_recurrence(x, d), lambda: sequence.linear_recurrence(d.sigmoid(), x)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            sequence.rms_norm(d, w)
+        # without gradients by its documentation
+        done = torch.zeros(6, 2, dtype=torch.int64, device=DEV)
+        adv = discount_values(done, x, d, x, 0.99, 0.95)
+        assert fwAD.unpack_dual(adv).tangent is None and torch.equal(adv, discount_values(done, x, x, x, 0.99, 0.95))
+    assert torch.isfinite(sequence.rms_norm(x, w)).all()  # and afterwards as before
+
+
+def test_trace_raises_in_place_of_unwritten_memory():
+    x, w = torch.randn(6, 2, 24, device=DEV), torch.ones(24, device=DEV)
+    with pytest.raises(NotImplementedError, match="torch.jit.trace"):
+        torch.jit.trace(lambda t: sequence.rms_norm(t, w), (x,), check_trace=False)
+    with pytest.raises(NotImplementedError, match="torch.jit.trace"):
+        torch.jit.trace(lambda t: sequence.linear_recurrence(t, t)[0], (x,), check_trace=False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_saved_tensor_hooks_see_every_saved_tensor(dtype):
+    """A hook that moves what the graph keeps to host memory and back changes no bit of the gradients."""
+    args = block_inputs(40, 3, 72, dtype)
+    want = block_pass(*args)
+    seen = []
+
+    def pack(t):
+        seen.append(t.dtype)
+        return t.cpu(), t.stride()
+
+    def unpack(kept):
+        t = torch.empty_strided(kept[0].shape, kept[1], dtype=kept[0].dtype, device=DEV)
+        t.copy_(kept[0])
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        got = block_pass(*args)
+    assert torch.int8 in seen and dtype in seen
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+def test_saved_tensor_hooks_see_the_unrounded_part():
+    gate, inp, state, reset, d_out, d_last = (t.to(DEV) for t in rollout(40, 3, 9, BF16, 301, resets=0.1))
+    gate.requires_grad_(True)
+    run = lambda: torch.autograd.grad(sequence.linear_recurrence(gate, inp, state=state, reset=reset, unrounded=True), gate,
+                                      (d_out, d_last))[0]
+    want, kinds = run(), []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (kinds.append(t.dtype), t.clone())[1], lambda t: t):
+        got = run()
+    assert torch.int8 in kinds and torch.equal(want, got)
