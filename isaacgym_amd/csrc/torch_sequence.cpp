@@ -196,8 +196,10 @@ Tensor recurrence_workspace(igx_recurrence &r, const Tensor &like)
     return ws;
 }
 
-igx_recurrence_rest rest_args(const Tensor &rest)
+igx_recurrence_rest rest_args(const Tensor &rest, const Tensor &like)
 {
+    same(rest, "rest", like.sizes(), at::kChar, like);
+    TORCH_CHECK_VALUE(adjacent(rest), "rest: the channels (last dimension) must be adjacent, their stride is ", rest.stride(2));
     return {static_cast<int8_t *>(rest.data_ptr()), {rest.stride(0), rest.stride(1)}};
 }
 
@@ -215,7 +217,7 @@ std::pair<Tensor, Tensor> run_recurrence(const Tensor &gate, const Tensor &inp, 
     r.last = static_cast<float *>(last.data_ptr());
     const Tensor ws = recurrence_workspace(r, inp);
     igx_recurrence_rest kept = {};
-    if (rest) kept = rest_args(*rest = at::empty_like(out, out.options().dtype(at::kChar)));
+    if (rest) kept = rest_args(*rest = at::empty_like(out, out.options().dtype(at::kChar)), out);
     check(lib.recurrence(&r, rest ? &kept : nullptr, stream_of(inp)));
     return {out, last};
 }
@@ -258,7 +260,7 @@ struct LinearRecurrence : torch::autograd::Function<LinearRecurrence> {
         }
         const Tensor ws = recurrence_workspace(r, out);
         igx_recurrence_rest kept = {};
-        if (rest.defined()) kept = rest_args(rest);
+        if (rest.defined()) kept = rest_args(rest, out);
         check(lib.recurrence_backward(&r, &g, rest.defined() ? &kept : nullptr, stream_of(out)));
         return result;
     }
@@ -353,6 +355,18 @@ std::vector<int64_t> scales_shape(const Tensor &t)
     return s;
 }
 
+// 8-bit codes of y (and gate) as a call writes or reads them
+void code_args(igx_block_norm &b, const Tensor *codes, size_t count, const Tensor &like)
+{
+    if (count < 2) return;
+    const std::vector<int64_t> groups = scales_shape(like);
+    b.y8 = packed<int8_t>(codes[0], "y codes", like.sizes(), at::kChar, like);
+    b.y8_scale = packed<float>(codes[1], "y scales", groups, at::kFloat, like);
+    if (count < 4) return;
+    b.gate8 = packed<int8_t>(codes[2], "gate codes", like.sizes(), at::kChar, like);
+    b.gate8_scale = packed<float>(codes[3], "gate scales", groups, at::kFloat, like);
+}
+
 struct Parameters {
     Tensor weight, scale, next_weight;
 };
@@ -370,7 +384,7 @@ igx_block_norm norm_args(const Tensor &like, const Parameters &p, const Tensor &
     b.scale = packed<float>(p.scale, "scale", vector, at::kFloat, like);
     b.next_weight = packed<float>(p.next_weight, "next_weight", vector, at::kFloat, like);
     if (inv_rms.defined() && b.rows) {
-        b.y_inv_rms = static_cast<float *>(inv_rms.data_ptr());
+        b.y_inv_rms = packed<float>(inv_rms, "inv_rms", {2, b.rows}, at::kFloat, like);
         b.out_inv_rms = b.y_inv_rms + b.rows;
     }
     return b;
@@ -390,14 +404,7 @@ std::pair<Tensor, Tensor> run_norm(const Tensor &x, const Tensor &y, const Tenso
     if (p.next_weight.defined()) next = at::empty(x.sizes(), x.options());
     if (out.defined()) b.out = out.data_ptr();
     if (next.defined()) b.next = next.data_ptr();
-    if (codes.size() > 1) {
-        b.y8 = static_cast<int8_t *>(codes[0].data_ptr());
-        b.y8_scale = static_cast<float *>(codes[1].data_ptr());
-    }
-    if (codes.size() > 3) {
-        b.gate8 = static_cast<int8_t *>(codes[2].data_ptr());
-        b.gate8_scale = static_cast<float *>(codes[3].data_ptr());
-    }
+    code_args(b, codes.data(), codes.size(), x);
     check(lib.norm(&b, stream_of(x)));
     return {out, next};
 }
@@ -453,14 +460,9 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         row_array(y, "y", like, b.y, b.y_stride);
         row_array(gate, "gate", like, b.gate, b.gate_stride);
         if (codes) {
-            b.y8 = static_cast<int8_t *>(saved[7].data_ptr());
-            b.y8_scale = static_cast<float *>(saved[8].data_ptr());
-            if (block) b.y = b.y8;  // says that there is a block; not read
-            if (saved.size() > 9) {
-                b.gate8 = static_cast<int8_t *>(saved[9].data_ptr());
-                b.gate8_scale = static_cast<float *>(saved[10].data_ptr());
-                b.gate = b.gate8;
-            }
+            code_args(b, &saved[7], saved.size() - 7, like);
+            if (block) b.y = b.y8;  // they say which parts there are; not read
+            b.gate = b.gate8;
         }
         igx_block_norm_grad g = {};
         row_array(d_out, "d_out", like, g.d_out, g.d_out_stride);

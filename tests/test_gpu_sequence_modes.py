@@ -67,3 +67,28 @@ def test_saved_tensor_hooks_see_the_unrounded_part():
     with torch.autograd.graph.saved_tensors_hooks(lambda t: (kinds.append(t.dtype), t.clone())[1], lambda t: t):
         got = run()
     assert torch.int8 in kinds and torch.equal(want, got)
+
+
+@pytest.mark.parametrize("wrong", [lambda t: t.cpu(), lambda t: t[:1], lambda t: t.to(torch.int16 if t.dtype == torch.int8 else torch.float64)])
+@pytest.mark.parametrize("kind", [torch.int8, F32])
+def test_what_a_hook_hands_back_is_checked(wrong, kind):
+    """A hook that gives the backward pass another device, shape or type gets an error, for the tensors that only the nodes
+    know (codes, their scales, the rows' inverse roots) like for the caller's own."""
+    def back(t):
+        return wrong(t) if t.dtype == kind and t.dim() > 1 else t
+
+    x = torch.randn(40, 130, device=DEV, dtype=BF16)
+    w = torch.ones(130, device=DEV)
+    gate, inp, state, reset, d_out, d_last = (t.to(DEV) for t in rollout(40, 3, 9, BF16, 302, resets=0.1))
+    calls = [lambda: sequence.residual_norm(x, x, w, gate=x, next_weight=w, checkpoint=True), lambda: (sequence.rms_norm(x, w, checkpoint=True),)]
+    if kind == torch.int8:
+        calls.append(lambda: sequence.linear_recurrence(gate, inp, unrounded=True))
+    else:
+        calls.append(lambda: sequence.linear_recurrence(gate, inp, state=state))
+    x.requires_grad_(True)
+    gate.requires_grad_(True)
+    for call in calls:
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+            outs = call()
+        with pytest.raises((ValueError, TypeError, RuntimeError), match="device tensors only|expected shape|expected dtype"):
+            torch.autograd.backward(outs, [torch.ones_like(o) for o in outs])
