@@ -12,6 +12,8 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
+#include <map>
 #include <unordered_set>
 
 #include "../../include/igx.h"
@@ -81,6 +83,87 @@ template <typename T> T *packed(const Tensor &t, const char *name, at::IntArrayR
 }
 
 bool adjacent(const Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
+
+int64_t address(const Tensor &t) { return reinterpret_cast<int64_t>(t.data_ptr()); }
+
+// from a tensor's first byte to behind its last
+int64_t reach(const Tensor &t)
+{
+    const auto sizes = t.sizes(), strides = t.strides();
+    int64_t elements = 1;
+    for (size_t i = 0; i < sizes.size(); i++) elements += (sizes[i] - 1) * strides[i];
+    return elements * (int64_t)t.element_size();
+}
+
+// A tensor's bytes: runs of `run` bytes, one for every index into the dimensions that are left (their sizes and strides).
+struct Bytes {
+    int64_t run;
+    std::vector<std::pair<int64_t, int64_t>> outer;  // (stride in bytes, size)
+    explicit Bytes(const Tensor &t) : run(t.element_size())
+    {
+        for (int64_t i = 0; i < t.dim(); i++)
+            if (t.size(i) > 1 && t.stride(i) != 0) outer.emplace_back(t.stride(i) * t.element_size(), t.size(i));
+        std::sort(outer.begin(), outer.end());
+        size_t kept = 0;
+        for (const auto &d : outer) {
+            if (d.first <= run) run += d.first * (d.second - 1);
+            else outer[kept++] = d;
+        }
+        outer.resize(kept);
+    }
+};
+
+// Is there a solution with d + sum of c[k].stride * x[k] inside (low, high), low[k] <= x[k] <= high[k]?  Strides in falling
+// order, so that what the smaller ones reach leaves few candidates for each; should a call need more than `budget` steps
+// after all, the answer is yes.
+struct Term {
+    int64_t stride, low, high;
+};
+
+bool solvable(const std::vector<Term> &c, size_t k, int64_t d, int64_t low, int64_t high, int64_t &budget)
+{
+    if (--budget < 0) return true;
+    if (k == c.size()) return low < d && d < high;
+    int64_t least = 0, most = 0;  // of the terms behind this one
+    for (size_t j = k + 1; j < c.size(); j++) {
+        least += c[j].stride * c[j].low;
+        most += c[j].stride * c[j].high;
+    }
+    auto below = [](int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); };
+    // low - d - most < stride x < high - d - least
+    const int64_t s = c[k].stride, from = std::max(c[k].low, below(low - d - most, s) + 1), to = std::min(c[k].high, below(high - d - least - 1, s));
+    for (int64_t x = from; x <= to; x++)
+        if (solvable(c, k + 1, d + s * x, low, high, budget)) return true;
+    return false;
+}
+
+// do two tensors share a byte?  Exact, also for views that lie between each other's rows or steps.
+bool overlap(const Tensor &a, const Tensor &b)
+{
+    if (!a.defined() || !b.defined() || !a.numel() || !b.numel()) return false;
+    const int64_t at = address(a), to = address(b);
+    if (at + reach(a) <= to || to + reach(b) <= at) return false;
+    const Bytes p(a), q(b);
+    if (p.outer.empty() && q.outer.empty()) return true;
+    std::map<int64_t, Term, std::greater<int64_t>> terms;  // of q's run less p's
+    for (const auto &d : p.outer) terms.emplace(d.first, Term{d.first, 0, 0}).first->second.low -= d.second - 1;
+    for (const auto &d : q.outer) terms.emplace(d.first, Term{d.first, 0, 0}).first->second.high += d.second - 1;
+    std::vector<Term> c;
+    for (const auto &t : terms) c.push_back(t.second);
+    int64_t budget = 1 << 18;
+    return solvable(c, 0, to - at, -q.run, p.run, budget);
+}
+
+// no tensor that a call writes shares memory with one that it reads, or with another one that it writes
+template <typename List> void apart(const List &written, const List &read)
+{
+    for (auto w = std::begin(written); w != std::end(written); ++w) {
+        for (const auto &r : read)
+            TORCH_CHECK_VALUE(!overlap(*w, r), "a written tensor must not overlap another one of the call");
+        for (auto v = std::begin(written); v != w; ++v)
+            TORCH_CHECK_VALUE(!overlap(*w, *v), "a written tensor must not overlap another one of the call");
+    }
+}
 
 Tensor given(const OptTensor &t) { return t ? *t : Tensor(); }
 OptTensor maybe(const Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
@@ -310,9 +393,15 @@ Tensor linear_recurrence_step(const Tensor &gate_, const Tensor &inp, const Tens
     c10::DeviceGuard guard(inp.device());
     const Tensor out = out_ ? *out_ : at::empty(inp.sizes(), inp.options());
     packed<char>(out, "out", inp.sizes(), inp.scalar_type(), inp);
-    auto apart = [&](const void *p) { return p != r.gate && p != r.inp; };
-    TORCH_CHECK_VALUE(!out.numel() || (apart(out.data_ptr()) && apart(r.last) && out.data_ptr() != r.state && out.data_ptr() != r.last),
-                      "a written tensor must not overlap another one of the call (state_out may be state)");
+    // state_out may be state: a lane has read its channels before it writes them
+    const bool in_place = r.last == r.state;
+    if (out_ || !in_place) {
+        const std::initializer_list<Tensor> written = {to, out}, read = {gate, inp, reset, in_place ? Tensor() : state};
+        apart(written, read);
+    } else {
+        const std::initializer_list<Tensor> written = {to}, read = {gate, inp, reset};
+        apart(written, read);
+    }
     r.out = out.data_ptr();
     r.out_stride[1] = r.width;
     check(lib.recurrence(&r, nullptr, stream_of(inp)));
@@ -584,6 +673,13 @@ PYBIND11_MODULE(_sequence, m)
                 PyErr_SetObject(error_class->ptr(), value.ptr());
             }
         });
+    });
+    m.def("overlap", &overlap);
+    m.def("apart", [](const std::vector<OptTensor> &written, const std::vector<OptTensor> &read) {
+        std::vector<Tensor> w, r;
+        for (const auto &t : written) w.push_back(given(t));
+        for (const auto &t : read) r.push_back(given(t));
+        apart(w, r);
     });
     m.def("linear_recurrence", &linear_recurrence);
     m.def("linear_recurrence_step", &linear_recurrence_step);

@@ -7,7 +7,7 @@ import ctypes as C
 
 import torch
 
-from . import _abi, _lib
+from . import _abi, _lib, sequence
 
 
 def cartpole_step(params, tensors, n_envs, cache=None):
@@ -689,7 +689,7 @@ class WindowQuantile:
         return False
 
 
-# ---- sequence operators (isaacgym_amd.sequence differentiates through them) ----------------------
+# ---- sequence operators: isaacgym_amd.sequence's calls on buffers that the caller owns ------------
 _ELEMENTS = {torch.float32: _abi.IGX_F32, torch.float16: _abi.IGX_F16, torch.bfloat16: _abi.IGX_BF16}
 _ACTIVATIONS = {"none": _abi.IGX_GATE_NONE, "sigmoid": _abi.IGX_GATE_SIGMOID, "silu": _abi.IGX_GATE_SILU}
 _GROUP = _abi.IGX_PACK8_GROUP
@@ -743,12 +743,8 @@ def _scratch(size, device):
 
 
 def _apart(written, read):
-    """No buffer that a call writes is one that it reads (or writes twice)."""
-    seen = {p for p in read if p}
-    for p in written:
-        if p and p in seen:
-            raise ValueError("a written tensor must not overlap another one of the call")
-        seen.add(p)
+    """Refuses a call in which a tensor that is written shares memory with one that is read or written (None: not there)."""
+    sequence._native().apart(written, read)
 
 
 def _rollout(t, name, shape, like, written=False):
@@ -817,7 +813,8 @@ def linear_recurrence(gate, inp, out, state=None, reset=None, last=None, reverse
     r.out, r.out_stride = _rollout(out, "out", shape, inp, written=True)
     r.last = _packed(last, "last", shape[1:], torch.float32, inp)
     q = _rest(rest, shape, inp)
-    _apart((r.out, None if last is state else r.last, q and q.codes), (r.gate, r.inp, r.state, r.reset))
+    in_place = last is not None and r.last == r.state
+    _apart((out, last, rest), (gate, inp, None if in_place else state, reset))
     L = _lib.lib()
     ws, r.workspace, r.workspace_bytes = _scratch(L.igx_linear_recurrence_workspace(C.byref(r)), inp.device)
     _lib.check(_lib._launch(L.igx_linear_recurrence_with_rest, inp.device, C.byref(r), q and C.byref(q)))
@@ -838,7 +835,7 @@ def linear_recurrence_backward(gate, out, d_out=None, d_last=None, d_gate=None, 
     g.d_last = _packed(d_last, "d_last", shape[1:], torch.float32, out)
     g.d_state = _packed(d_state, "d_state", shape[1:], torch.float32, out)
     q = _rest(rest, shape, out)
-    _apart((g.d_gate, g.d_inp, g.d_state), (r.gate, r.out, r.state, r.reset, g.d_out, g.d_last, q and q.codes))
+    _apart((d_gate, d_inp, d_state), (gate, out, state, reset, d_out, d_last, rest))
     L = _lib.lib()
     ws, r.workspace, r.workspace_bytes = _scratch(L.igx_linear_recurrence_workspace(C.byref(r)), out.device)
     _lib.check(_lib._launch(L.igx_linear_recurrence_backward_with_rest, out.device, C.byref(r), C.byref(g), q and C.byref(q)))
@@ -906,8 +903,7 @@ def block_norm(x, y=None, weight=None, gate=None, scale=None, next_weight=None, 
     b.gate, b.gate_stride = _row_array(gate, "gate", shape, x)
     b.out = _packed(out, "out", shape, x.dtype, x)
     b.next = _packed(next, "next", shape, x.dtype, x)
-    _apart((b.out, b.next, b.y_inv_rms, b.y8, b.y8_scale, b.gate8, b.gate8_scale),
-           (b.x, b.y, b.gate, b.weight, b.scale, b.next_weight))
+    _apart((out, next, inv_rms, *(codes or ())), (x, y, gate, weight, scale, next_weight))
     _lib.check(_lib._launch(_lib.lib().igx_block_norm_forward, x.device, C.byref(b)))
 
 
@@ -934,8 +930,8 @@ def block_norm_backward(like, x=None, y=None, weight=None, gate=None, scale=None
     g.d_weight = _packed(d_weight, "d_weight", vector, f, like)
     g.d_scale = _packed(d_scale, "d_scale", vector, f, like)
     g.d_next_weight = _packed(d_next_weight, "d_next_weight", vector, f, like)
-    _apart((g.d_x, g.d_y, g.d_gate, g.d_weight, g.d_scale, g.d_next_weight),
-           (b.x, b.y, b.gate, b.weight, b.scale, b.next_weight, b.y_inv_rms, b.y8_scale, b.gate8_scale, g.d_out, g.d_next))
+    _apart((d_x, d_y, d_gate, d_weight, d_scale, d_next_weight),
+           (x, *(codes or (y, gate)), weight, scale, next_weight, inv_rms, d_out, d_next))
     L = _lib.lib()
     if d_weight is not None or d_scale is not None or d_next_weight is not None:
         ws, g.workspace, g.workspace_bytes = _scratch(L.igx_block_norm_workspace(C.byref(b)), like.device)
@@ -948,6 +944,7 @@ def pack8(x, codes, scales):
     p, stride = _row_array(x, "x", x.shape, x)
     q = _packed(codes, "codes", x.shape, torch.int8, x)
     s = _packed(scales, "scales", scales_shape, torch.float32, x)
+    _apart((codes, scales), (x,))
     _lib.check(_lib._launch(_lib.lib().igx_pack8, x.device, p, e, rows, width, stride, q, s))
 
 
@@ -957,4 +954,5 @@ def unpack8(codes, scales, out):
     q = _packed(codes, "codes", out.shape, torch.int8, out)
     s = _packed(scales, "scales", scales_shape, torch.float32, out)
     o = _packed(out, "out", out.shape, out.dtype, out)
+    _apart((out,), (codes, scales))
     _lib.check(_lib._launch(_lib.lib().igx_unpack8, out.device, q, s, e, rows, width, o))
