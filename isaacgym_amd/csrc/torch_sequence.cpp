@@ -404,10 +404,11 @@ Tensor linear_recurrence_step(const Tensor &gate_, const Tensor &inp, const Tens
     }
     r.out = out.data_ptr();
     r.out_stride[1] = r.width;
-    check(lib.recurrence(&r, nullptr, stream_of(inp)));
-    // a graph that saved what was overwritten has to notice
-    torch::autograd::impl::bump_version(to);
+    // A graph that saved what is overwritten has to notice.  Before the launch, for outside inference mode a tensor that was
+    // made in it is refused here: the step must not have been taken then.
     if (out_) torch::autograd::impl::bump_version(out);
+    torch::autograd::impl::bump_version(to);
+    check(lib.recurrence(&r, nullptr, stream_of(inp)));
     return out;
 }
 

@@ -92,3 +92,29 @@ def test_what_a_hook_hands_back_is_checked(wrong, kind):
             outs = call()
         with pytest.raises((ValueError, TypeError, RuntimeError), match="device tensors only|expected shape|expected dtype"):
             torch.autograd.backward(outs, [torch.ones_like(o) for o in outs])
+
+
+def test_a_step_that_is_refused_has_not_been_taken():
+    """A state that was made in inference mode may be advanced there, not outside; refused, it still holds its values."""
+    gate, inp, start, reset, _, _ = (t.to(DEV) for t in rollout(1, 5, 12, F32, 303, resets=0.2))
+    want = start.clone()
+    out = sequence.linear_recurrence_step(gate[0], inp[0], want, reset=reset[0])
+    with torch.inference_mode():
+        state, to, result = start.clone(), torch.full_like(start, 7.0), torch.full_like(start, 7.0)
+        inner = start.clone()
+        assert torch.equal(sequence.linear_recurrence_step(gate[0], inp[0], inner, reset=reset[0]), out) and torch.equal(inner, want)
+    for kw in (dict(), dict(state_out=to), dict(out=result), dict(state_out=to, out=torch.empty_like(start)),
+               dict(state_out=torch.empty_like(start), out=result)):
+        given = start.clone() if kw else state
+        kept = given.clone()
+        with pytest.raises(RuntimeError, match="inference tensor"):
+            sequence.linear_recurrence_step(gate[0], inp[0], given, reset=reset[0], **kw)
+        assert torch.equal(given, kept) and (to == 7).all() and (result == 7).all()
+    with torch.inference_mode():
+        sequence.linear_recurrence_step(gate[0], inp[0], state, reset=reset[0])
+    assert torch.equal(state, want)
+    # the other operators read inference tensors, and write none of them
+    with torch.inference_mode():
+        x, w = torch.randn(4, 24, device=DEV), torch.ones(24, device=DEV)
+        inside = sequence.rms_norm(x, w)
+    assert torch.equal(sequence.rms_norm(x, w), inside)
