@@ -116,15 +116,20 @@ def discount_values(fdones, values, rewards, next_values, gamma, tau):
     """Advantages of a rollout as the agent's discount_values computes them, step by step from the last one:
         delta = rewards + gamma * next_values - values,  adv[t] = delta[t] + gamma * tau * (1 - fdones[t]) * adv[t + 1]
     - the reversed linear recurrence with one gate for everything (one launch instead of a Python loop over the horizon).
-    fdones [T, N]: the reset flags the steps returned (int64; the agents' floats are taken too), the others
-    [T, N] or [T, N, D] float32 (one episode end for all D values).  Returns the advantages without gradients."""
+    fdones [T, N] or [T, N, 1]: the reset flags the steps returned (int64; the agents' floats are taken too), the others
+    [T, N] or [T, N, D] float32 in any layout (one episode end for all D values).  Returns the advantages without
+    gradients."""
     with torch.no_grad():
         delta = torch.add(rewards, next_values, alpha=float(gamma)).sub_(values).detach()  # of forward-mode tangents, too
         rows = delta if delta.dim() == 3 else delta.unsqueeze(-1)
+        if rows.shape[-1] > 1 and rows.stride(-1) != 1:  # laid out as its inputs are: the recurrence needs adjacent channels
+            rows = rows.contiguous()
         gate = torch.full((1, 1, 1), float(gamma) * float(tau), dtype=rows.dtype, device=rows.device)
         done = fdones if fdones.dtype == torch.int64 else (fdones != 0).to(torch.int64)
+        if done.dim() == 3 and done.shape[-1] == 1:
+            done = done.squeeze(-1)
         adv, _ = sequence.linear_recurrence(gate, rows, reset=done, reverse=True)
-        return adv.view(delta.shape)
+        return adv.reshape(delta.shape)
 
 
 class RLGPUAlgoObserver:
