@@ -395,31 +395,23 @@ __global__ __launch_bounds__(kRecBlock) void recurrence_kernel(RecArgs a)
     store_end<V>(a, l, h);
 }
 
-// V floats of each of a workgroup's lanes, as 16-byte columns without bank conflicts
+// V floats (4 or 1) of each of a workgroup's lanes
 template <int V, int LANES> struct Exchange {
-    static constexpr int Q = V >= 4 ? V / 4 : 1, W = V >= 4 ? 4 : V;
-    typedef typename Pack<float, W>::type Word __attribute__((aligned(4 * W)));
-    Word w[Q][LANES];
+    typedef typename Pack<float, V>::type Word __attribute__((aligned(4 * V)));
+    Word w[LANES];
     __device__ __forceinline__ void put(int lane, const float (&f)[V])
     {
-        if constexpr (V == 1) {
-            w[0][lane] = f[0];
-        } else {
-#pragma unroll
-            for (int q = 0; q < Q; q++) w[q][lane] = {f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]};
-        }
+        if constexpr (V == 1) w[lane] = f[0];
+        else w[lane] = {f[0], f[1], f[2], f[3]};
     }
     __device__ __forceinline__ void get(int lane, float (&f)[V]) const
     {
+        const Word x = w[lane];
         if constexpr (V == 1) {
-            f[0] = w[0][lane];
+            f[0] = x;
         } else {
 #pragma unroll
-            for (int q = 0; q < Q; q++) {
-                const Word x = w[q][lane];
-#pragma unroll
-                for (int i = 0; i < 4; i++) f[4 * q + i] = x[i];
-            }
+            for (int i = 0; i < V; i++) f[i] = x[i];
         }
     }
 };
@@ -614,21 +606,27 @@ struct Plan {
     int64_t workspace() const { return spans > 1 ? (1 + 2 * spans) * a.vectors * vec * (int64_t)sizeof(float) : 0; }
 };
 
+// Lanes that share the time hold 4 channels or 1, a lane that walks alone holds 16 bytes or 1 channel: the other kernels are
+// not there.
 template <typename T, int V, int FL, bool BACKWARD> void launch_as(const Plan &p, hipStream_t s)
 {
+    constexpr bool kAlone = V == 1 || V * sizeof(T) == 16, kShared = V <= 4;
     const dim3 block(kRecBlock);
     const uint32_t v = p.a.vectors;
-    if (p.spans > 1)
-        recurrence_spans_kernel<T, V, FL, BACKWARD><<<dim3((unsigned)ceil_div(v, kRecBlock / 16), (unsigned)p.spans), block, 0, s>>>(p.a);
-    if (p.seg == 1) {
-        const dim3 grid((unsigned)ceil_div(v, kRecBlock));
-        if constexpr (sizeof(T) == 2) {
-            if (p.a.rest) return recurrence_kernel<T, V, FL, BACKWARD, true><<<grid, block, 0, s>>>(p.a);
+    if constexpr (kAlone) {
+        if (p.seg == 1) {
+            const dim3 grid((unsigned)ceil_div(v, kRecBlock));
+            if constexpr (sizeof(T) == 2) {
+                if (p.a.rest) return recurrence_kernel<T, V, FL, BACKWARD, true><<<grid, block, 0, s>>>(p.a);
+            }
+            return recurrence_kernel<T, V, FL, BACKWARD, false><<<grid, block, 0, s>>>(p.a);
         }
-        recurrence_kernel<T, V, FL, BACKWARD, false><<<grid, block, 0, s>>>(p.a);
-    } else if (p.seg == 4) {
-        recurrence_split_kernel<T, V, FL, BACKWARD, 4><<<dim3((unsigned)ceil_div(v, lanes_of(4))), block, 0, s>>>(p.a);
-    } else {
+    }
+    if constexpr (kShared) {
+        if (p.spans > 1)
+            recurrence_spans_kernel<T, V, FL, BACKWARD><<<dim3((unsigned)ceil_div(v, kRecBlock / 16), (unsigned)p.spans), block, 0, s>>>(p.a);
+        if (p.seg == 4)
+            return recurrence_split_kernel<T, V, FL, BACKWARD, 4><<<dim3((unsigned)ceil_div(v, lanes_of(4))), block, 0, s>>>(p.a);
         const dim3 grid((unsigned)ceil_div(v, lanes_of(16)), (unsigned)p.spans);
         if constexpr (FL <= kOneFlag) {
             if (p.seg == 64) return recurrence_split_kernel<T, V, FL, BACKWARD, 64><<<grid, dim3(lanes_of(64) * 64), 0, s>>>(p.a);
