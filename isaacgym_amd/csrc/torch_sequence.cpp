@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <map>
+#include <numeric>
 #include <unordered_set>
 
 #include "../../include/igx.h"
@@ -414,15 +415,12 @@ Tensor linear_recurrence_step(const Tensor &gate_, const Tensor &inp, const Tens
 
 // ---- block norms ---------------------------------------------------------------------------------------------------
 
-// the address of a [..., width] tensor with adjacent columns and evenly spaced rows, and the stride from row to row
-template <typename P> void row_array(const Tensor &t, const char *name, const Tensor &like, P &address, int64_t &stride)
+// Are the rows (all but the last dimension) of a [..., width] tensor evenly spaced in the order of its dimensions?  Then
+// `stride` is the distance from row to row.
+bool even_rows(const Tensor &t, int64_t &stride)
 {
-    if (!t.defined()) return;
-    same(t, name, like.sizes(), like.scalar_type(), like);
-    address = t.data_ptr();
-    stride = like.size(-1);
-    if (t.is_contiguous()) return;
-    TORCH_CHECK_VALUE(adjacent(t), name, ": the columns (last dimension) must be adjacent, their stride is ", t.stride(-1));
+    stride = t.size(-1);
+    if (t.is_contiguous()) return true;
     int64_t reach = 0;  // rows between two entries of the dimension in front; 0 as long as there is one row
     for (int64_t i = t.dim() - 2; i >= 0; i--) {
         if (t.size(i) == 1) continue;
@@ -430,10 +428,41 @@ template <typename P> void row_array(const Tensor &t, const char *name, const Te
             stride = t.stride(i);
             reach = t.size(i);
         } else {
-            TORCH_CHECK_VALUE(t.stride(i) == stride * reach, name, ": its rows (all but the last dimension) must be evenly spaced");
+            if (t.stride(i) != stride * reach) return false;
             reach *= t.size(i);
         }
     }
+    return true;
+}
+
+// the address of a [..., width] tensor with adjacent columns and evenly spaced rows, and the stride from row to row
+template <typename P> void row_array(const Tensor &t, const char *name, const Tensor &like, P &address, int64_t &stride)
+{
+    if (!t.defined()) return;
+    same(t, name, like.sizes(), like.scalar_type(), like);
+    address = t.data_ptr();
+    TORCH_CHECK_VALUE(t.is_contiguous() || adjacent(t), name, ": the columns (last dimension) must be adjacent, their stride is ", t.stride(-1));
+    TORCH_CHECK_VALUE(even_rows(t, stride), name, ": its rows (all but the last dimension) must be evenly spaced, in one order for the whole call");
+}
+
+// Rows do not know of each other, so any order will do that suits x, y and gate alike.  The order of their dimensions in
+// which all of them have evenly spaced rows; empty where that is the one they have, or where there is none.
+std::vector<int64_t> row_order(const Tensor &x, const Tensor &y, const Tensor &gate)
+{
+    int64_t stride;
+    const Tensor *odd = nullptr;
+    for (const Tensor *t : {&gate, &y, &x})
+        if (t->defined() && t->dim() > 0 && !even_rows(*t, stride)) odd = t;
+    if (!odd) return {};
+    if (y.defined()) same(y, "y", x.sizes(), x.scalar_type(), x);
+    if (gate.defined()) same(gate, "gate", x.sizes(), x.scalar_type(), x);
+    std::vector<int64_t> order(x.dim());
+    std::iota(order.begin(), order.end(), 0);
+    std::stable_sort(order.begin(), order.end() - 1, [&](int64_t i, int64_t j) { return odd->stride(i) > odd->stride(j); });
+    const at::NoGradGuard no_grad;
+    for (const Tensor *t : {&x, &y, &gate})
+        if (t->defined() && !even_rows(t->permute(order), stride)) return {};
+    return order;
 }
 
 int64_t rows_of(const Tensor &t) { return t.size(-1) ? t.numel() / t.size(-1) : 0; }
@@ -499,7 +528,7 @@ std::pair<Tensor, Tensor> run_norm(const Tensor &x, const Tensor &y, const Tenso
     return {out, next};
 }
 
-Tensor even_rows(const Tensor &t) { return !t.defined() || t.is_contiguous() ? t : t.contiguous(); }
+Tensor packed_rows(const Tensor &t) { return !t.defined() || t.is_contiguous() ? t : t.contiguous(); }
 
 struct BlockNorm : torch::autograd::Function<BlockNorm> {
     static variable_list forward(AutogradContext *ctx, const Tensor &x, const OptTensor &y_, const OptTensor &weight_,
@@ -541,7 +570,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         const Parameters p = {saved[3], saved[4], saved[5]};
         const bool block = p.weight.defined(), behind = p.next_weight.defined(), codes = saved.size() > 7;
         const Tensor given_out = block ? grads[0] : Tensor();
-        const Tensor d_out = even_rows(given_out), d_next = even_rows(behind ? grads.back() : Tensor());
+        const Tensor d_out = packed_rows(given_out), d_next = packed_rows(behind ? grads.back() : Tensor());
         if (!d_out.defined() && !d_next.defined()) return result;
         const Tensor &like = d_out.defined() ? d_out : d_next;
         c10::DeviceGuard guard(like.device());
@@ -594,6 +623,16 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
     }
 };
 
+std::pair<Tensor, Tensor> block_norm_of(const Tensor &x, const Tensor &y, const Tensor &gate, const Parameters &p, int64_t act, double eps,
+                                        bool checkpoint)
+{
+    const std::initializer_list<const Tensor *> inputs = {&x, &y, &p.weight, &gate, &p.scale, &p.next_weight};
+    if (!differentiated(inputs)) return run_norm(x, y, gate, p, act, eps, {}, {});
+    if (x.is_cuda()) refuse_foreign_nodes(inputs, x);
+    const variable_list v = BlockNorm::apply(x, maybe(y), maybe(p.weight), maybe(gate), maybe(p.scale), maybe(p.next_weight), act, eps, checkpoint);
+    return {y.defined() ? v[0] : Tensor(), p.next_weight.defined() ? v.back() : Tensor()};
+}
+
 std::pair<Tensor, Tensor> block_norm(const Tensor &x, const OptTensor &y_, const OptTensor &weight_, const OptTensor &gate_,
                                      const OptTensor &scale_, const OptTensor &next_weight_, const std::string &activation, double eps,
                                      bool checkpoint)
@@ -601,13 +640,17 @@ std::pair<Tensor, Tensor> block_norm(const Tensor &x, const OptTensor &y_, const
     const int64_t act = activation == "silu" ? IGX_GATE_SILU : activation == "sigmoid" ? IGX_GATE_SIGMOID : activation == "none" ? IGX_GATE_NONE : -1;
     TORCH_CHECK_VALUE(act >= 0, "activation must be one of 'none', 'sigmoid', 'silu', got '", activation, "'");
     TORCH_CHECK_VALUE(x.dim() >= 1, "x must be a tensor of at least one dimension");
-    const Tensor y = given(y_), weight = given(weight_), gate = given(gate_), scale = given(scale_), next_weight = given(next_weight_);
-    refuse_tangents({&x, &y, &weight, &gate, &scale, &next_weight});
-    if (!differentiated({&x, &y, &weight, &gate, &scale, &next_weight}))
-        return run_norm(x, y, gate, {weight, scale, next_weight}, act, eps, {}, {});
-    if (x.is_cuda()) refuse_foreign_nodes({&x, &y, &weight, &gate, &scale, &next_weight}, x);
-    const variable_list v = BlockNorm::apply(x, maybe(y), maybe(weight), maybe(gate), maybe(scale), maybe(next_weight), act, eps, checkpoint);
-    return {y.defined() ? v[0] : Tensor(), next_weight.defined() ? v.back() : Tensor()};
+    const Tensor y = given(y_), gate = given(gate_);
+    const Parameters p = {given(weight_), given(scale_), given(next_weight_)};
+    refuse_tangents({&x, &y, &p.weight, &gate, &p.scale, &p.next_weight});
+    const std::vector<int64_t> order = row_order(x, y, gate);
+    if (order.empty()) return block_norm_of(x, y, gate, p, act, eps, checkpoint);
+    // a rollout kept environment by environment, for one: its rows in the order they are stored, the results laid out like it
+    auto turned = [&](const Tensor &t) { return t.defined() ? t.permute(order) : t; };
+    std::vector<int64_t> back(order.size());
+    for (size_t i = 0; i < order.size(); i++) back[order[i]] = i;
+    const auto [out, next] = block_norm_of(turned(x), turned(y), turned(gate), p, act, eps, checkpoint);
+    return {out.defined() ? out.permute(back) : out, next.defined() ? next.permute(back) : next};
 }
 
 // ---- 8-bit checkpoints ----------------------------------------------------------------------------------------------

@@ -74,7 +74,8 @@ def linear_recurrence_step(gate, inp, state, reset=None, state_out=None, out=Non
 def rms_norm(x, weight, eps=1e-5, checkpoint=False):
     """x / sqrt(mean(x^2) + eps) * weight over the last dimension (at most 8192 wide): the norm in front of a block.
 
-    x [..., D] float32 / float16 / bfloat16 with evenly spaced rows, weight [D] float32.  checkpoint=True: the backward
+    x [..., D] float32 / float16 / bfloat16 with adjacent columns and rows that are evenly spaced in some order of their
+    dimensions (a transposed rollout is fine, and its result is laid out like it), weight [D] float32.  checkpoint=True: the backward
     pass sees x through its 8-bit codes (`pack8`), and x itself need not be kept for it."""
     return _native().block_norm(x, None, None, None, None, weight, "none", float(eps), bool(checkpoint))[1]
 
@@ -83,11 +84,12 @@ def residual_norm(x, y, weight, gate=None, scale=None, next_weight=None, activat
     """out = x + scale * act(gate) * (rms(y) * weight) behind a block with output y on the residual stream x; with
     next_weight returns (out, rms(out) * next_weight), the norm in front of the next block, from the same pass.
 
-    x, y, gate [..., D] of one shape and type with evenly spaced rows; weight, scale, next_weight [D] float32;
-    activation of the gate: "silu", "sigmoid" or "none".  Differentiable (once) in all of them.  checkpoint=True: y and
-    gate are kept for the backward pass as 8-bit codes (`pack8`) and the gradients are those at the values the codes stand
-    for; x is kept as it is.  There a gate counts as >= -16 with "silu" and within +-16 with "sigmoid", so that one that
-    is shut by a very low value leaves the other 63 of its group their precision."""
+    x, y, gate [..., D] of one shape and type, their rows evenly spaced in one order of the dimensions that all three
+    share and in which the results are laid out; weight, scale, next_weight [D] float32; activation of the gate: "silu",
+    "sigmoid" or "none".  Differentiable (once) in all of them.  checkpoint=True: y and gate are kept for the backward pass
+    as 8-bit codes (`pack8`) and the gradients are those at the values the codes stand for; x is kept as it is.  There a
+    gate counts as >= -16 with "silu" and within +-16 with "sigmoid", so that one that is shut by a very low value leaves
+    the other 63 of its group their precision."""
     out, after = _native().block_norm(x, y, weight, gate, scale, next_weight, activation, float(eps), bool(checkpoint))
     return out if next_weight is None else (out, after)
 

@@ -1,0 +1,87 @@
+"""The norms on rollouts whose rows are not stored in the order of their dimensions."""
+import pytest
+import torch
+
+from isaacgym_amd import sequence
+from tests import seq_cases as S
+from tests.test_gpu_sequence import BF16, DEV, F32, block_inputs, block_pass, norm_inputs
+
+pytestmark = pytest.mark.gpu
+
+
+def run(t, heads, activation, checkpoint):
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items() if v is not None}
+    outs = sequence.residual_norm(**leaves, activation=activation, checkpoint=checkpoint)
+    grads = torch.autograd.grad(outs, list(leaves.values()), heads)
+    x = t["x"].detach().requires_grad_(True)
+    w = t["next_weight"].detach().requires_grad_(True)
+    alone = sequence.rms_norm(x, w, checkpoint=checkpoint)
+    return [*outs, alone], [*grads, *torch.autograd.grad(alone, (x, w), heads[1])]
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("sizes,order", [((6, 7), (1, 0)), ((40, 300), (1, 0)), ((3, 4, 5), (2, 0, 1)), ((3, 4, 5), (1, 2, 0)), ((3, 1, 5), (2, 1, 0)),
+                                         ((2, 3, 4, 5), (3, 1, 0, 2))])
+def test_any_order_is_the_call_on_the_rows_as_they_are_stored(sizes, order, dtype, checkpoint):
+    D = 70
+    R = torch.Size(sizes).numel()
+    t, do, dn = norm_inputs(R, D, dtype, 701, spread=False)
+    t = {k: v.to(DEV) for k, v in t.items()}
+    stored = [sizes[i] for i in order]
+    back = [order.index(i) for i in range(len(order))] + [len(order)]
+
+    def place(v):  # [R, D] as it is stored -> the tensor with those rows
+        return v.view(*stored, D).permute(back) if v.dim() == 2 else v
+
+    flat = run(t, (do.to(DEV), dn.to(DEV)), "sigmoid", checkpoint)
+    for heads in ((place(do.to(DEV)), place(dn.to(DEV))), (place(do.to(DEV)).contiguous(), place(dn.to(DEV)).contiguous())):
+        turned = run({k: place(v) for k, v in t.items()}, heads, "sigmoid", checkpoint)
+        for a, b in zip(flat[0] + flat[1], turned[0] + turned[1]):
+            assert torch.equal(place(a), b)
+        for out in turned[0]:
+            assert out.shape == (*sizes, D)  # and laid out like x; the stride of a dimension of size 1 addresses nothing
+            assert [q for n, q in zip(sizes, out.stride()) if n > 1] == [q for n, q in zip(sizes, place(t["x"]).stride()) if n > 1]
+    with torch.no_grad():
+        out, _ = sequence.residual_norm(**{k: place(v) for k, v in t.items()}, activation="sigmoid")
+        assert torch.equal(out, place(flat[0][0]))
+    # one gate row for all, which any order suits, and the gradient that torch hands in with stride 0
+    row = t["gate"][:1].expand(R, D)
+    want = sequence.residual_norm(t["x"], t["y"], t["weight"], gate=row)
+    x = place(t["x"]).detach().requires_grad_(True)
+    got = sequence.residual_norm(x, place(t["y"]), t["weight"], gate=t["gate"][0].expand(*sizes, D))
+    assert torch.equal(got, place(want))
+    got.sum().backward()
+    assert (x.grad == 1).all()
+
+
+def test_a_block_on_a_rollout_kept_by_environment():
+    """norm -> recurrence -> gated norm as on the rollout kept by steps, up to the order of the roundings: T steps and two norms
+    of at most 100 u each on either side."""
+    T, N, D = 60, 9, 40
+    x, p, state, reset, heads = block_inputs(T, N, D, seed=702)
+    want = block_pass(x, p, state, reset, heads)
+
+    def by_env(t):
+        return t.detach().transpose(0, 1).contiguous().transpose(0, 1)
+
+    for d in (heads, [by_env(h) for h in heads]):
+        got = block_pass(by_env(x), {k: v.detach() for k, v in p.items()}, state.detach(), reset, d)
+        assert got[0].stride() == by_env(x).stride() and got[1].stride() == by_env(x).stride()
+        for a, b in zip(want, got):
+            assert float((a - b).abs().max()) <= 2 * (T + 2) * 100 * S.U * float(a.abs().max())
+
+
+def test_orders_that_do_not_agree_are_refused():
+    x, y, w = torch.zeros(4, 5, 6, device=DEV), torch.zeros(5, 4, 6, device=DEV).transpose(0, 1), torch.ones(6, device=DEV)
+    for a, b in ((x, y), (y, x)):
+        with pytest.raises(ValueError, match="evenly spaced"):
+            sequence.residual_norm(a, b, w)
+        with pytest.raises(ValueError, match="evenly spaced"):
+            sequence.residual_norm(a, a, w, gate=b)
+    with pytest.raises(ValueError, match="evenly spaced"):
+        sequence.rms_norm(torch.zeros(5, 8, 6, device=DEV)[:, ::2].transpose(0, 1)[:, ::2], w)
+    with pytest.raises(ValueError, match="expected shape"):
+        sequence.residual_norm(y, torch.zeros((), device=DEV), w)
+    with pytest.raises(ValueError, match="expected shape"):
+        sequence.residual_norm(y, torch.zeros(6, device=DEV), w)
