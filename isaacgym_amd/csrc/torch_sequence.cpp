@@ -528,7 +528,12 @@ std::pair<Tensor, Tensor> run_norm(const Tensor &x, const Tensor &y, const Tenso
     return {out, next};
 }
 
-Tensor packed_rows(const Tensor &t) { return !t.defined() || t.is_contiguous() ? t : t.contiguous(); }
+// a gradient as the kernels can read it: copied only where its rows are not evenly spaced or its columns not adjacent
+Tensor readable_rows(const Tensor &t)
+{
+    int64_t stride;
+    return !t.defined() || (adjacent(t) && even_rows(t, stride)) ? t : t.contiguous();
+}
 
 struct BlockNorm : torch::autograd::Function<BlockNorm> {
     static variable_list forward(AutogradContext *ctx, const Tensor &x, const OptTensor &y_, const OptTensor &weight_,
@@ -570,7 +575,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         const Parameters p = {saved[3], saved[4], saved[5]};
         const bool block = p.weight.defined(), behind = p.next_weight.defined(), codes = saved.size() > 7;
         const Tensor given_out = block ? grads[0] : Tensor();
-        const Tensor d_out = packed_rows(given_out), d_next = packed_rows(behind ? grads.back() : Tensor());
+        const Tensor d_out = readable_rows(given_out), d_next = readable_rows(behind ? grads.back() : Tensor());
         if (!d_out.defined() && !d_next.defined()) return result;
         const Tensor &like = d_out.defined() ? d_out : d_next;
         c10::DeviceGuard guard(like.device());

@@ -85,3 +85,26 @@ def test_orders_that_do_not_agree_are_refused():
         sequence.residual_norm(y, torch.zeros((), device=DEV), w)
     with pytest.raises(ValueError, match="expected shape"):
         sequence.residual_norm(y, torch.zeros(6, device=DEV), w)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradients_that_are_views_of_wider_rows_are_read_in_place(dtype):
+    """The columns of a wider gradient, every second row of a longer one, one row for all: the same bits as of a copy, and no copy
+    is made."""
+    R, D = 16384, 250
+    t, do, dn = norm_inputs(R, D, dtype, 703, spread=False)
+    leaves = {k: v.to(DEV).requires_grad_(True) for k, v in t.items()}
+    wide = torch.full((2 * R, D + 9), float("nan"), dtype=dtype, device=DEV)
+    wide[::2, 5:5 + D] = do.to(DEV)
+    rows = (wide[::2, 5:5 + D], dn.to(DEV)[:1].expand(R, D))
+    packed = [h.contiguous() for h in rows]
+    outs = sequence.residual_norm(**leaves)
+    want = torch.autograd.grad(outs, list(leaves.values()), packed, retain_graph=True)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    start = torch.cuda.memory_allocated()
+    got = torch.autograd.grad(outs, list(leaves.values()), rows)
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+    # the gradients of x, y and gate and 2 x 768 rows of fp32 sums, less than a fourth array
+    assert torch.cuda.max_memory_allocated() - start < 4 * R * D * outs[0].element_size()
