@@ -1136,7 +1136,7 @@ int igx_linear_recurrence_backward_with_rest(const igx_recurrence *r, const igx_
  *     out  = x + scale * act(gate) * (rms(y) * weight)      behind a block whose output is y      (y given)
  *     next = rms(out) * next_weight                         in front of the next one              (next_weight given)
  * with out = x where y is NULL (a norm in front of the first block), scale and gate 1 where NULL.  Statistics and the
- * whole row's arithmetic are fp32, `next` is computed from the unrounded out, every result is rounded once.
+ * whole row's arithmetic are fp32 (so a row's sum of squares has to be representable), `next` is computed from the unrounded out, every result is rounded once.
  * Checkpoints (optional outputs of the forward call): the 8-bit codes of y and gate - of x where y is NULL - in the
  * form of igx_pack8, for a backward call that has the codes in place of those arrays.  A gate is limited before it
  * is coded: to >= -16 for the SiLU, to within +-16 for the sigmoid. */
@@ -1174,8 +1174,9 @@ int igx_block_norm_forward(const igx_block_norm *b, igx_stream_t stream);
 
 /* Gradients.  b holds the forward call's arguments with y_inv_rms (with y) and out_inv_rms (with next_weight) as the
  * forward call wrote them; out and next are not read, x only with next_weight.  Where y8 (gate8) is given it is read in
- * place of y (gate; x where y is NULL): the gradients are then those at the values the codes stand for.  y (gate) itself
- * says which of the operator's parts exist, so with codes it must still be non-NULL; it is not read.
+ * place of y (gate; x where y is NULL): the gradients are then those at the values the codes stand for, with the inverse
+ * roots that the forward call took from the arrays themselves.  y (gate) itself says which of the operator's parts exist,
+ * so with codes it must still be non-NULL; it is not read.
  * Column sums are added in a fixed order: the same call gives the same bits. */
 typedef struct igx_block_norm_grad {
     const void *d_out;   /* elements [rows, width] at d_out_stride; NULL = zeros */

@@ -2,7 +2,9 @@
 //     out = x + scale * act(gate) * (rms(y) * weight),   next = rms(out) * next_weight
 //
 // Row-wise and bound by HBM: forward moves up to 5 elements per (row, column), backward up to 8, a few dozen operations
-// each (2^20 x 256 bf16 with gate, scale and next: 526 us forward, 831 backward, 5.1 TB/s; the norm alone 165 us, 6.5 TB/s).
+// each (2^20 x 256 bf16 with gate, scale and next: 522 us forward, 5.1 TB/s, 815 backward, 5.3 TB/s; the norm alone 170 us
+// forward, 6.3 TB/s, and 273 backward, 5.9 TB/s, through 8-bit codes 226 and 253).  All times here are device times of graph
+// replays on one set of buffers, backward with the column sums; where the buffers lie moves them by up to 15 %.
 // A row stays in the registers of the lanes that loaded it - 16 bytes a lane, 8 to 64 lanes of one wave or the waves of a
 // whole workgroup, whichever the width fills - so every array is read and written once and the statistics need no second
 // pass.  Groups of lanes walk over the rows, which keeps the parameter vectors in registers and lets backward add up the
@@ -16,7 +18,7 @@ namespace {
 // Gates as their codes hold them: no further out than +-16, so that one that is shut by a very low value does not take the
 // other 63 of its group their scale.  Beyond it the activations are off by less than 16 exp(-16) < 2^-19, where a code of
 // such a group has steps of 16 / 127.  NaN stays.  One instruction an element, with a branch for the sigmoid's upper end (the
-// whole kernel on 131 072 x 512 bf16: 156 us, 154 without limits, 161 with two instructions or selects).
+// whole kernel on 131 072 x 512 bf16: 177 us, 172 without limits).
 template <int V, int K> __device__ __forceinline__ void limit_gates(const float (&z)[K][V], int act, float (&g)[K][V])
 {
     const float most = 16.0f, lowest = act == IGX_GATE_NONE ? -__builtin_inff() : -most;
@@ -241,9 +243,9 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(SumArgs a)
 }
 
 // Workgroups: as many as run at a time, which walk over the rows - more would start when the first are done and leave most
-// of the card idle at the end (backward of 2^20 x 256 bf16: 829 us with the 12 waves a CU holds, 956 with 16).  Without a
+// of the card idle at the end (backward of 2^20 x 256 bf16: 815 us with the 12 waves a CU holds, 943 with 16).  Without a
 // block (waves 0) a lane keeps only the norm's weight, and a workgroup for every group of rows is faster: 2^20 x 256 fp32
-// 335 us, 370 walking.
+// 341 us, 378 walking.
 int64_t blocks_for(int64_t rows, int64_t width, int dtype, int64_t waves_per_cu)
 {
     const int lanes = lanes_for(width, dtype, waves_per_cu == 0);
@@ -254,8 +256,8 @@ int64_t blocks_for(int64_t rows, int64_t width, int dtype, int64_t waves_per_cu)
 }
 constexpr int64_t kForwardWaves = 16, kBackwardWaves = 12;
 
-// Does the call move more than the 256 MB that the last level of cache holds?  (2^20 x 256 bf16, forward and backward: 1 362 us
-// past the caches, 1 431 through them; 16 411 x 211 fp32: 49 and 43.)
+// Does the call move more than the 256 MB that the last level of cache holds?  (2^20 x 256 bf16, forward and backward: 1 340 us
+// past the caches, 1 425 through them; 16 411 x 211 fp32: 48 and 45.)
 bool beyond_cache(const igx_block_norm *b, int64_t arrays)
 {
     return arrays * b->rows * b->width * element_size(b->dtype) > (int64_t)256 << 20;

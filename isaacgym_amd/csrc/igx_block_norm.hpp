@@ -8,9 +8,9 @@ namespace igx {
 
 constexpr int kNormBlock = 256;   // of the kernels whose row fits one wave
 
-// 16-byte vectors of a row in a lane.  One, which leaves registers for enough waves (16 411 x 211 fp32 forward and backward: 38 us,
-// 41 with two) - but two where the forward kernel has a single array to read and its norm's weight to hold (2^20 x 64 fp32: 84 us,
-// 94 with one), and where 1024 lanes need them for the widest rows.
+// 16-byte vectors of a row in a lane.  One, which leaves registers for enough waves (2^20 x 256 bf16 forward and backward with the
+// column sums: 1 340 us, 1 545 with two; 16 411 x 211 fp32: 45, 46) - but two where the forward kernel has a single array to read
+// and its norm's weight to hold (2^20 x 64 fp32: 85 us, 94 with one), and where 1024 lanes need them for the widest rows.
 constexpr int vectors_of(bool alone, bool largest, int vec) { return alone || (largest && vec == 4) ? 2 : 1; }
 
 struct NormArgs {

@@ -76,8 +76,8 @@ template <typename T, int V> __device__ __forceinline__ void store_step(const Re
 // in bf16, 2^13 in fp16) and rounded to that: value and sum differ by at most 2^-7 of the half step that out is off by, and not
 // at all where out is the value.  fp16's subnormals, whose steps are wider, gain less.  Beside inf and NaN it is 0.  8 bits, not
 // the 16 that would be fp32: what is computed from the sum is itself rounded to T, a step 2^8 times as wide.  They take half
-// of an array's bytes each way and go through the caches even where the arrays go past them (32 x 65 536 x 64 bf16, forward and
-// backward: 427 us, 469 past the caches, 398 without codes).
+// of an array's bytes each way and go through the caches even where the arrays go past them (32 x 65 536 x 64 bf16, a training
+// pass: 427 us, 469 past the caches, 398 without codes).
 template <typename T> constexpr int kRestShift = sizeof(T) == 4 ? 0 : std::is_same<T, __bf16>::value ? 8 : 5;
 
 template <typename T> __device__ __forceinline__ int rest_code(float h)
@@ -148,10 +148,10 @@ template <int V, int FL> struct LaneFlags {
     }
 };
 
-// Steps whose loads a lane has in flight, by the groups that share a workgroup's channels (measured, forward + backward):
-// with a lane for all steps 1, since thousands of waves are in flight and fewer rows [N, D] open at a time suit HBM better
-// (32 x 65 536 x 64 bf16: 406 us with 1, 415 with 2, 431 with 4, 475 with 8); with four groups 2 (32 x 4 096 x 64 fp32:
-// 49 us, 51 with 4, 55 with 8); with sixteen, where waves are few, 8 (2 048 x 16 x 1 024 bf16: 172 us, 237 with 4); with
+// Steps whose loads a lane has in flight, by the groups that share a workgroup's channels (device time of forward and
+// backward): with a lane for all steps 1, since thousands of waves are in flight and fewer rows [N, D] open at a time suit
+// HBM better (32 x 65 536 x 64 bf16: 387 us with 1, 408 with 2, 413 with 4, 467 with 8); with four groups 2 (32 x 4 096 x 64
+// fp32: 49 us, 50 with 4, 53 with 8); with sixteen, where waves are few, 8 (256 x 16 x 1 024 bf16: 27 us, 34 with 4); with
 // sixty-four, whose 16 waves leave 128 registers each, 4.
 constexpr int steps_of(int seg) { return seg == 1 ? 1 : seg == 4 ? 2 : seg == 16 ? 8 : 4; }
 
@@ -376,7 +376,7 @@ template <int V> __device__ __forceinline__ void store_end(const RecArgs &a, con
 }
 
 // enough channels: a lane walks all the steps.  REST is an argument of the template here, for a branch around its loads costs
-// calls without it 2 % (32 x 65 536 x 64 bf16, forward and backward: 399 us, 408 with the branch).
+// calls without it 2 % (32 x 65 536 x 64 bf16, a training pass: 398 us, 408 with the branch).
 template <typename T, int V, int FL, bool BACKWARD, bool REST>
 __global__ __launch_bounds__(kRecBlock) void recurrence_kernel(RecArgs a)
 {

@@ -2,7 +2,8 @@
 //
 // The lanes of one group take 32 bytes of its elements each and agree on the largest magnitude by exchanging it within the
 // wave, so the elements are read once and stay in registers: e + 1 + 4/64 bytes an element each way, bound by HBM (2^20 x 256
-// bf16: 155 us to pack, 5.3 TB/s, 137 to unpack, 6.0 TB/s; with 16 bytes a lane 176 and 135).
+// bf16: 146 us to pack, 5.6 TB/s, 144 to unpack, 5.7 TB/s, with 16 bytes a lane 172 and 143; 2^20 x 211 fp32: 199 and 219, with
+// 16 bytes a lane 267 and 268).
 #include "igx_seq.hpp"
 
 namespace igx {

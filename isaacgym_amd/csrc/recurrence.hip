@@ -3,9 +3,9 @@
 // Channels are independent and adjacent in memory, so a lane owns a vector of channels (16 bytes) and walks the steps with
 // the carried value in fp32 registers.  A call moves 3 elements per (t, n, d) forward and 5 backward and does 2 - 3
 // operations on each: HBM bounds it where there are enough channels to fill the card (32 x 65 536 x 64 bf16 forward and
-// backward: 2.25 GB in 400 us, 5.6 TB/s; one step of 262 144 x 64 with its fp32 state: 235 MB in 38 us, 6.2 TB/s).  Arrays
-// that nothing reads again soon go past the caches' replacement (non-temporal; loads too where a lane walks alone: 400 us
-// against 427).
+// backward: 2.25 GB in 387 us, 5.8 TB/s; one step of 262 144 x 64 with its fp32 state: 235 MB in 40 us, 5.9 TB/s).  Arrays
+// that nothing reads again soon go past the caches' replacement (non-temporal; loads too where a lane walks alone: 387 us
+// against 438).  All times here are device times of graph replays on one set of buffers.
 //
 // With fewer channels the time is split, for the recurrence is a composition of maps h -> A h + B that is associative:
 //   - within a workgroup SEG groups of lanes take a few consecutive steps each of the same channels, reduce them to
@@ -15,7 +15,7 @@
 //     the second composes the spans before its own, while its first steps are on their way.  That reads gate and inp twice
 //     (the second time mostly from the caches), so it is done only where the channels alone leave CUs without work: 8 192
 //     steps of 512 channels in bf16 take 17 us forward and 20 us backward, bound by the latency of two launches and the
-//     exchange (a lane for every 8 channels needs 7 565 us).
+//     exchange (a lane for every 8 channels needs 10 600 us).
 #include "igx_recurrence.hpp"
 
 namespace igx {
@@ -47,14 +47,14 @@ int check(const igx_recurrence *r, const char *who)
 bool follows(const igx_recurrence *r, int64_t stride_n) { return r->envs == 1 || stride_n == r->width; }
 
 // How the time is split (both sides measured, forward + backward).  131 072 lanes and more walk the steps alone (64 x 16 384 x
-// 64 fp32: 364 us, 452 in four groups).  With fewer, four groups share a workgroup's steps (32 x 4 096 x 64 fp32, 65 536
-// lanes: 49 us, 82 alone), below 16 384 lanes sixteen.  A sequence goes to several workgroups in spans only where the
-// channels fill fewer than 256 of them, one for each CU (1 024 x 64 x 256 fp32 fills 256: 118 us in one span, 153 in two,
-// for gate and inp are then read twice); 512 workgroups in all are enough.  Where they fill 256 and the sequence is long,
-// sixty-four groups keep a CU's waves busy (2 048 x 16 x 1 024 bf16: 137 us, 164 in sixteen; 1 024 x 64 x 256 fp32: 105, 139),
-// unless a lane needs more than one flag a step, which takes the registers (1 000 x 200 x 105 bf16: 234, 166 in sixteen).
+// 64 fp32: 367 us, 441 in four groups).  With fewer, four groups share a workgroup's steps (32 x 4 096 x 64 fp32, 65 536
+// lanes: 49 us, 89 alone), below 16 384 lanes sixteen.  A sequence goes to several workgroups in spans only where the
+// channels fill fewer than 256 of them, one for each CU (300 x 64 x 256 fp32 fills 256: 45 us in one span, 64 in two, for
+// gate and inp are then read twice); 512 workgroups in all are enough.  Where they fill 256 and the sequence is long,
+// sixty-four groups keep a CU's waves busy (2 048 x 16 x 1 024 bf16: 134 us, 173 in sixteen; 1 024 x 64 x 256 fp32: 107, 123),
+// unless a lane needs more than one flag a step, which takes the registers (1 000 x 200 x 105 bf16: 263, 207 in sixteen).
 // Rollouts kept environment by environment have their next steps next to each other: four groups, however many lanes there
-// are, and the caches, which complete the lines that narrow rows share (32 x 20 000 x 60 fp32: 288 us, 474 with lanes that walk
+// are, and the caches, which complete the lines that narrow rows share (32 x 20 000 x 60 fp32: 290 us, 481 with lanes that walk
 // alone past the caches).
 void split(Plan &p)
 {
@@ -107,7 +107,7 @@ void make_plan(const igx_recurrence *r, const igx_recurrence_grad *g, const igx_
         split(p);
     };
     lanes(r->dtype == IGX_F32 ? 4 : 8);
-    if (r->dtype != IGX_F32 && p.seg > 1) {  // too few lanes: twice as many with half the bytes (8 192 x 1 x 512 bf16: 64 -> 43 us)
+    if (r->dtype != IGX_F32 && p.seg > 1) {  // too few lanes: twice as many with half the bytes (8 192 x 1 x 512 bf16: 37 us, 51 with 8 channels)
         lanes(4);
         if (p.seg == 1) p.seg = 4;
     }

@@ -912,7 +912,7 @@ def block_norm_backward(like, x=None, y=None, weight=None, gate=None, scale=None
                         d_scale=None, d_next_weight=None):
     """The gradients of block_norm (igx_block_norm_backward): those given are filled in.  like: a [..., width] tensor of
     the rows' shape, type and device.  codes in place of y and gate (of x in a call without a block): the gradients at the
-    values the codes stand for."""
+    values the codes stand for, with inv_rms as block_norm filled it."""
     b = _block_norm(like, weight, gate, scale, next_weight, inv_rms, codes, activation, eps)
     shape, dtype = like.shape, like.dtype
     b.x, b.x_stride = _row_array(x, "x", shape, like)

@@ -87,9 +87,9 @@ def residual_norm(x, y, weight, gate=None, scale=None, next_weight=None, activat
     x, y, gate [..., D] of one shape and type, their rows evenly spaced in one order of the dimensions that all three
     share and in which the results are laid out; weight, scale, next_weight [D] float32; activation of the gate: "silu",
     "sigmoid" or "none".  Differentiable (once) in all of them.  checkpoint=True: y and gate are kept for the backward pass
-    as 8-bit codes (`pack8`) and the gradients are those at the values the codes stand for; x is kept as it is.  There a
-    gate counts as >= -16 with "silu" and within +-16 with "sigmoid", so that one that is shut by a very low value leaves
-    the other 63 of its group their precision."""
+    as 8-bit codes (`pack8`) and the gradients are those at the values the codes stand for, with the rows' statistics of
+    the forward pass; x is kept as it is.  There a gate counts as >= -16 with "silu" and within +-16 with "sigmoid", so
+    that one that is shut by a very low value leaves the other 63 of its group their precision."""
     out, after = _native().block_norm(x, y, weight, gate, scale, next_weight, activation, float(eps), bool(checkpoint))
     return out if next_weight is None else (out, after)
 
