@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 
 # one row; fewer row groups than workgroups, just as many, one more; several rounds with an odd end; whole workgroups on a row;
 # past the caches
-SHAPES = [(1, 64), (3071, 256), (3073, 256), (24577, 8), (40001, 24), (300007, 10), (20011, 200), (9001, 600), (1537, 2046),
+SHAPES = [(1, 64), (6143, 128), (6145, 128), (24577, 8), (40001, 24), (300007, 10), (20011, 200), (9001, 600), (1537, 2046),
           (3001, 4100), (700, 8192), (16411, 211), (1 << 18, 200)]
 
 

@@ -62,7 +62,7 @@ def test_views_that_a_rollout_is_made_of():
 
 
 def test_it_is_quick_for_large_tensors():
-    """Storage without memory behind it (a meta tensor has no addresses): strides of 2^20 rows, interleaved in every way."""
+    """Views of half a million rows that lie between each other's rows, in every order of the strides: no row is visited."""
     big = torch.zeros(1 << 22, dtype=torch.uint8)
     views = [big.as_strided((1 << 10, 1 << 9, 3), (4096, 8, 1), k) for k in (0, 3, 4096 * 0 + 4)]
     views += [big.as_strided((511, 1 << 9, 3), (8192, 8, 1), 4096 + 3), big.as_strided((1 << 9, 1 << 10, 3), (8, 4096, 1), 5)]
